@@ -380,6 +380,127 @@ int vy_moe_combine(const float* contrib, const void* expert_ids, int32_t ids_dty
                    int64_t n_tokens, int32_t top_k, int64_t hidden, float* out,
                    int64_t out_row_stride, void* stream);
 
+/* ── dense layers: gated feed-forward blocks and 8-bit integer linears ──────────────────────
+ *
+ * The layers of a MoE model that are not packed int4: dense blocks, shared experts kept in 16 bits,
+ * linears in the "int-quantized" 8-bit form.  No counterpart in the reference's packed-expert path
+ * (a dense entry leaves it there).  Conventions as above; `flags` (device int32, may be NULL) is
+ * ORed with VY_FLAG_TIMEOUT / VY_FLAG_DRAIN when a bounded device-side wait runs out.
+ */
+enum vy_activation {
+    VY_ACT_SILU = 0,     /* g / (1 + exp(-g)) */
+    VY_ACT_GELU_TANH = 1 /* g (1 + tanh(sqrt(2/pi) (g + 0.044715 g^3))) / 2 */
+};
+
+typedef struct vy_ffn_call {
+    int32_t act_dtype;  /* VY_BF16 or VY_F16: x, the weights, out and all gradients */
+    int32_t activation; /* vy_activation */
+    int64_t n_tokens;
+    int32_t hidden, inter;      /* multiples of 8 */
+    const void* x;              /* [n_tokens, hidden], 16-byte aligned rows */
+    int64_t x_row_stride;       /* elements, a multiple of 8 */
+    const void *w_gate, *w_up;  /* [inter, hidden], contiguous */
+    const void* w_down;         /* [hidden, inter], contiguous */
+    void* out;                  /* forward: [n_tokens, hidden] */
+    int64_t out_row_stride;     /* a multiple of 8 */
+    float* saved;               /* g and u in fp32, vy_gated_ffn_saved_floats() of them: written by
+                                   the forward call when not NULL, read by the backward call */
+    void* workspace;
+    size_t workspace_bytes;
+    int32_t* flags;
+    /* backward only; a NULL gradient is not computed */
+    const void* d_out;          /* [n_tokens, hidden] */
+    int64_t d_out_row_stride;   /* a multiple of 8 */
+    void* d_x;                  /* [n_tokens, hidden] */
+    int64_t d_x_row_stride;     /* a multiple of 8 */
+    void *d_w_gate, *d_w_up;    /* [inter, hidden], contiguous */
+    void* d_w_down;             /* [hidden, inter], contiguous */
+} vy_ffn_call;
+
+/* Floats of `saved` for a block of this size. */
+int64_t vy_gated_ffn_saved_floats(int64_t n_tokens, int32_t inter);
+/* Bytes of workspace for the forward (backward = 0) or backward (1) call. */
+size_t vy_gated_ffn_workspace_size(const vy_ffn_call* call, int32_t backward);
+
+/*
+ * out = (act(x Wg^T) * (x Wu^T)) Wd^T with fp32 sums; g and u stay in fp32, the hidden row
+ * h = act(g) * u is rounded once to the activation type (it is a tensor-core operand of the second
+ * product), and so is out.
+ */
+int vy_gated_ffn_forward(const vy_ffn_call* call, void* stream);
+
+/*
+ * The gradients of that block from d_out and the forward call's `saved`:
+ *   dh = d_out Wd;  dg = dh * u * act'(g);  du = dh * act(g)
+ *   d_x = dg Wg + du Wu;  d_w_gate = dg^T x;  d_w_up = du^T x;  d_w_down = d_out^T h
+ * fp32 sums; dg, du and h are rounded once to the activation type (tensor-core operands).
+ */
+int vy_gated_ffn_backward(const vy_ffn_call* call, void* stream);
+
+/*
+ * One int8 scale per row: scale = fl32(amax(|x|) / 127); code = the nearest integer of the exact
+ * quotient x / scale, ties to even, in [-127, 127].  A zero row (or one whose scale underflows to
+ * zero) has scale 0 or the underflow's and codes 0; a row holding an infinity or NaN has scale NaN
+ * and codes 0, so a product with it is NaN in that row alone.  x: VY_BF16 / VY_F16 / VY_F32, any
+ * row length and stride; codes [rows, cols] contiguous.
+ */
+int vy_int8_quantize(const void* x, int32_t x_dtype, int64_t x_row_stride, int64_t rows, int64_t cols,
+                     int8_t* codes, float* scales, void* stream);
+
+typedef struct vy_int8_linear_call {
+    int64_t n_tokens;
+    int32_t k, n;              /* k: a multiple of 16, below 131072 (an int32 sum cannot overflow) */
+    const int8_t* codes;       /* [n_tokens, k], 16-byte aligned rows */
+    int64_t codes_row_stride;  /* a multiple of 16 */
+    const float* scales;       /* [n_tokens] */
+    const int8_t* weight;      /* [n, k], contiguous */
+    const float* weight_scales; /* [n] */
+    const void* bias;          /* [n] or NULL */
+    int32_t bias_dtype;        /* VY_BF16 / VY_F16 / VY_F32 */
+    int32_t out_dtype;         /* VY_BF16 / VY_F16 / VY_F32 */
+    void* out;                 /* [n_tokens, n] */
+    int64_t out_row_stride;
+    void* workspace;           /* vy_int8_linear_workspace_size() */
+    size_t workspace_bytes;
+    int32_t* flags;
+} vy_int8_linear_call;
+
+size_t vy_int8_linear_workspace_size(const vy_int8_linear_call* call);
+
+/*
+ * out[t, n] = (sum_k codes[t, k] * weight[n, k]) * scales[t] * weight_scales[n] (+ bias[n]): the
+ * sum exact in int32, then one rounding to fp32 and one per product and sum in that order, then
+ * one to the output type.
+ */
+int vy_int8_linear(const vy_int8_linear_call* call, void* stream);
+
+typedef struct vy_int8_ffn_call {
+    int32_t act_dtype;  /* VY_BF16 or VY_F16: x and out */
+    int32_t activation; /* vy_activation */
+    int64_t n_tokens;
+    int32_t hidden, inter;      /* multiples of 16, below 131072 */
+    const void* x;              /* [n_tokens, hidden] */
+    int64_t x_row_stride;
+    const int8_t *w_gate, *w_up;         /* [inter, hidden], contiguous */
+    const int8_t* w_down;                /* [hidden, inter], contiguous */
+    const float *gate_scales, *up_scales; /* [inter] */
+    const float* down_scales;            /* [hidden] */
+    void* out;                  /* [n_tokens, hidden] */
+    int64_t out_row_stride;
+    void* workspace;
+    size_t workspace_bytes;
+    int32_t* flags;
+} vy_int8_ffn_call;
+
+size_t vy_int8_gated_ffn_workspace_size(const vy_int8_ffn_call* call);
+
+/*
+ * The gated block on int8 weights: x quantised per token (vy_int8_quantize), g and u as
+ * vy_int8_linear's fp32 sums, h = act(g) * u kept in fp32 and quantised per token from there (a
+ * rounding before the quantisation would move codes), out as vy_int8_linear's.
+ */
+int vy_int8_gated_ffn(const vy_int8_ffn_call* call, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

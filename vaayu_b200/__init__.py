@@ -9,6 +9,7 @@ from .arena import ExpertArena
 from .block_scaled import (dequantize_block_scaled, dequantize_fp4_block_scaled, fp4_gemv,
                            fp8_gemv)
 from .checkpoint import Checkpoint, group_packed_tensors_by_weight, packed_roles_complete
+from .dense import gated_ffn, int8_gated_ffn, int8_linear, quantize_int8
 from .moe_patch import (accumulate_expert_outputs, build_expert_blob, compute_expert_dispatch,
                         dequantize_expert_blob, dequantize_expert_weights,
                         dequantize_packed_weight, expert_weights_from_entry, route_experts,
@@ -24,8 +25,10 @@ __all__ = [
     "build_expert_blob", "combine", "compute_expert_dispatch", "dequantize_block_scaled",
     "dequantize_expert_blob", "dequantize_expert_weights", "dequantize_fp4_block_scaled",
     "dequantize_packed_weight", "expert_weights_from_entry", "fp4_gemv", "fp8_gemv",
-    "group_packed_tensors_by_weight", "install_packed_expert_kernels", "moe_forward",
-    "moe_forward_with_shared", "moe_workspace_bytes", "packed_roles_complete", "shared_expert_forward",
+    "gated_ffn", "group_packed_tensors_by_weight", "install_packed_expert_kernels", "int8_gated_ffn",
+    "int8_linear", "moe_forward",
+    "moe_forward_with_shared", "moe_workspace_bytes", "packed_roles_complete", "quantize_int8",
+    "shared_expert_forward",
     "packed_experts_decode", "packed_experts_decode_graphed", "packed_experts_prefill",
     "route_experts", "route_permute", "topk_softmax", "unpack_int32_to_int8",
 ]

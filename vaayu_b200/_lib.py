@@ -43,6 +43,31 @@ class MoeCall(ctypes.Structure):
                 ("shared_last", I32T), ("k_splits", I32T), ("result", P), ("result_row_stride", I64T)]
 
 
+class FfnCall(ctypes.Structure):
+    """vy_ffn_call."""
+    _fields_ = [("act_dtype", I32T), ("activation", I32T), ("n_tokens", I64T), ("hidden", I32T),
+                ("inter", I32T), ("x", P), ("x_row_stride", I64T), ("w_gate", P), ("w_up", P),
+                ("w_down", P), ("out", P), ("out_row_stride", I64T), ("saved", P), ("workspace", P),
+                ("workspace_bytes", SZ), ("flags", P), ("d_out", P), ("d_out_row_stride", I64T),
+                ("d_x", P), ("d_x_row_stride", I64T), ("d_w_gate", P), ("d_w_up", P), ("d_w_down", P)]
+
+
+class Int8LinearCall(ctypes.Structure):
+    """vy_int8_linear_call."""
+    _fields_ = [("n_tokens", I64T), ("k", I32T), ("n", I32T), ("codes", P), ("codes_row_stride", I64T),
+                ("scales", P), ("weight", P), ("weight_scales", P), ("bias", P), ("bias_dtype", I32T),
+                ("out_dtype", I32T), ("out", P), ("out_row_stride", I64T), ("workspace", P),
+                ("workspace_bytes", SZ), ("flags", P)]
+
+
+class Int8FfnCall(ctypes.Structure):
+    """vy_int8_ffn_call."""
+    _fields_ = [("act_dtype", I32T), ("activation", I32T), ("n_tokens", I64T), ("hidden", I32T),
+                ("inter", I32T), ("x", P), ("x_row_stride", I64T), ("w_gate", P), ("w_up", P),
+                ("w_down", P), ("gate_scales", P), ("up_scales", P), ("down_scales", P), ("out", P),
+                ("out_row_stride", I64T), ("workspace", P), ("workspace_bytes", SZ), ("flags", P)]
+
+
 # name -> (restype, argtypes); every symbol include/vaayu_b200.h declares
 SIGNATURES = {
     "vy_last_error": (ctypes.c_char_p, []),
@@ -67,6 +92,15 @@ SIGNATURES = {
     "vy_ep_combine": (ctypes.c_int, [P, P, P, I32T, I64T, I64T, I32T, I64T, P, I64T, P]),
     "vy_moe_error_flags": (ctypes.c_int, [ctypes.POINTER(MoeCall), I32T, P, P]),
     "vy_selftest_bounded_wait": (ctypes.c_int, [I32T, I64T, P, P]),
+    "vy_gated_ffn_saved_floats": (I64T, [I64T, I32T]),
+    "vy_gated_ffn_workspace_size": (SZ, [ctypes.POINTER(FfnCall), I32T]),
+    "vy_gated_ffn_forward": (ctypes.c_int, [ctypes.POINTER(FfnCall), P]),
+    "vy_gated_ffn_backward": (ctypes.c_int, [ctypes.POINTER(FfnCall), P]),
+    "vy_int8_quantize": (ctypes.c_int, [P, I32T, I64T, I64T, I64T, P, P, P]),
+    "vy_int8_linear_workspace_size": (SZ, [ctypes.POINTER(Int8LinearCall)]),
+    "vy_int8_linear": (ctypes.c_int, [ctypes.POINTER(Int8LinearCall), P]),
+    "vy_int8_gated_ffn_workspace_size": (SZ, [ctypes.POINTER(Int8FfnCall)]),
+    "vy_int8_gated_ffn": (ctypes.c_int, [ctypes.POINTER(Int8FfnCall), P]),
 }
 
 _LIB = None

@@ -1,0 +1,117 @@
+// vy_dense.cuh -- what the dense 16-bit and int8 operators share: activations, epilogue
+// parameters, vector stores.
+#pragma once
+
+#include "vy_umma.cuh"
+
+namespace vy {
+
+// ── activations of a gated block and their derivatives (fp32) ───────────────────────────────
+
+__device__ __forceinline__ float gelu_inner(float g) {
+    // tanh is +-1 to the last bit well inside +-16; the clamp keeps g^3 finite
+    const float c = fminf(fmaxf(g, -16.f), 16.f);
+    return 0.7978845608028654f * (c + 0.044715f * c * c * c);
+}
+// silu(g) = g / (1 + e^-g); gelu_tanh(g) = g (1 + tanh(sqrt(2/pi) (g + 0.044715 g^3))) / 2
+__device__ __forceinline__ float gate_act(float g, int act) {
+    if (act == VY_ACT_SILU) return g / (1.f + expf(-g));
+    return 0.5f * g * (1.f + tanhf(gelu_inner(g)));
+}
+// (value, derivative)
+__device__ __forceinline__ float2 gate_act_grad(float g, int act) {
+    if (act == VY_ACT_SILU) {
+        const float s = 1.f / (1.f + expf(-g));
+        return make_float2(g * s, s * (1.f + g * (1.f - s)));
+    }
+    const float t = tanhf(gelu_inner(g));
+    const float c = fminf(fmaxf(g, -16.f), 16.f);
+    // beyond the clamp 1 - t^2 is zero, so the clamped factor beside it changes nothing
+    const float d = 0.5f * (1.f + t) + 0.5f * c * (1.f - t * t) * 0.7978845608028654f * (1.f + 0.134145f * c * c);
+    return make_float2(0.5f * g * (1.f + t), (g != g) ? g : d);
+}
+
+template <int ACT>
+__device__ __forceinline__ uint32_t pack_act(float lo, float hi) {
+    if constexpr (ACT == VY_BF16) {
+        __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+        return *reinterpret_cast<uint32_t*>(&v);
+    } else {
+        __half2 v = __floats2half2_rn(lo, hi);
+        return *reinterpret_cast<uint32_t*>(&v);
+    }
+}
+
+// 16 consecutive values of a row as 16-bit floats; `valid` of them (a multiple of 8) are stored.
+template <int ACT>
+__device__ __forceinline__ void store16(uint16_t* dst, const float (&v)[16], int valid) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        if (valid >= 8 * (h + 1)) {
+            uint4 o;
+            o.x = pack_act<ACT>(v[8 * h + 0], v[8 * h + 1]);
+            o.y = pack_act<ACT>(v[8 * h + 2], v[8 * h + 3]);
+            o.z = pack_act<ACT>(v[8 * h + 4], v[8 * h + 5]);
+            o.w = pack_act<ACT>(v[8 * h + 6], v[8 * h + 7]);
+            *reinterpret_cast<uint4*>(dst + 8 * h) = o;
+        }
+    }
+}
+
+__device__ __forceinline__ void store_as(void* p, int dtype, int64_t i, float v) {
+    switch (dtype) {
+        case VY_BF16: reinterpret_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v); break;
+        case VY_F16: reinterpret_cast<__half*>(p)[i] = __float2half_rn(v); break;
+        default: reinterpret_cast<float*>(p)[i] = v;
+    }
+}
+
+// Up to 16 consecutive values at element `at` of a row in `dtype`; vec: 16-byte stores are aligned
+// and `valid` is 16.
+__device__ __forceinline__ void store16_dyn(void* p, int dtype, int64_t at, const float (&v)[16], int valid, bool vec) {
+    if (vec && valid == 16) {
+        if (dtype == VY_BF16) {
+            store16<VY_BF16>(reinterpret_cast<uint16_t*>(p) + at, v, 16);
+        } else if (dtype == VY_F16) {
+            store16<VY_F16>(reinterpret_cast<uint16_t*>(p) + at, v, 16);
+        } else {
+            float4* d = reinterpret_cast<float4*>(reinterpret_cast<float*>(p) + at);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) d[q] = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+        }
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < 16; ++j)
+        if (j < valid) store_as(p, dtype, at + j, v[j]);
+}
+
+// What a GEMM's epilogue does with its sums.
+enum Epilogue {
+    EPI_STORE = 0,   // out = sum, in the activation type
+    EPI_GATE = 1,    // h = act(g) * u in the activation type; g and u kept in fp32 when `saved`
+    EPI_DGATE = 2,   // from dh, g, u: dg, du and h in the activation type
+    EPI_I8 = 3,      // out = (int32 sum * row scale) * column scale (+ bias)
+    EPI_I8GATE = 4   // h = act(g) * u in fp32, g and u scaled like EPI_I8
+};
+__host__ __device__ constexpr bool epi_is_gate(int e) { return e == EPI_GATE || e == EPI_I8GATE; }
+__host__ __device__ constexpr bool epi_is_i8(int e) { return e == EPI_I8 || e == EPI_I8GATE; }
+
+struct EpiParams {
+    void* out;               // rows = tokens (or weight rows of a weight gradient)
+    int64_t ldo;
+    int out_dtype;
+    int vec;                 // out rows take 16-byte stores
+    int act;                 // vy_activation
+    // g and u as [2][inter][ld_saved]: a column of the tile is contiguous over the tokens, so a
+    // warp (one token per lane) moves it in one 128-byte line both ways
+    float* saved;
+    int64_t ld_saved, saved_u;      // token stride, offset of u
+    uint16_t *dg, *du, *h;          // EPI_DGATE, rows `ldo` apart
+    const float* row_scale;
+    const float* col_scale[2];
+    const void* bias;
+    int bias_dtype;
+};
+
+}  // namespace vy

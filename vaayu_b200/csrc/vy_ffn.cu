@@ -1,0 +1,220 @@
+// vy_ffn.cu -- dense gated feed-forward block in bf16 / fp16, forward and backward.
+//
+//   forward   gate/up product with the activation in its epilogue -> h; down product
+//   backward  dh = dy Wd with the gate's derivative in its epilogue -> dg, du, h; then dx and the
+//             three weight gradients as one launch of four GEMMs
+//
+// Bounds.  Forward 6 T H I flops on 6 H I bytes of weights: HBM below about 250 tokens, the tensor
+// cores above.  Backward 12 T H I flops.
+#include "vy_tile.cuh"
+
+namespace vy {
+namespace {
+
+// Tokens of a column of `saved`: whole 128-byte lines of fp32.
+int64_t saved_ld(int64_t tokens) { return (tokens + 31) / 32 * 32; }
+
+size_t align256(size_t v) { return (v + 255) & ~size_t(255); }
+
+int64_t h_elems(const vy_ffn_call* c) { return c->n_tokens * int64_t(c->inter); }
+
+int check_ffn(const vy_ffn_call* c, bool backward) {
+    if (!c) return fail(VY_ERR_INVALID, "null call");
+    if (c->act_dtype != VY_BF16 && c->act_dtype != VY_F16)
+        return fail(VY_ERR_UNSUPPORTED, "activation dtype code %d (bf16 or fp16)", c->act_dtype);
+    if (c->activation != VY_ACT_SILU && c->activation != VY_ACT_GELU_TANH)
+        return fail(VY_ERR_UNSUPPORTED, "activation code %d", c->activation);
+    if (c->n_tokens < 0 || c->hidden <= 0 || c->inter <= 0)
+        return fail(VY_ERR_INVALID, "n_tokens %lld, hidden %d, inter %d", (long long)c->n_tokens, c->hidden, c->inter);
+    if (c->n_tokens > (int64_t(1) << 30)) return fail(VY_ERR_UNSUPPORTED, "n_tokens %lld", (long long)c->n_tokens);
+    if (c->hidden % 8 || c->inter % 8)
+        return fail(VY_ERR_UNSUPPORTED, "hidden %d and inter %d must be multiples of 8", c->hidden, c->inter);
+    const bool empty = c->n_tokens == 0;
+    const void* need[] = {empty ? c->w_gate : c->x, c->w_gate, c->w_up, c->w_down};
+    for (const void* q : need) {
+        if (!q) return fail(VY_ERR_INVALID, "null operand");
+        if (!aligned16(q)) return fail(VY_ERR_ALIGNMENT, "operands must be 16-byte aligned");
+    }
+    if (c->x_row_stride < c->hidden || c->x_row_stride % 8)
+        return fail(VY_ERR_ALIGNMENT, "x row stride %lld", (long long)c->x_row_stride);
+    if (!backward) {
+        if (!empty && !c->out) return fail(VY_ERR_INVALID, "null out");
+        if (!aligned16(c->out) || c->out_row_stride % 8 || c->out_row_stride < c->hidden)
+            return fail(VY_ERR_ALIGNMENT, "out %p, row stride %lld", c->out, (long long)c->out_row_stride);
+    } else {
+        if (!empty && (!c->d_out || !c->saved)) return fail(VY_ERR_INVALID, "backward needs d_out and saved");
+        if (!aligned16(c->d_out) || c->d_out_row_stride % 8 || c->d_out_row_stride < c->hidden)
+            return fail(VY_ERR_ALIGNMENT, "d_out %p, row stride %lld", c->d_out, (long long)c->d_out_row_stride);
+        if (!aligned16(c->d_x) || !aligned16(c->d_w_gate) || !aligned16(c->d_w_up) || !aligned16(c->d_w_down) ||
+            (c->d_x && (c->d_x_row_stride % 8 || c->d_x_row_stride < c->hidden)))
+            return fail(VY_ERR_ALIGNMENT, "gradients must be 16-byte aligned (d_x row stride %lld)",
+                        (long long)c->d_x_row_stride);
+    }
+    const size_t bytes = vy_gated_ffn_workspace_size(c, backward);
+    if (!empty && (!c->workspace || c->workspace_bytes < bytes))
+        return fail(VY_ERR_WORKSPACE, "workspace %zu bytes, %zu needed", c->workspace_bytes, bytes);
+    return VY_OK;
+}
+
+void epi_store(TileProblem* q, void* out, int64_t ldo) {
+    q->epi.out = out;
+    q->epi.ldo = ldo;
+}
+
+#define VY_TRY(expr)                         \
+    do {                                     \
+        const int vy_st = (expr);            \
+        if (vy_st != VY_OK) return vy_st;    \
+    } while (0)
+
+template <int ACT>
+int forward(const vy_ffn_call* c, const DeviceInfo* dev, cudaStream_t s) {
+    const int64_t T = c->n_tokens, H = c->hidden, I = c->inter;
+    const int clusters = dev->sm_count / 2;
+    uint16_t* h = reinterpret_cast<uint16_t*>((reinterpret_cast<uintptr_t>(c->workspace) + 255) & ~uintptr_t(255));
+    {
+        TileParams p{};
+        TileProblem& q = p.prob[0];
+        q.m = static_cast<int>(T);
+        q.n = c->inter;
+        q.bn = tile_columns(T, 2 * I, clusters);
+        q.nk[0] = static_cast<int>((H + 63) / 64);
+        VY_TRY(tile_operand(&q.a[0], ACT, c->x, T, H, c->x_row_stride, false, 128));
+        VY_TRY(tile_operand(&q.b[0], ACT, c->w_gate, I, H, H, false, q.bn / 2));
+        VY_TRY(tile_operand(&q.b[1], ACT, c->w_up, I, H, H, false, q.bn / 2));
+        epi_store(&q, h, I);
+        q.epi.act = c->activation;
+        q.epi.saved = c->saved;
+        q.epi.ld_saved = saved_ld(T);
+        q.epi.saved_u = saved_ld(T) * I;
+        p.flags = c->flags;
+        tile_place(&p, 0, true);
+        VY_TRY((tile_launch<EPI_GATE, ACT>(p, dev, s)));
+    }
+    TileParams p{};
+    TileProblem& q = p.prob[0];
+    q.m = static_cast<int>(T);
+    q.n = c->hidden;
+    q.bn = tile_columns(T, H, clusters);
+    q.nk[0] = static_cast<int>((I + 63) / 64);
+    VY_TRY(tile_operand(&q.a[0], ACT, h, T, I, I, false, 128));
+    VY_TRY(tile_operand(&q.b[0], ACT, c->w_down, H, I, I, false, q.bn / 2));
+    epi_store(&q, c->out, c->out_row_stride);
+    p.flags = c->flags;
+    tile_place(&p, 0, false);
+    return tile_launch<EPI_STORE, ACT>(p, dev, s);
+}
+
+template <int ACT>
+int backward(const vy_ffn_call* c, const DeviceInfo* dev, cudaStream_t s) {
+    const int64_t T = c->n_tokens, H = c->hidden, I = c->inter;
+    const int clusters = dev->sm_count / 2;
+    char* base = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(c->workspace) + 255) & ~uintptr_t(255));
+    const size_t each = align256(size_t(h_elems(c)) * 2);
+    uint16_t* dg = reinterpret_cast<uint16_t*>(base);
+    uint16_t* du = reinterpret_cast<uint16_t*>(base + each);
+    uint16_t* h = reinterpret_cast<uint16_t*>(base + 2 * each);
+    {
+        TileParams p{};
+        TileProblem& q = p.prob[0];
+        q.m = static_cast<int>(T);
+        q.n = c->inter;
+        q.bn = tile_columns(T, I, clusters);
+        q.nk[0] = static_cast<int>((H + 63) / 64);
+        q.b_mn = 1;
+        VY_TRY(tile_operand(&q.a[0], ACT, c->d_out, T, H, c->d_out_row_stride, false, 128));
+        VY_TRY(tile_operand(&q.b[0], ACT, c->w_down, I, H, I, true, 0));
+        q.epi.act = c->activation;
+        q.epi.saved = c->saved;
+        q.epi.ld_saved = saved_ld(T);
+        q.epi.saved_u = saved_ld(T) * I;
+        q.epi.ldo = I;
+        q.epi.dg = dg;
+        q.epi.du = du;
+        q.epi.h = h;
+        p.flags = c->flags;
+        tile_place(&p, 0, false);
+        VY_TRY((tile_launch<EPI_DGATE, ACT>(p, dev, s)));
+    }
+    TileParams p{};
+    p.flags = c->flags;
+    int n = 0;
+    if (c->d_x) {      // two K segments: dg Wg + du Wu
+        TileProblem& q = p.prob[n];
+        q.m = static_cast<int>(T);
+        q.n = c->hidden;
+        q.bn = tile_columns(T, H, clusters);
+        q.nk[0] = q.nk[1] = static_cast<int>((I + 63) / 64);
+        q.b_mn = 1;
+        VY_TRY(tile_operand(&q.a[0], ACT, dg, T, I, I, false, 128));
+        VY_TRY(tile_operand(&q.a[1], ACT, du, T, I, I, false, 128));
+        VY_TRY(tile_operand(&q.b[0], ACT, c->w_gate, H, I, H, true, 0));
+        VY_TRY(tile_operand(&q.b[1], ACT, c->w_up, H, I, H, true, 0));
+        epi_store(&q, c->d_x, c->d_x_row_stride);
+        tile_place(&p, n++, false);
+    }
+    struct Grad {
+        void* out;
+        const void *a, *b;
+        int64_t m, n, lda, ldb;
+    };
+    const Grad grads[3] = {{c->d_w_gate, dg, c->x, I, H, I, c->x_row_stride},
+                           {c->d_w_up, du, c->x, I, H, I, c->x_row_stride},
+                           {c->d_w_down, c->d_out, h, H, I, c->d_out_row_stride, I}};
+    for (const Grad& g : grads) {
+        if (!g.out) continue;
+        TileProblem& q = p.prob[n];
+        q.m = static_cast<int>(g.m);
+        q.n = static_cast<int>(g.n);
+        q.bn = tile_columns(g.m, g.n, clusters);
+        q.nk[0] = static_cast<int>((T + 63) / 64);
+        q.a_mn = q.b_mn = 1;
+        VY_TRY(tile_operand(&q.a[0], ACT, g.a, g.m, T, g.lda, true, 0));
+        VY_TRY(tile_operand(&q.b[0], ACT, g.b, g.n, T, g.ldb, true, 0));
+        epi_store(&q, g.out, g.n);
+        tile_place(&p, n++, false);
+    }
+    if (n == 0) return VY_OK;
+    return tile_launch<EPI_STORE, ACT>(p, dev, s);
+}
+
+}  // namespace
+}  // namespace vy
+
+using namespace vy;
+
+extern "C" int64_t vy_gated_ffn_saved_floats(int64_t n_tokens, int32_t inter) {
+    return n_tokens < 0 || inter < 0 ? 0 : 2 * saved_ld(n_tokens) * int64_t(inter);
+}
+
+extern "C" size_t vy_gated_ffn_workspace_size(const vy_ffn_call* c, int32_t backward) {
+    if (!c || c->n_tokens <= 0 || c->inter <= 0) return 0;
+    const size_t each = align256(size_t(h_elems(c)) * 2);
+    return (backward ? 3 * each : each) + 256;
+}
+
+extern "C" int vy_gated_ffn_forward(const vy_ffn_call* c, void* stream) {
+    int st;
+    if ((st = check_ffn(c, false)) != VY_OK) return st;
+    const DeviceInfo* dev = device_info(&st);
+    if (!dev) return st;
+    if (c->n_tokens == 0) return ok();
+    st = c->act_dtype == VY_BF16 ? forward<VY_BF16>(c, dev, as_stream(stream)) : forward<VY_F16>(c, dev, as_stream(stream));
+    return st != VY_OK ? st : check_launch("vy_gated_ffn_forward");
+}
+
+extern "C" int vy_gated_ffn_backward(const vy_ffn_call* c, void* stream) {
+    int st;
+    if ((st = check_ffn(c, true)) != VY_OK) return st;
+    const DeviceInfo* dev = device_info(&st);
+    if (!dev) return st;
+    if (c->n_tokens == 0) {      // no token, no contribution: the weight gradients are zero
+        const size_t bytes = size_t(c->hidden) * size_t(c->inter) * 2;
+        for (void* w : {c->d_w_gate, c->d_w_up, c->d_w_down})
+            if (w && cudaMemsetAsync(w, 0, bytes, as_stream(stream)) != cudaSuccess)
+                return check_launch("vy_gated_ffn_backward");
+        return ok();
+    }
+    st = c->act_dtype == VY_BF16 ? backward<VY_BF16>(c, dev, as_stream(stream)) : backward<VY_F16>(c, dev, as_stream(stream));
+    return st != VY_OK ? st : check_launch("vy_gated_ffn_backward");
+}

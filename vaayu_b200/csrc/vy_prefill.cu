@@ -32,11 +32,8 @@
 //            their registers.
 // Every barrier wait is bounded: on a timeout the CTA records an error flag, drains what it
 // issued, frees TMEM and returns.
-#include <cuda.h>
-
-#include <mutex>
-
 #include "vy_moe.cuh"
+#include "vy_umma.cuh"
 
 namespace vy {
 namespace {
@@ -75,87 +72,7 @@ static_assert(kDqThreads == kBN, "one dequant thread per weight-tile row");
 constexpr uint32_t kBufCols = kBN;            // one accumulator buffer: 128 lanes x N = 256
 constexpr uint32_t kTmemCols = 2 * kBufCols;  // double-buffered: 512 columns
 constexpr int kFoldVals = kBN / 4;            // fp32 sums one fold thread holds (its row, 64 columns)
-constexpr uint64_t kWaitNs = 2000000000ull;   // a barrier wait gives up after 2 s
 constexpr int kTileBytes = kUnit * kBK * 2;   // 16 KB: one 128 x 64 activation tile
-
-__device__ __forceinline__ uint32_t smem_u32(const void* p) {
-    return static_cast<uint32_t>(__cvta_generic_to_shared(p));
-}
-
-// ── mbarrier / TMA / tcgen05 wrappers ───────────────────────────────────────────────────────
-
-__device__ __forceinline__ void mbar_init(uint64_t* bar, uint32_t count) {
-    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(count) : "memory");
-}
-__device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
-}
-__device__ __forceinline__ void mbar_expect_tx(uint64_t* bar, uint32_t bytes) {
-    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes)
-                 : "memory");
-}
-__device__ __forceinline__ bool mbar_try(uint64_t* bar, uint32_t parity) {
-    uint32_t ok;
-    asm volatile(
-        "{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }"
-        : "=r"(ok)
-        : "r"(smem_u32(bar)), "r"(parity)
-        : "memory");
-    return ok != 0;
-}
-// The same test, but a thread whose phase is not complete yet may be suspended (woken when it
-// completes) for up to `hint_ns` instead of returning at once: waiting warps then take no issue
-// slots from the working ones.
-__device__ __forceinline__ bool mbar_try_sleep(uint64_t* bar, uint32_t parity, uint32_t hint_ns) {
-    uint32_t ok;
-    asm volatile(
-        "{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3; selp.u32 %0, 1, 0, p; }"
-        : "=r"(ok)
-        : "r"(smem_u32(bar)), "r"(parity), "r"(hint_ns)
-        : "memory");
-    return ok != 0;
-}
-constexpr uint32_t kSuspendNs = 100000;   // a waiting thread rechecks abort / timeout every 0.1 ms
-__device__ __forceinline__ uint64_t now_ns() {
-    uint64_t t;
-    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-    return t;
-}
-
-// Bounded wait (try_wait suspends in hardware between polls); false once the CTA has aborted, or
-// after `limit_ns`, when it aborts the CTA itself (error bit 4).
-__device__ __forceinline__ bool mbar_wait_for(uint64_t* bar, uint32_t parity, volatile int* abort_flag,
-                                              int32_t* err, uint64_t limit_ns) {
-    if (mbar_try(bar, parity)) return true;
-    const uint64_t t0 = now_ns();
-    for (;;) {
-        if (mbar_try_sleep(bar, parity, kSuspendNs)) return true;
-        if (*abort_flag) return false;
-        if (now_ns() - t0 > limit_ns) {
-            *abort_flag = 1;
-            atomicOr(err, 4);
-            return false;
-        }
-    }
-}
-
-__device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag,
-                                          int32_t* err) {
-    return mbar_wait_for(bar, parity, abort_flag, err, kWaitNs);
-}
-
-// Bounded wait that ignores the abort flag: drains work already issued (TMA loads, MMAs) before
-// the CTA releases its shared memory and TMEM (error bit 8 if even that times out).
-__device__ __forceinline__ bool mbar_drain(uint64_t* bar, uint32_t parity, int32_t* err) {
-    const uint64_t t0 = now_ns();
-    for (;;) {
-        if (mbar_try_sleep(bar, parity, kSuspendNs)) return true;
-        if (now_ns() - t0 > kWaitNs) {
-            atomicOr(err, 8);
-            return false;
-        }
-    }
-}
 
 __device__ __forceinline__ uint2 ld_nc_v2(const void* p) {
     uint2 v;
@@ -191,18 +108,6 @@ struct WordStream {
         return cur;
     }
 };
-
-__device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
-            smem_u32(dst)),
-        "l"(map), "r"(x), "r"(y), "r"(smem_u32(bar))
-        : "memory");
-}
-
-__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
 __device__ __forceinline__ void tmem_alloc(uint32_t* dst, uint32_t ncols) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(dst)), "r"(ncols)
@@ -627,28 +532,10 @@ __global__ void selftest_wait_kernel(int arrivals, uint64_t limit_ns, int32_t* f
 
 // ── host ────────────────────────────────────────────────────────────────────────────────────
 
-using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-EncodeTiledFn encode_fn(int* status) {
-    static EncodeTiledFn fn = nullptr;
-    static std::once_flag once;
-    std::call_once(once, [] {
-        void* p = nullptr;
-        cudaDriverEntryPointQueryResult q;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
-            q == cudaDriverEntryPointSuccess)
-            fn = reinterpret_cast<EncodeTiledFn>(p);
-    });
-    *status = fn ? VY_OK : fail(VY_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
-    return fn;
-}
-
 // A [rows, cols] 16-bit matrix as 256 x 64 tiles with the 128-byte swizzle.
 int make_tile_map(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, int act) {
     int st;
-    EncodeTiledFn fn = encode_fn(&st);
+    EncodeTiledFn fn = encode_tiled_fn(&st);
     if (!fn) return st;
     const cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
     const cuuint64_t strides[1] = {static_cast<cuuint64_t>(cols) * 2};

@@ -1,0 +1,333 @@
+// vy_tile.cuh -- dense GEMM on CTA pairs: out[M, N] = A[M, K] B[N, K]^T for many rows.
+//
+// A pair of CTAs computes a 256 x bn tile (bn = 256 or 128) with tcgen05.mma.cta_group::2: each
+// CTA holds 128 rows of A and half of B's rows in shared memory, so an operand byte is read from
+// L2 once for twice the work of one CTA's tile (a 128 x 256 tile on its own would ask L2 for about
+// 96 bytes a clock and SM, the pair for 64).  K advances in blocks of 128 bytes (64 16-bit
+// elements or 128 int8) through a ring of TMA-filled stages; accumulators are double-buffered in
+// TMEM, so the epilogue of one tile runs under the MMAs of the next.  Both operands may be K-major
+// or MN-major (the weight gradients contract over tokens, the activations' slow axis), and K may
+// come in two segments from two tensor pairs (dx = dg Wg + du Wu).  One launch takes up to four
+// GEMMs, whose tiles fill the machine together.
+//
+// Roles of a CTA (12 warps): warp 0 loads, warp 1 of the pair's first CTA issues the MMAs, warp 2
+// owns TMEM, warps 4-11 run the epilogue.  Every wait is bounded: on a timeout the CTA records the
+// error, leaves its loop, and the pair still meets at its final barrier.
+#pragma once
+
+#include "vy_dense.cuh"
+
+namespace vy {
+
+constexpr int kTileThreads = 384;
+constexpr int kTileStages = 6;
+constexpr int kTileProblems = 4;
+constexpr int kHalfBytes = 128 * 128;          // one operand's share of a stage: 128 rows x 128 bytes
+constexpr uint32_t kTileTmemCols = 512;
+
+struct TileProblem {
+    CUtensorMap a[2], b[2];      // per K segment (per CTA for a gated product: gate, up)
+    int m, n;                    // rows, output columns
+    int nk[2];                   // K blocks of each segment
+    int a_mn, b_mn;              // 1: that operand is MN-major (memory [K, M] / [K, N])
+    int bn;                      // tile columns, 256 or 128
+    int m_tiles, n_tiles, first; // tiles [first, first + m_tiles * n_tiles)
+    EpiParams epi;
+};
+
+struct TileParams {
+    TileProblem prob[kTileProblems];
+    int n_problems, n_tiles;
+    int32_t* flags;
+};
+
+struct __align__(1024) TileSmem {
+    unsigned char a[kTileStages][kHalfBytes];
+    unsigned char b[kTileStages][kHalfBytes];
+    uint64_t full[kTileStages], empty[kTileStages];
+    uint64_t acc_full[2], acc_empty[2];
+    uint32_t tmem_base;
+    int abort_flag;
+};
+
+struct TileAt {
+    int prob, m, n;   // tile's problem, row tile, column tile
+};
+// Bands of 8 row tiles, row tiles fastest inside a band: the tiles in flight share few operand rows.
+__device__ __forceinline__ TileAt tile_at(const TileParams& p, int tile) {
+    TileAt t;
+    t.prob = 0;
+    while (t.prob + 1 < p.n_problems && tile >= p.prob[t.prob + 1].first) ++t.prob;
+    const TileProblem& q = p.prob[t.prob];
+    const int r = tile - q.first, band = r / (8 * q.n_tiles);
+    const int rows = min(8, q.m_tiles - band * 8), in = r - band * 8 * q.n_tiles;
+    t.m = band * 8 + in % rows;
+    t.n = in / rows;
+    return t;
+}
+
+template <int EPI, int ACT>
+__device__ __forceinline__ void tile_epilogue(const TileProblem& q, int row, int n_tile, uint32_t tmem, int half) {
+    const EpiParams& e = q.epi;
+    const bool live = row < q.m;
+    if constexpr (epi_is_gate(EPI)) {
+        const int width = q.bn / 2;                  // output columns of the tile
+        const int c0 = half * (width / 2), c1 = c0 + width / 2;
+        const float rs = EPI == EPI_I8GATE && live ? e.row_scale[row] : 0.f;
+        for (int c = c0; c < c1; c += 16) {
+            uint32_t g[16], u[16];
+            tmem_ld16(tmem + c, g);
+            tmem_ld16(tmem + width + c, u);
+            tmem_wait16(g);
+            tmem_wait16(u);
+            const int col = n_tile * width + c;
+            const int valid = min(16, q.n - col);
+            if (!live || valid <= 0) continue;
+            float h[16];
+            if constexpr (EPI == EPI_I8GATE) {
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    const int cc = j < valid ? col + j : col;
+                    const float gf = __fmul_rn(__fmul_rn(float(int(g[j])), rs), __ldg(e.col_scale[0] + cc));
+                    const float uf = __fmul_rn(__fmul_rn(float(int(u[j])), rs), __ldg(e.col_scale[1] + cc));
+                    h[j] = gate_act(gf, e.act) * uf;
+                }
+                store16_dyn(e.out, VY_F32, int64_t(row) * e.ldo + col, h, valid, true);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 16; ++j) h[j] = gate_act(__uint_as_float(g[j]), e.act) * __uint_as_float(u[j]);
+                if (e.saved) {
+                    float* s = e.saved + int64_t(col) * e.ld_saved + row;
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) {
+                        if (j < valid) {
+                            s[j * e.ld_saved] = __uint_as_float(g[j]);
+                            s[e.saved_u + j * e.ld_saved] = __uint_as_float(u[j]);
+                        }
+                    }
+                }
+                store16<ACT>(reinterpret_cast<uint16_t*>(e.out) + int64_t(row) * e.ldo + col, h, valid);
+            }
+        }
+    } else {
+        const int c0 = half * (q.bn / 2), c1 = c0 + q.bn / 2;
+        const float rs = EPI == EPI_I8 && live ? e.row_scale[row] : 0.f;
+        for (int c = c0; c < c1; c += 16) {
+            uint32_t r[16];
+            tmem_ld16(tmem + c, r);
+            tmem_wait16(r);
+            const int col = n_tile * q.bn + c;
+            const int valid = min(16, q.n - col);
+            if (!live || valid <= 0) continue;
+            float v[16];
+            if constexpr (EPI == EPI_I8) {
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    const int cc = j < valid ? col + j : col;
+                    v[j] = __fmul_rn(__fmul_rn(float(int(r[j])), rs), __ldg(e.col_scale[0] + cc));
+                    if (e.bias) v[j] = __fadd_rn(v[j], load_as_float(e.bias, e.bias_dtype, cc));
+                }
+                store16_dyn(e.out, e.out_dtype, int64_t(row) * e.ldo + col, v, valid, e.vec != 0);
+            } else if constexpr (EPI == EPI_STORE) {
+#pragma unroll
+                for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(r[j]);
+                store16<ACT>(reinterpret_cast<uint16_t*>(e.out) + int64_t(row) * e.ldo + col, v, valid);
+            } else {
+                const float* s = e.saved + int64_t(col) * e.ld_saved + row;
+                float du[16], h[16];
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    const int64_t o = (j < valid ? j : 0) * e.ld_saved;
+                    const float g = s[o], u = s[e.saved_u + o], dh = __uint_as_float(r[j]);
+                    const float2 a = gate_act_grad(g, e.act);
+                    v[j] = dh * u * a.y;
+                    du[j] = dh * a.x;
+                    h[j] = a.x * u;
+                }
+                const int64_t at = int64_t(row) * e.ldo + col;
+                store16<ACT>(e.dg + at, v, valid);
+                store16<ACT>(e.du + at, du, valid);
+                store16<ACT>(e.h + at, h, valid);
+            }
+        }
+    }
+}
+
+template <int EPI, int ACT>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTileThreads, 1)
+    tile_kernel(const __grid_constant__ TileParams p) {
+    extern __shared__ __align__(1024) unsigned char smem_raw[];
+    TileSmem& S = *reinterpret_cast<TileSmem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    constexpr bool I8 = epi_is_i8(EPI);
+    constexpr int kBlockK = I8 ? 128 : 64;      // elements of a 128-byte K block
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const uint32_t rank = cluster_rank();
+    const int cluster = blockIdx.x >> 1, n_clusters = gridDim.x >> 1;
+
+    if (tid == 0) {
+        for (int i = 0; i < kTileStages; ++i) {
+            mbar_init(&S.full[i], 1);     // the first CTA's loader; bytes of both CTAs
+            mbar_init(&S.empty[i], 1);    // the pair's commit
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&S.acc_full[i], 1);
+            mbar_init(&S.acc_empty[i], 16);   // 8 epilogue warps of each CTA
+        }
+        S.abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 2) tmem_alloc_n<1>(&S.tmem_base, kTileTmemCols);
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync();
+    tc_fence_after();
+    const uint32_t tmem = S.tmem_base;
+    volatile int* abort_flag = &S.abort_flag;
+    grid_dependency_wait();
+    grid_dependents_launch();
+
+    if (warp == 0) {
+        if (lane == 0) {
+            uint32_t it = 0;
+            bool go = true;
+            for (int tile = cluster; go && tile < p.n_tiles; tile += n_clusters) {
+                const TileAt t = tile_at(p, tile);
+                const TileProblem& q = p.prob[t.prob];
+                const int m0 = t.m * 256 + int(rank) * 128;
+                // a gated product's pair holds the same columns of gate (first CTA) and up
+                const int n0 = epi_is_gate(EPI) ? t.n * (q.bn / 2) : t.n * q.bn + int(rank) * (q.bn / 2);
+                const uint32_t bytes = 2u * (kHalfBytes + uint32_t(q.bn) * 64u);
+                for (int seg = 0; go && seg < 2; ++seg) {
+                    const CUtensorMap* ma = &q.a[epi_is_gate(EPI) ? 0 : seg];
+                    const CUtensorMap* mb = &q.b[epi_is_gate(EPI) ? rank : seg];
+                    for (int kb = 0; kb < q.nk[seg]; ++kb, ++it) {
+                        const uint32_t s = it % kTileStages;
+                        if (!mbar_wait(&S.empty[s], ((it / kTileStages) & 1) ^ 1, abort_flag, p.flags)) {
+                            go = false;
+                            break;
+                        }
+                        const uint32_t bar = map_to_rank(smem_u32(&S.full[s]), 0);
+                        if (rank == 0) mbar_expect_tx(&S.full[s], bytes);
+                        const int k0 = kb * kBlockK;
+                        const uint32_t da = smem_u32(S.a[s]), db = smem_u32(S.b[s]);
+                        if (!I8 && q.a_mn) {
+                            tma_load_2d_pair(da, ma, m0, k0, bar);
+                            tma_load_2d_pair(da + 8192, ma, m0 + 64, k0, bar);
+                        } else {
+                            tma_load_2d_pair(da, ma, k0, m0, bar);
+                        }
+                        if (!I8 && q.b_mn) {
+                            tma_load_2d_pair(db, mb, n0, k0, bar);
+                            if (q.bn == 256) tma_load_2d_pair(db + 8192, mb, n0 + 64, k0, bar);
+                        } else {
+                            tma_load_2d_pair(db, mb, k0, n0, bar);
+                        }
+                    }
+                }
+            }
+            // every stage this loader filled is read before the CTA may leave (bounded)
+            for (uint32_t i = 0; i < kTileStages && i < it; ++i) {
+                const uint32_t last = it - 1 - i;
+                mbar_drain(&S.empty[last % kTileStages], (last / kTileStages) & 1, p.flags);
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0 && rank == 0) {
+            uint32_t it = 0, n = 0;
+            bool go = true;
+            for (int tile = cluster; go && tile < p.n_tiles; tile += n_clusters, ++n) {
+                const TileProblem& q = p.prob[tile_at(p, tile).prob];
+                const uint32_t idesc = umma_idesc(I8, ACT == VY_BF16, q.a_mn, q.b_mn, 256, q.bn);
+                const uint32_t a_lbo = q.a_mn ? 8192 : 16, b_lbo = q.b_mn ? 8192 : 16;
+                // one MMA's K (32 bytes): along the swizzled row, or 16 rows of 128 bytes
+                const uint32_t a_step = q.a_mn ? 128 : 2, b_step = q.b_mn ? 128 : 2;
+                const uint32_t buf = n & 1, d = tmem + buf * 256;
+                const int nk = q.nk[0] + q.nk[1];
+                if (!mbar_wait(&S.acc_empty[buf], ((n >> 1) & 1) ^ 1, abort_flag, p.flags)) break;
+                tc_fence_after();
+                for (int kb = 0; kb < nk; ++kb, ++it) {
+                    const uint32_t s = it % kTileStages;
+                    if (!mbar_wait(&S.full[s], (it / kTileStages) & 1, abort_flag, p.flags)) {
+                        go = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    const uint64_t da = umma_desc(smem_u32(S.a[s]), a_lbo, 1024);
+                    const uint64_t db = umma_desc(smem_u32(S.b[s]), b_lbo, 1024);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        mma_ss<I8, 1>(d, da + k * a_step, db + k * b_step, idesc, (kb | k) != 0);
+                    mma_commit_pair(&S.empty[s]);
+                }
+                if (go) mma_commit_pair(&S.acc_full[buf]);
+            }
+        }
+    } else if (warp >= 4) {
+        const int quarter = warp & 3, half = (warp - 4) >> 2;
+        uint32_t n = 0;
+        for (int tile = cluster; tile < p.n_tiles; tile += n_clusters, ++n) {
+            const TileAt t = tile_at(p, tile);
+            const uint32_t buf = n & 1;
+            const bool ready = mbar_wait(&S.acc_full[buf], (n >> 1) & 1, abort_flag, p.flags);
+            if (!__all_sync(0xffffffffu, ready)) break;
+            tc_fence_after();
+            tile_epilogue<EPI, ACT>(p.prob[t.prob], t.m * 256 + int(rank) * 128 + quarter * 32 + lane, t.n,
+                                    tmem + buf * 256 + (uint32_t(quarter * 32) << 16), half);
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_remote(map_to_rank(smem_u32(&S.acc_empty[buf]), 0));
+        }
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync();      // neither CTA leaves while the other may still signal or read it
+    tc_fence_after();
+    if (warp == 2) tmem_free_n<1>(tmem, kTileTmemCols);
+}
+
+// ── host ────────────────────────────────────────────────────────────────────────────────────
+
+// The operands of one K segment: `rows` x K matrices, K-major or (mn) stored [K, rows].
+inline int tile_operand(CUtensorMap* map, int dtype, const void* base, int64_t rows, int64_t k, int64_t ld, bool mn,
+                        int box_rows) {
+    const int block = dtype == VY_BF16 || dtype == VY_F16 ? 64 : 128;
+    return mn ? make_map_2d(map, dtype, base, k, rows, ld, 64, 64)
+              : make_map_2d(map, dtype, base, rows, k, ld, block, box_rows);
+}
+
+// Tile columns: 256, unless that leaves most of the clusters without a tile.
+inline int tile_columns(int64_t m, int64_t n, int clusters) {
+    const int64_t wide = ((m + 255) / 256) * ((n + 255) / 256);
+    return wide * 2 <= clusters ? 128 : 256;
+}
+
+// Gives problem i (its sizes and bn set, problems before it placed) its tiles; a gated product's
+// tile has bn / 2 output columns.
+inline void tile_place(TileParams* p, int i, bool gate) {
+    TileProblem& q = p->prob[i];
+    const int width = gate ? q.bn / 2 : q.bn;
+    q.m_tiles = (q.m + 255) / 256;
+    q.n_tiles = (q.n + width - 1) / width;
+    q.first = p->n_tiles;
+    p->n_tiles += q.m_tiles * q.n_tiles;
+    p->n_problems = i + 1;
+}
+
+template <int EPI, int ACT>
+int tile_launch(TileParams& p, const DeviceInfo* dev, cudaStream_t s) {
+    auto kern = tile_kernel<EPI, ACT>;
+    constexpr int smem = sizeof(TileSmem) + 1024;
+    int st = once_per_device(reinterpret_cast<const void*>(kern), [](int, void* k) {
+        const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        return e == cudaSuccess ? VY_OK : fail(VY_ERR_CUDA, "dense GEMM shared memory: %s", cudaGetErrorString(e));
+    }, reinterpret_cast<void*>(kern));
+    if (st != VY_OK) return st;
+    const int pairs = dev->sm_count / 2;
+    const int clusters = p.n_tiles < pairs ? p.n_tiles : pairs;
+    const cudaError_t e = launch_chained(kern, dim3(2 * clusters), dim3(kTileThreads), smem, s, p);
+    if (e != cudaSuccess) return fail(VY_ERR_CUDA, "dense GEMM launch: %s", cudaGetErrorString(e));
+    return VY_OK;
+}
+
+}  // namespace vy
