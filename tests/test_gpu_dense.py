@@ -77,6 +77,19 @@ def test_gradients_against_differences(act):
         assert (slope - (grads[i].double() * v).sum()).abs() <= (bounds[i] * v.abs()).sum() + 1e-6 * size
 
 
+def test_a_thread_that_has_made_no_cuda_call():
+    """The first call of a fresh host thread (autograd's own threads are such) finds no bound context."""
+    import threading
+    ops, _ = make(2, 64, 40, BF16)
+    want, got = vb.gated_ffn(*ops), []
+    out = torch.empty(2, 64, dtype=BF16, device="cuda")
+    torch.cuda.synchronize()
+    thread = threading.Thread(target=lambda: got.append(vb.gated_ffn(*ops, out=out)))
+    thread.start()
+    thread.join()
+    assert torch.equal(got[0], want)
+
+
 def test_only_wanted_gradients():
     for wanted in ((0,), (1,), (2,), (3,), (1, 3), (0, 2)):
         ops, dy = make(40, 128, 72, BF16)

@@ -252,9 +252,18 @@ inline int make_map_2d(CUtensorMap* map, int dtype, const void* base, int64_t ro
     const cuuint64_t strides[1] = {static_cast<cuuint64_t>(ld * size)};
     const cuuint32_t box[2] = {static_cast<cuuint32_t>(box_cols), static_cast<cuuint32_t>(box_rows)};
     const cuuint32_t estr[2] = {1, 1};
-    const CUresult r = fn(map, type, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    auto encode = [&] {
+        return fn(map, type, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    };
+    CUresult r = encode();
+    if (r == CUDA_ERROR_INVALID_CONTEXT) {
+        // a host thread that has made no runtime call yet (autograd's, say) has no context bound:
+        // setting its current device again binds the device's primary context
+        const int dev = current_device();
+        if (dev < 0) return VY_ERR_CUDA;
+        if (cudaSetDevice(dev) == cudaSuccess) r = encode();
+    }
     if (r != CUDA_SUCCESS)
         return fail(VY_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d) for [%lld, %lld], row stride %lld",
                     static_cast<int>(r), (long long)rows, (long long)cols, (long long)ld);
