@@ -8,7 +8,7 @@ import pytest
 import torch
 
 import vaayu_b200 as vb
-from vaayu_b200 import _lib
+from vaayu_b200 import _lib, dense
 
 HEADER = Path(__file__).resolve().parent.parent / "include" / "vaayu_b200.h"
 BF16 = torch.bfloat16
@@ -190,6 +190,12 @@ def test_ctypes_structures_match_the_c_layout(tmp_path):
     subprocess.run(["gcc", "-o", str(tmp_path / "layout"), str(tmp_path / "layout.c")], check=True)
     out = subprocess.run([str(tmp_path / "layout")], capture_output=True, text=True, check=True).stdout
     got = dict(line.split() for line in out.splitlines())
+    for packer, cls in ((dense._FFN, _lib.FfnCall), (dense._LINEAR, _lib.Int8LinearCall),
+                        (dense._INT8_FFN, _lib.Int8FfnCall)):
+        # the packed form puts the same values at the same places as the structure does
+        fields = [(n, i + 1) for i, (n, _t) in enumerate(cls._fields_)]
+        c = cls(**dict(fields))
+        assert packer.pack(*(v for _n, v in fields)) == bytes(c)
     for st, cls in structs.items():
         assert int(got[st]) == ctypes.sizeof(cls)
         for n, _t in cls._fields_:

@@ -92,15 +92,16 @@ SIGNATURES = {
     "vy_ep_combine": (ctypes.c_int, [P, P, P, I32T, I64T, I64T, I32T, I64T, P, I64T, P]),
     "vy_moe_error_flags": (ctypes.c_int, [ctypes.POINTER(MoeCall), I32T, P, P]),
     "vy_selftest_bounded_wait": (ctypes.c_int, [I32T, I64T, P, P]),
+    # the dense calls' structures arrive packed (bytes) or by reference
     "vy_gated_ffn_saved_floats": (I64T, [I64T, I32T]),
-    "vy_gated_ffn_workspace_size": (SZ, [ctypes.POINTER(FfnCall), I32T]),
-    "vy_gated_ffn_forward": (ctypes.c_int, [ctypes.POINTER(FfnCall), P]),
-    "vy_gated_ffn_backward": (ctypes.c_int, [ctypes.POINTER(FfnCall), P]),
+    "vy_gated_ffn_workspace_size": (SZ, [P, I32T]),
+    "vy_gated_ffn_forward": (ctypes.c_int, [P, P]),
+    "vy_gated_ffn_backward": (ctypes.c_int, [P, P]),
     "vy_int8_quantize": (ctypes.c_int, [P, I32T, I64T, I64T, I64T, P, P, P]),
-    "vy_int8_linear_workspace_size": (SZ, [ctypes.POINTER(Int8LinearCall)]),
-    "vy_int8_linear": (ctypes.c_int, [ctypes.POINTER(Int8LinearCall), P]),
-    "vy_int8_gated_ffn_workspace_size": (SZ, [ctypes.POINTER(Int8FfnCall)]),
-    "vy_int8_gated_ffn": (ctypes.c_int, [ctypes.POINTER(Int8FfnCall), P]),
+    "vy_int8_linear_workspace_size": (SZ, [P]),
+    "vy_int8_linear": (ctypes.c_int, [P, P]),
+    "vy_int8_gated_ffn_workspace_size": (SZ, [P]),
+    "vy_int8_gated_ffn": (ctypes.c_int, [P, P]),
 }
 
 _LIB = None

@@ -6,6 +6,7 @@
 //
 // Bounds.  Forward 6 T H I flops on 6 H I bytes of weights: HBM below about 250 tokens, the tensor
 // cores above.  Backward 12 T H I flops.
+#include "vy_stream.cuh"
 #include "vy_tile.cuh"
 
 namespace vy {
@@ -72,6 +73,22 @@ int forward(const vy_ffn_call* c, const DeviceInfo* dev, cudaStream_t s) {
     const int64_t T = c->n_tokens, H = c->hidden, I = c->inter;
     const int clusters = dev->sm_count / 2;
     uint16_t* h = reinterpret_cast<uint16_t*>((reinterpret_cast<uintptr_t>(c->workspace) + 255) & ~uintptr_t(255));
+    if (T <= kStreamMaxTokens) {
+        EpiParams e{};
+        e.out = h;
+        e.ldo = I;
+        e.act = c->activation;
+        e.saved = c->saved;
+        e.ld_saved = saved_ld(T);
+        e.saved_u = saved_ld(T) * I;
+        VY_TRY((stream_launch<EPI_GATE, ACT>(c->w_gate, c->w_up, c->x, c->x_row_stride, static_cast<int>(T), c->inter,
+                                             c->hidden, false, e, c->flags, dev, s)));
+        EpiParams d{};
+        d.out = c->out;
+        d.ldo = c->out_row_stride;
+        return stream_launch<EPI_STORE, ACT>(c->w_down, nullptr, h, I, static_cast<int>(T), c->hidden, c->inter, true, d,
+                                             c->flags, dev, s);
+    }
     {
         TileParams p{};
         TileProblem& q = p.prob[0];

@@ -4,6 +4,7 @@
 // Bounds.  Quantisation: HBM (each value read once, kept in registers between the row maximum and
 // the rounding).  The products: the weights' bytes for few tokens, the tensor cores' int8 rate
 // (twice the bf16 rate) for many.
+#include "vy_stream.cuh"
 #include "vy_tile.cuh"
 
 namespace vy {
@@ -154,7 +155,7 @@ int launch_quantize(const void* x, int dtype, int64_t stride, int64_t rows, int6
         if (vy_st != VY_OK) return vy_st;    \
     } while (0)
 
-// out = scaled codes x weight^T; gate: w[0], w[1] are gate and up and out is h (fp32).
+// out = scaled codes x weight^T (`first`: no kernel of the same call runs in front of it); gate: w[0], w[1] are gate and up and out is h (fp32).
 struct Product {
     const int8_t* codes;
     int64_t codes_ld;
@@ -172,17 +173,8 @@ struct Product {
 };
 
 template <bool GATE>
-int launch_product(const Product& a, const DeviceInfo* dev, cudaStream_t s) {
-    TileParams p{};
-    TileProblem& q = p.prob[0];
-    q.m = static_cast<int>(a.tokens);
-    q.n = a.n;
-    q.bn = tile_columns(a.tokens, GATE ? 2 * int64_t(a.n) : a.n, dev->sm_count / 2);
-    q.nk[0] = (a.k + 127) / 128;
-    VY_TRY(tile_operand(&q.a[0], VY_E4M3, a.codes, a.tokens, a.k, a.codes_ld, false, 128));
-    VY_TRY(tile_operand(&q.b[0], VY_E4M3, a.w[0], a.n, a.k, a.k, false, q.bn / 2));
-    if (GATE) VY_TRY(tile_operand(&q.b[1], VY_E4M3, a.w[1], a.n, a.k, a.k, false, q.bn / 2));
-    EpiParams& e = q.epi;
+int launch_product(const Product& a, bool first, const DeviceInfo* dev, cudaStream_t s) {
+    EpiParams e{};
     e.out = a.out;
     e.ldo = a.ldo;
     e.out_dtype = a.out_dtype;
@@ -193,9 +185,23 @@ int launch_product(const Product& a, const DeviceInfo* dev, cudaStream_t s) {
     e.col_scale[1] = a.ws[1];
     e.bias = a.bias;
     e.bias_dtype = a.bias_dtype;
+    constexpr int EPI = GATE ? EPI_I8GATE : EPI_I8;
+    if (a.tokens <= kStreamMaxTokens)
+        return stream_launch<EPI, VY_BF16>(a.w[0], a.w[1], a.codes, a.codes_ld, static_cast<int>(a.tokens), a.n, a.k,
+                                           !first, e, a.flags, dev, s);
+    TileParams p{};
+    TileProblem& q = p.prob[0];
+    q.m = static_cast<int>(a.tokens);
+    q.n = a.n;
+    q.bn = tile_columns(a.tokens, GATE ? 2 * int64_t(a.n) : a.n, dev->sm_count / 2);
+    q.nk[0] = (a.k + 127) / 128;
+    VY_TRY(tile_operand(&q.a[0], VY_E4M3, a.codes, a.tokens, a.k, a.codes_ld, false, 128));
+    VY_TRY(tile_operand(&q.b[0], VY_E4M3, a.w[0], a.n, a.k, a.k, false, q.bn / 2));
+    if (GATE) VY_TRY(tile_operand(&q.b[1], VY_E4M3, a.w[1], a.n, a.k, a.k, false, q.bn / 2));
+    q.epi = e;
     p.flags = a.flags;
     tile_place(&p, 0, GATE);
-    return tile_launch<GATE ? EPI_I8GATE : EPI_I8, VY_BF16>(p, dev, s);
+    return tile_launch<EPI, VY_BF16>(p, dev, s);
 }
 
 bool float_dtype(int d) { return d == VY_BF16 || d == VY_F16 || d == VY_F32; }
@@ -296,7 +302,7 @@ extern "C" int vy_int8_linear(const vy_int8_linear_call* c, void* stream) {
     if (c->n_tokens == 0) return ok();
     Product a{c->codes, c->codes_row_stride, c->scales, {c->weight, nullptr}, {c->weight_scales, nullptr}, c->n_tokens,
               c->k, c->n, c->out, c->out_row_stride, c->out_dtype, 0, c->bias, c->bias_dtype, c->flags};
-    st = launch_product<false>(a, dev, as_stream(stream));
+    st = launch_product<false>(a, true, dev, as_stream(stream));
     return st != VY_OK ? st : check_launch("vy_int8_linear");
 }
 
@@ -317,10 +323,10 @@ extern "C" int vy_int8_gated_ffn(const vy_int8_ffn_call* c, void* stream) {
     VY_TRY(launch_quantize(c->x, c->act_dtype, c->x_row_stride, c->n_tokens, c->hidden, L.x_codes, L.x_scales, s));
     Product gu{L.x_codes, c->hidden, L.x_scales, {c->w_gate, c->w_up}, {c->gate_scales, c->up_scales}, c->n_tokens,
                c->hidden, c->inter, L.h, c->inter, VY_F32, c->activation, nullptr, 0, c->flags};
-    VY_TRY(launch_product<true>(gu, dev, s));
+    VY_TRY(launch_product<true>(gu, false, dev, s));
     VY_TRY(launch_quantize(L.h, VY_F32, c->inter, c->n_tokens, c->inter, L.h_codes, L.h_scales, s));
     Product down{L.h_codes, c->inter, L.h_scales, {c->w_down, nullptr}, {c->down_scales, nullptr}, c->n_tokens, c->inter,
                  c->hidden, c->out, c->out_row_stride, c->act_dtype, 0, nullptr, 0, c->flags};
-    VY_TRY(launch_product<false>(down, dev, s));
+    VY_TRY(launch_product<false>(down, false, dev, s));
     return check_launch("vy_int8_gated_ffn");
 }

@@ -1,0 +1,314 @@
+// vy_stream.cuh -- dense GEMM for few rows: out[T, N] = x[T, K] W[N, K]^T with T <= 128.
+//
+// The weights' bytes are the cost, so the kernel is a weight stream that happens to use the tensor
+// core: 128 weight rows are the MMA's M (a gated product holds 128 gate and 128 up rows), the tokens
+// its N, rounded up to 16.  Weight tiles arrive by TMA in a ring deep enough to keep about 100 KB in
+// flight per CTA, two CTAs on an SM; HBM needs about 45 KB an SM in flight at its latency.
+//
+// K is split over the CTAs of a cluster: each accumulates its share in TMEM, leaves the sums in its
+// shared memory, and after one cluster barrier every CTA adds a slice of the rows over all shares, in
+// rank order, through distributed shared memory.  No workspace, no atomics, one order of summation.
+//
+// A kernel that is not the first of its call starts loading weights before the kernel in front of it
+// has finished (they do not depend on it); its token tiles wait for it.
+#pragma once
+
+#include <cstdlib>
+
+#include "vy_dense.cuh"
+
+namespace vy {
+
+constexpr int kStreamRows = 128;        // weight rows of a unit (of each matrix)
+constexpr int kStreamMaxTokens = 128;
+constexpr int kStreamThreads = 192;     // warps 0-3 read the sums, 4 loads, 5 issues the MMAs
+constexpr int kStreamMaxStages = 12;
+
+struct StreamParams {
+    CUtensorMap w[2], x;
+    int tokens, n, nk;      // nk: K blocks of 128 bytes
+    int cols;               // MMA N: tokens rounded up to 16
+    int stages, tmem_cols;
+    int early;              // weights may be loaded before the previous kernel has finished
+    EpiParams epi;
+    int32_t* flags;
+};
+
+struct StreamBars {
+    uint64_t full[kStreamMaxStages], empty[kStreamMaxStages], done;
+    uint32_t tmem_base;
+    int abort_flag;
+};
+
+// One output value (weight row `row`, token `t`) from its sums.
+template <int EPI, int ACT>
+__device__ __forceinline__ void stream_put(const StreamParams& p, int row, int t, uint32_t s0, uint32_t s1) {
+    const EpiParams& e = p.epi;
+    const int64_t at = int64_t(t) * e.ldo + row;
+    if constexpr (EPI == EPI_GATE) {
+        const float g = __uint_as_float(s0), u = __uint_as_float(s1);
+        reinterpret_cast<uint16_t*>(e.out)[at] = static_cast<uint16_t>(act_bits<ACT>(gate_act(g, e.act) * u));
+        if (e.saved) {
+            float* s = e.saved + int64_t(row) * e.ld_saved + t;
+            s[0] = g;
+            s[e.saved_u] = u;
+        }
+    } else if constexpr (EPI == EPI_STORE) {
+        reinterpret_cast<uint16_t*>(e.out)[at] = static_cast<uint16_t>(act_bits<ACT>(__uint_as_float(s0)));
+    } else if constexpr (EPI == EPI_I8GATE) {
+        const float rs = __ldg(e.row_scale + t);
+        const float g = __fmul_rn(__fmul_rn(float(int(s0)), rs), __ldg(e.col_scale[0] + row));
+        const float u = __fmul_rn(__fmul_rn(float(int(s1)), rs), __ldg(e.col_scale[1] + row));
+        reinterpret_cast<float*>(e.out)[at] = gate_act(g, e.act) * u;
+    } else {
+        float v = __fmul_rn(__fmul_rn(float(int(s0)), __ldg(e.row_scale + t)), __ldg(e.col_scale[0] + row));
+        if (e.bias) v = __fadd_rn(v, load_as_float(e.bias, e.bias_dtype, row));
+        store_as(e.out, e.out_dtype, at, v);
+    }
+}
+
+__device__ __forceinline__ uint32_t ld_cluster(uint32_t addr) {
+    uint32_t v;
+    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr));
+    return v;
+}
+
+template <int EPI, int ACT>
+__global__ void __launch_bounds__(kStreamThreads) stream_kernel(const __grid_constant__ StreamParams p) {
+    extern __shared__ __align__(1024) unsigned char smem_raw[];
+    __shared__ StreamBars S;
+    unsigned char* ring = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    constexpr bool I8 = epi_is_i8(EPI);
+    constexpr int NW = epi_is_gate(EPI) ? 2 : 1;
+    constexpr int kBlockK = I8 ? 128 : 64;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    uint32_t splits;
+    asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(splits));
+    const uint32_t rank = cluster_rank();
+    const int unit = blockIdx.x / splits;
+    const int row0 = unit * kStreamRows;
+    const uint32_t x_bytes = uint32_t(p.cols) * 128u;
+    const uint32_t stage_bytes = NW * 16384u + x_bytes;
+    const int k_first = int(int64_t(p.nk) * rank / splits), k_last = int(int64_t(p.nk) * (rank + 1) / splits);
+    const int nk = k_last - k_first;
+
+    if (tid == 0) {
+        for (int i = 0; i < p.stages; ++i) {
+            mbar_init(&S.full[i], 1);
+            mbar_init(&S.empty[i], 1);
+        }
+        mbar_init(&S.done, 1);
+        S.abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 0) tmem_alloc_n<0>(&S.tmem_base, p.tmem_cols);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = S.tmem_base;
+    volatile int* abort_flag = &S.abort_flag;
+    if (warp != 4) {
+        grid_dependency_wait();
+        grid_dependents_launch();
+    }
+
+    if (warp == 4) {
+        if (lane == 0) {
+            auto load_w = [&](int i) {
+                const uint32_t s = i % p.stages;
+                const int k = (k_first + i) * kBlockK;
+                unsigned char* at = ring + s * stage_bytes;
+                mbar_expect_tx(&S.full[s], stage_bytes);
+                tma_load_2d(at, &p.w[0], k, row0, &S.full[s]);
+                if (NW == 2) tma_load_2d(at + 16384, &p.w[1], k, row0, &S.full[s]);
+            };
+            auto load_x = [&](int i) {
+                const uint32_t s = i % p.stages;
+                tma_load_2d(ring + s * stage_bytes + NW * 16384, &p.x, (k_first + i) * kBlockK, 0, &S.full[s]);
+            };
+            int ahead = 0;
+            if (p.early)
+                for (; ahead < p.stages && ahead < nk; ++ahead) load_w(ahead);
+            grid_dependency_wait();
+            grid_dependents_launch();
+            for (int i = 0; i < ahead; ++i) load_x(i);
+            int i = ahead;
+            for (; i < nk; ++i) {
+                if (i >= p.stages && !mbar_wait(&S.empty[i % p.stages], ((i / p.stages) & 1) ^ 1, abort_flag, p.flags)) break;
+                load_w(i);
+                load_x(i);
+            }
+            // all loads have landed and been read before the ring is used again or the CTA leaves
+            for (int j = max(0, i - p.stages); j < i; ++j) mbar_drain(&S.empty[j % p.stages], (j / p.stages) & 1, p.flags);
+        } else {
+            grid_dependency_wait();
+            grid_dependents_launch();
+        }
+    } else if (warp == 5) {
+        if (lane == 0) {
+            const uint32_t idesc = umma_idesc(I8, ACT == VY_BF16, 0, 0, kStreamRows, p.cols);
+            bool go = true;
+            for (int i = 0; i < nk; ++i) {
+                const uint32_t s = i % p.stages;
+                if (!mbar_wait(&S.full[s], (i / p.stages) & 1, abort_flag, p.flags)) {
+                    go = false;
+                    break;
+                }
+                tc_fence_after();
+                const uint32_t at = smem_u32(ring) + s * stage_bytes;
+                const uint64_t dx = umma_desc(at + NW * 16384, 16, 1024);
+#pragma unroll
+                for (int m = 0; m < NW; ++m) {
+                    const uint64_t dw = umma_desc(at + m * 16384, 16, 1024);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        mma_ss<I8, 0>(tmem + m * p.cols, dw + 2 * k, dx + 2 * k, idesc, (i | k) != 0);
+                }
+                mma_commit_one(&S.empty[s]);
+            }
+            if (go) mma_commit_one(&S.done);
+        }
+    }
+    __syncwarp();
+
+    // sums [matrix][token][row] in shared memory, rows fastest (a warp's lanes are rows)
+    uint32_t* part = reinterpret_cast<uint32_t*>(ring);
+    bool ready = true;
+    if (warp < 4) {
+        ready = __all_sync(0xffffffffu, mbar_wait(&S.done, 0, abort_flag, p.flags));
+        tc_fence_after();
+        const uint32_t lanes = uint32_t(warp * 32) << 16;
+        const int row = warp * 32 + lane;
+        if (ready) {
+            for (int c = 0; c < p.cols; c += 16) {
+                uint32_t v[NW][16];
+#pragma unroll
+                for (int m = 0; m < NW; ++m) tmem_ld16(tmem + lanes + m * p.cols + c, v[m]);
+#pragma unroll
+                for (int m = 0; m < NW; ++m) tmem_wait16(v[m]);
+                if (nk == 0) {      // a share of no K blocks: TMEM holds nothing of this call
+#pragma unroll
+                    for (int m = 0; m < NW; ++m)
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) v[m][j] = 0;
+                }
+                if (splits == 1) {
+                    if (row0 + row < p.n) {
+#pragma unroll
+                        for (int j = 0; j < 16; ++j)
+                            if (c + j < p.tokens) stream_put<EPI, ACT>(p, row0 + row, c + j, v[0][j], v[NW - 1][j]);
+                    }
+                } else {
+#pragma unroll
+                    for (int m = 0; m < NW; ++m)
+#pragma unroll
+                        for (int j = 0; j < 16; ++j)
+                            if (c + j < p.tokens) part[(m * p.cols + c + j) * kStreamRows + row] = v[m][j];
+                }
+            }
+        }
+        tc_fence_before();
+    }
+    if (splits > 1) {
+        cluster_sync();
+        const int rows = kStreamRows / splits, first = rank * rows;      // 2, 4 or 8 shares: a power of two
+        const uint32_t base = smem_u32(part);
+        for (int q = tid; q < rows * p.tokens; q += kStreamThreads) {
+            const int row = first + q % rows, t = q / rows;
+            if (row0 + row >= p.n) continue;
+            uint32_t sum[NW];
+#pragma unroll
+            for (int m = 0; m < NW; ++m) {
+                const uint32_t at = base + 4u * ((m * p.cols + t) * kStreamRows + row);
+                uint32_t v[8];
+#pragma unroll
+                for (uint32_t r = 0; r < 8; ++r)
+                    if (r < splits) v[r] = ld_cluster(map_to_rank(at, r));
+                uint32_t acc = v[0];
+#pragma unroll
+                for (uint32_t r = 1; r < 8; ++r)
+                    if (r < splits)
+                        acc = I8 ? acc + v[r] : __float_as_uint(__fadd_rn(__uint_as_float(acc), __uint_as_float(v[r])));
+                sum[m] = acc;
+            }
+            stream_put<EPI, ACT>(p, row0 + row, t, sum[0], sum[NW - 1]);
+        }
+        cluster_sync();      // no CTA leaves while another still reads its sums
+    } else {
+        __syncthreads();
+    }
+    tc_fence_after();
+    if (warp == 0) tmem_free_n<0>(tmem, p.tmem_cols);
+}
+
+// ── host ────────────────────────────────────────────────────────────────────────────────────
+
+// CTAs that share a unit's K.
+inline int stream_splits(int64_t n, int nk, int sm_count) {
+    const int64_t units = (n + kStreamRows - 1) / kStreamRows;
+    int s = 1;
+    while (s < 8 && units * s < sm_count && nk >= 4 * s) s *= 2;
+    if (const char* e = getenv("VY_SPLITS")) s = atoi(e);
+    return s;
+}
+
+// w: NW weight matrices [n, k], contiguous; x: [tokens, k].
+template <int EPI, int ACT>
+int stream_launch(const void* w0, const void* w1, const void* x, int64_t x_ld, int tokens, int n, int k, bool early,
+                  const EpiParams& epi, int32_t* flags, const DeviceInfo* dev, cudaStream_t s) {
+    constexpr bool I8 = epi_is_i8(EPI);
+    constexpr int NW = epi_is_gate(EPI) ? 2 : 1;
+    constexpr int block = I8 ? 128 : 64;
+    const int dtype = I8 ? VY_E4M3 : ACT;
+    StreamParams p{};
+    p.tokens = tokens;
+    p.n = n;
+    p.nk = (k + block - 1) / block;
+    p.cols = (tokens + 15) / 16 * 16;
+    p.early = early;
+    p.epi = epi;
+    p.flags = flags;
+    p.tmem_cols = 32;
+    while (p.tmem_cols < NW * p.cols) p.tmem_cols *= 2;
+    int st;
+    if ((st = make_map_2d(&p.w[0], dtype, w0, n, k, k, block, kStreamRows)) != VY_OK) return st;
+    if (NW == 2 && (st = make_map_2d(&p.w[1], dtype, w1, n, k, k, block, kStreamRows)) != VY_OK) return st;
+    if ((st = make_map_2d(&p.x, dtype, x, tokens, k, x_ld, block, p.cols)) != VY_OK) return st;
+    const int splits = stream_splits(n, p.nk, dev->sm_count);
+    const int stage = NW * 16384 + p.cols * 128;
+    const int sums = splits > 1 ? NW * p.cols * kStreamRows * 4 : 0;
+    // about 100 KB of stages: two CTAs on an SM; more only where the sums to be joined ask for it
+    p.stages = 100 * 1024 / stage;
+    if (p.stages > kStreamMaxStages) p.stages = kStreamMaxStages;
+    if (p.stages < 2) p.stages = 2;
+    int bytes = p.stages * stage;
+    if (bytes < sums) bytes = sums;
+    bytes += 1024;
+    auto kern = stream_kernel<EPI, ACT>;
+    constexpr int kMost = 2 * 128 * kStreamRows * 4 + 2 * 1024 + 32768;
+    st = once_per_device(reinterpret_cast<const void*>(kern), [](int, void* f) {
+        const cudaError_t e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost);
+        return e == cudaSuccess ? VY_OK : fail(VY_ERR_CUDA, "dense stream shared memory: %s", cudaGetErrorString(e));
+    }, reinterpret_cast<void*>(kern));
+    if (st != VY_OK) return st;
+    if (bytes > kMost) return fail(VY_ERR_UNSUPPORTED, "dense stream: %d bytes of shared memory", bytes);
+    const unsigned units = (n + kStreamRows - 1) / kStreamRows;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(units * splits);
+    cfg.blockDim = dim3(kStreamThreads);
+    cfg.dynamicSmemBytes = bytes;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = splits;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, p);
+    if (e != cudaSuccess) return fail(VY_ERR_CUDA, "dense stream launch: %s", cudaGetErrorString(e));
+    return VY_OK;
+}
+
+}  // namespace vy

@@ -18,17 +18,50 @@ when a device-side wait ran out.  They may be captured in a CUDA graph.
 """
 from __future__ import annotations
 
-import ctypes
+import struct
 
 import torch
 
 from . import _lib
 
 ACTIVATIONS = {"silu": 0, "gelu_tanh": 1}
-_FLOATS = (torch.bfloat16, torch.float16, torch.float32)
+_BF16, _F16, _F32, _INT8 = torch.bfloat16, torch.float16, torch.float32, torch.int8
+_CODE = {_BF16: _lib.BF16, _F16: _lib.F16, _F32: _lib.F32}
+_MAX_K = 131072      # an int32 sum of fewer int8 products cannot overflow
+
+# The call structures of include/vaayu_b200.h, packed in one go: a ctypes structure filled field by
+# field costs more host time than the launch of a small call.
+_FFN = struct.Struct("@iiqiiPqPPPPqPPNPPqPqPPP")
+_LINEAR = struct.Struct("@qiiPqPPPPiiPqPNP")
+_INT8_FFN = struct.Struct("@iiqiiPqPPPPPPPqPNP")
+
+_current_device = torch._C._cuda_getDevice
+_raw_stream = torch._C._cuda_getCurrentRawStream
 
 
-def _act_code(act: str, what: str) -> int:
+def _device(what: str, first: torch.Tensor, *others) -> int:
+    """The index of the CUDA device all tensors are on; raises as `_lib.require_cuda` does."""
+    index = first.get_device()
+    for t in others:
+        if t is not None and t.get_device() != index:
+            index = -1
+    if index < 0:
+        _lib.require_cuda(first, *others, what=what)
+    return index
+
+
+def _enqueue(fn, call, index: int, what: str) -> None:
+    """One C call on the device's current stream, with that device current."""
+    if index == _current_device():
+        status = fn(call, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            status = fn(call, _raw_stream(index))
+    if status:
+        _lib.check(status, what)
+
+
+def _activation(act: str, what: str) -> int:
     code = ACTIVATIONS.get(act)
     if code is None:
         raise NotImplementedError(f"{what}: activation {act!r} (one of {', '.join(ACTIVATIONS)})")
@@ -38,42 +71,69 @@ def _act_code(act: str, what: str) -> int:
 def _rows(x: torch.Tensor, unit: int) -> torch.Tensor:
     """x as [tokens, width] rows that start on 16-byte boundaries (`unit` elements): a view where the
     strides allow it, else a copy."""
-    x = x.reshape(-1, x.shape[-1])
-    if x.stride(1) != 1 or x.data_ptr() % 16 or (x.shape[0] > 1 and (x.stride(0) % unit or x.stride(0) < x.shape[1])):
-        x = x.clone(memory_format=torch.contiguous_format)
-    return x
+    if x.dim() != 2:
+        x = x.reshape(-1, x.shape[-1])
+    if x.data_ptr() % 16 == 0:
+        if x.is_contiguous():
+            if x.shape[1] % unit == 0 or x.shape[0] <= 1:
+                return x
+        else:
+            row, col = x.stride()
+            if col == 1 and (x.shape[0] <= 1 or (row % unit == 0 and row >= x.shape[1])):
+                return x
+    return x.clone(memory_format=torch.contiguous_format)
+
+
+def _unit_rows(x: torch.Tensor) -> torch.Tensor:
+    """x as [tokens, width] with a unit column stride."""
+    if x.dim() != 2:
+        x = x.reshape(-1, x.shape[-1])
+    return x if x.stride(1) == 1 else x.contiguous()
 
 
 def _stride(x: torch.Tensor) -> int:
-    return x.stride(0) if x.shape[0] > 1 else x.shape[1]
+    tokens, width = x.shape
+    return x.stride(0) if tokens > 1 else width
 
 
 def _aligned(w: torch.Tensor) -> torch.Tensor:
-    w = w.contiguous()
+    if not w.is_contiguous():
+        w = w.contiguous()
     return w.clone() if w.data_ptr() % 16 else w
 
 
-def _check_ffn(x, w_gate, w_up, w_down, what: str) -> None:
-    if x.dim() < 1 or w_gate.dim() != 2 or w_up.shape != w_gate.shape or w_down.shape != w_gate.shape[::-1]:
+def _check_ffn(x, w_gate, w_up, w_down, what: str) -> tuple:
+    """(hidden, inter) of a block whose operands fit together."""
+    shape = w_gate.shape
+    if x.dim() < 1 or len(shape) != 2 or w_up.shape != shape or w_down.shape != shape[::-1]:
         raise ValueError(f"{what}: weights {tuple(w_gate.shape)}, {tuple(w_up.shape)}, {tuple(w_down.shape)} "
                          "are not [inter, hidden], [inter, hidden], [hidden, inter]")
-    if x.shape[-1] != w_gate.shape[1]:
-        raise ValueError(f"{what}: x {tuple(x.shape)} does not fit hidden {w_gate.shape[1]}")
+    if x.shape[-1] != shape[1]:
+        raise ValueError(f"{what}: x {tuple(x.shape)} does not fit hidden {shape[1]}")
+    return shape[1], shape[0]
 
 
-def _output(out, shape, dtype, dev, what: str) -> torch.Tensor:
-    """`out` checked, or a new tensor."""
+def _output(out, like, shape, dtype, what: str) -> tuple:
+    """(`out` checked or a new tensor on like's device, it as [tokens, width])."""
     if out is None:
-        return torch.empty(shape, dtype=dtype, device=dev)
-    if out.shape != torch.Size(shape) or out.dtype != dtype:
+        out = torch.empty(shape, dtype=dtype, device=like.device)
+    elif out.shape != shape or out.dtype != dtype:
         raise ValueError(f"{what}: out {tuple(out.shape)} {out.dtype}, expected {tuple(shape)} {dtype}")
-    if not out.is_contiguous() and (out.dim() != 2 or out.stride(1) != 1 or out.stride(0) < out.shape[1]):
+    elif not out.is_contiguous() and (out.dim() != 2 or out.stride(1) != 1 or out.stride(0) < out.shape[1]):
         raise ValueError(f"{what}: out must be contiguous, or a 2-D view with unit column stride")
-    return out
+    return out, (out if out.dim() == 2 else out.view(-1, shape[-1]))
 
 
-def _flags(dev, check: bool) -> "torch.Tensor | None":
-    return torch.zeros(1, dtype=torch.int32, device=dev) if check else None
+def _workspace(size: int, like: torch.Tensor) -> "torch.Tensor | None":
+    return torch.empty(size, dtype=_INT8, device=like.device) if size else None
+
+
+def _flags(like: torch.Tensor, check: bool) -> "torch.Tensor | None":
+    return torch.zeros(1, dtype=torch.int32, device=like.device) if check else None
+
+
+def _ptr(t: "torch.Tensor | None") -> int:
+    return 0 if t is None else t.data_ptr()
 
 
 def _raise_on(flags: "torch.Tensor | None", what: str) -> None:
@@ -83,39 +143,34 @@ def _raise_on(flags: "torch.Tensor | None", what: str) -> None:
 
 # ── gated feed-forward, 16-bit ───────────────────────────────────────────────────────────────
 
-
-def _ffn_call(x, w_gate, w_up, w_down, act: int) -> _lib.FfnCall:
-    c = _lib.FfnCall()
-    c.act_dtype, c.activation = _lib.DTYPE_CODE[x.dtype], act
-    c.n_tokens, c.hidden, c.inter = x.shape[0], x.shape[1], w_gate.shape[0]
-    c.x, c.x_row_stride = x.data_ptr(), _stride(x)
-    c.w_gate, c.w_up, c.w_down = w_gate.data_ptr(), w_up.data_ptr(), w_down.data_ptr()
-    return c
+_FFN_SIZES: dict = {}      # (tokens, hidden, inter, backward) -> workspace bytes
 
 
-def _run_ffn(c: _lib.FfnCall, backward: bool, dev) -> None:
-    lib = _lib.lib()
-    what = "gated_ffn backward" if backward else "gated_ffn"
-    with torch.cuda.device(dev):
-        c.workspace_bytes = lib.vy_gated_ffn_workspace_size(ctypes.byref(c), int(backward))
-        ws = torch.empty(c.workspace_bytes, dtype=torch.uint8, device=dev)
-        c.workspace = ws.data_ptr()
-        fn = lib.vy_gated_ffn_backward if backward else lib.vy_gated_ffn_forward
-        _lib.check(fn(ctypes.byref(c), _lib.stream_of(dev)), what)
+def _ffn_workspace(tokens: int, hidden: int, inter: int, backward: int) -> int:
+    key = (tokens, hidden, inter, backward)
+    size = _FFN_SIZES.get(key)
+    if size is None:
+        call = _FFN.pack(0, 0, tokens, hidden, inter, *(0,) * 18)
+        if len(_FFN_SIZES) >= 4096:
+            _FFN_SIZES.clear()
+        size = _FFN_SIZES[key] = _lib.lib().vy_gated_ffn_workspace_size(call, backward)
+    return size
 
 
-def _ffn_forward(x, w_gate, w_up, w_down, act: int, out, save: bool, check: bool):
-    """(out [T, hidden], saved or None) for 2-D rows x."""
-    dev = x.device
-    c = _ffn_call(x, w_gate, w_up, w_down, act)
-    c.out, c.out_row_stride = out.data_ptr(), _stride(out)
+def _ffn_forward(rows, wg, wu, wd, act: int, flat, index: int, save: bool, check: bool):
+    """The forward call on 2-D rows into `flat`; returns what the backward pass needs when `save`."""
+    tokens, hidden = rows.shape
+    inter = wg.shape[0]
+    size = _ffn_workspace(tokens, hidden, inter, 0)
+    ws = _workspace(size, rows)
     saved = None
     if save:
-        saved = torch.empty(_lib.lib().vy_gated_ffn_saved_floats(c.n_tokens, c.inter), dtype=torch.float32, device=dev)
-        c.saved = saved.data_ptr()
-    flags = _flags(dev, check)
-    c.flags = _lib.ptr(flags)
-    _run_ffn(c, False, dev)
+        saved = torch.empty(_lib.lib().vy_gated_ffn_saved_floats(tokens, inter), dtype=_F32, device=rows.device)
+    flags = _flags(rows, check)
+    call = _FFN.pack(_CODE[rows.dtype], act, tokens, hidden, inter, rows.data_ptr(), _stride(rows), wg.data_ptr(),
+                     wu.data_ptr(), wd.data_ptr(), flat.data_ptr(), _stride(flat), _ptr(saved), _ptr(ws), size,
+                     _ptr(flags), 0, 0, 0, 0, 0, 0, 0)
+    _enqueue(_lib.lib().vy_gated_ffn_forward, call, index, "gated_ffn")
     _raise_on(flags, "gated_ffn")
     return saved
 
@@ -124,11 +179,12 @@ class _GatedFfn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w_gate, w_up, w_down, act, check):
         rows, wg, wu, wd = _rows(x, 8), _aligned(w_gate), _aligned(w_up), _aligned(w_down)
-        out = torch.empty(rows.shape[0], wd.shape[0], dtype=x.dtype, device=x.device)
-        saved = _ffn_forward(rows, wg, wu, wd, act, out, True, check)
+        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        flat = out if out.dim() == 2 else out.view(-1, x.shape[-1])
+        saved = _ffn_forward(rows, wg, wu, wd, act, flat, x.get_device(), True, check)
         ctx.save_for_backward(x, w_gate, w_up, w_down, saved)
         ctx.act, ctx.check = act, check
-        return out.view(x.shape)
+        return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -136,20 +192,22 @@ class _GatedFfn(torch.autograd.Function):
         x, w_gate, w_up, w_down, saved = ctx.saved_tensors
         rows, dy = _rows(x, 8), _rows(d_out, 8)
         wg, wu, wd = _aligned(w_gate), _aligned(w_up), _aligned(w_down)
-        c = _ffn_call(rows, wg, wu, wd, ctx.act)
-        c.saved = saved.data_ptr()
-        c.d_out, c.d_out_row_stride = dy.data_ptr(), _stride(dy)
-        grads = [torch.empty(t.shape, dtype=t.dtype, device=t.device) if need else None
-                 for t, need in zip((rows, wg, wu, wd), ctx.needs_input_grad)]
-        c.d_x, c.d_w_gate, c.d_w_up, c.d_w_down = map(_lib.ptr, grads)
-        c.d_x_row_stride = rows.shape[1]
-        flags = _flags(x.device, ctx.check)
-        c.flags = _lib.ptr(flags)
-        _run_ffn(c, True, x.device)
+        tokens, hidden = rows.shape
+        inter = wg.shape[0]
+        need = ctx.needs_input_grad
+        like = torch.empty_like
+        keep = torch.contiguous_format
+        d_x = like(x, memory_format=keep) if need[0] else None
+        d_wg, d_wu, d_wd = (like(w, memory_format=keep) if n else None for w, n in zip((wg, wu, wd), need[1:4]))
+        size = _ffn_workspace(tokens, hidden, inter, 1)
+        ws, flags = _workspace(size, rows), _flags(rows, ctx.check)
+        call = _FFN.pack(_CODE[rows.dtype], ctx.act, tokens, hidden, inter, rows.data_ptr(), _stride(rows),
+                         wg.data_ptr(), wu.data_ptr(), wd.data_ptr(), 0, 0, saved.data_ptr(), _ptr(ws), size,
+                         _ptr(flags), dy.data_ptr(), _stride(dy), _ptr(d_x), hidden, _ptr(d_wg), _ptr(d_wu),
+                         _ptr(d_wd))
+        _enqueue(_lib.lib().vy_gated_ffn_backward, call, x.get_device(), "gated_ffn backward")
         _raise_on(flags, "gated_ffn backward")
-        if grads[0] is not None:
-            grads[0] = grads[0].view(x.shape)
-        return (*grads, None, None)
+        return d_x, d_wg, d_wu, d_wd, None, None
 
 
 def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor,
@@ -163,24 +221,24 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
     and u (8 bytes per token and intermediate channel) for the backward pass; `out` is refused then.
     Rows of x may be strided; rows or weights that do not start on 16-byte boundaries are copied."""
     what = "gated_ffn"
-    code = _act_code(act, what)
-    _check_ffn(x, w_gate, w_up, w_down, what)
-    if x.dtype not in (torch.bfloat16, torch.float16) or any(w.dtype != x.dtype for w in (w_gate, w_up, w_down)):
-        raise NotImplementedError(f"{what}: x {x.dtype}, weights {w_gate.dtype}, {w_up.dtype}, {w_down.dtype} "
+    code = _activation(act, what)
+    hidden, inter = _check_ffn(x, w_gate, w_up, w_down, what)
+    dtype = x.dtype
+    if (dtype is not _BF16 and dtype is not _F16) or not (w_gate.dtype is w_up.dtype is w_down.dtype is dtype):
+        raise NotImplementedError(f"{what}: x {dtype}, weights {w_gate.dtype}, {w_up.dtype}, {w_down.dtype} "
                                   "(all bf16 or all fp16)")
-    if x.shape[-1] % 8 or w_gate.shape[0] % 8:
-        raise NotImplementedError(f"{what}: hidden {x.shape[-1]} and inter {w_gate.shape[0]} must be multiples of 8")
-    dev = _lib.require_cuda(x, w_gate, w_up, w_down, out, what=what)
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (x, w_gate, w_up, w_down)):
+    if hidden % 8 or inter % 8 or not hidden or not inter:
+        raise NotImplementedError(f"{what}: hidden {hidden} and inter {inter} must be multiples of 8")
+    index = _device(what, x, w_gate, w_up, w_down, out)
+    if torch.is_grad_enabled() and (x.requires_grad or w_gate.requires_grad or w_up.requires_grad
+                                    or w_down.requires_grad):
         if out is not None:
             raise RuntimeError(f"{what}: out= with gradients")
         return _GatedFfn.apply(x, w_gate, w_up, w_down, code, check)
-    rows = _rows(x, 8)
-    y = _output(out, x.shape, x.dtype, dev, what)
-    flat = y.view(-1, x.shape[-1]) if y.is_contiguous() else y
+    y, flat = _output(out, x, x.shape, dtype, what)
     if flat.data_ptr() % 16 or (flat.shape[0] > 1 and flat.stride(0) % 8):
         raise ValueError(f"{what}: out rows must start on 16-byte boundaries")
-    _ffn_forward(rows, _aligned(w_gate), _aligned(w_up), _aligned(w_down), code, flat, False, check)
+    _ffn_forward(_rows(x, 8), _aligned(w_gate), _aligned(w_up), _aligned(w_down), code, flat, index, False, check)
     return y
 
 
@@ -194,32 +252,30 @@ def quantize_int8(x: torch.Tensor) -> tuple:
     x / scale (ties to even), so the codes do not depend on how the division is carried out.  A zero
     row has codes 0 and scale 0; a row with an infinity or NaN has codes 0 and scale NaN."""
     what = "quantize_int8"
-    if x.dtype not in _FLOATS:
+    code = _CODE.get(x.dtype)
+    if code is None:
         raise NotImplementedError(f"{what}: x dtype {x.dtype} (bf16, fp16 or fp32)")
-    if x.dim() < 1 or x.shape[-1] == 0:
-        raise ValueError(f"{what}: x {tuple(x.shape)} has no values in a row")
-    dev = _lib.require_cuda(x, what=what)
-    rows = x.reshape(-1, x.shape[-1])
-    if rows.stride(1) != 1:
-        rows = rows.contiguous()
-    codes = torch.empty(x.shape, dtype=torch.int8, device=dev)
-    scale = torch.empty(*x.shape[:-1], 1, dtype=torch.float32, device=dev)
-    with torch.cuda.device(dev):
-        _lib.check(_lib.lib().vy_int8_quantize(rows.data_ptr(), _lib.DTYPE_CODE[x.dtype], _stride(rows), rows.shape[0],
-                                               rows.shape[1], codes.data_ptr(), scale.data_ptr(), _lib.stream_of(dev)),
-                   what)
+    shape = x.shape
+    if not shape or shape[-1] == 0:
+        raise ValueError(f"{what}: x {tuple(shape)} has no values in a row")
+    index = _device(what, x)
+    rows = _unit_rows(x)
+    codes = torch.empty(shape, dtype=_INT8, device=x.device)
+    scale = torch.empty((*shape[:-1], 1), dtype=_F32, device=x.device)
+    tokens, width = rows.shape
+    fn = _lib.lib().vy_int8_quantize
+    _enqueue(lambda call, stream: fn(*call, stream),
+             (rows.data_ptr(), code, rows.stride(0) if tokens > 1 else width, tokens, width, codes.data_ptr(),
+              scale.data_ptr()), index, what)
     return codes, scale
 
 
 def _scales(scale: torch.Tensor, n: int, what: str) -> torch.Tensor:
     if scale.numel() != n or not scale.is_floating_point():
         raise ValueError(f"{what}: {tuple(scale.shape)} {scale.dtype} scales for {n} rows")
-    return scale.reshape(-1).to(torch.float32).contiguous()
-
-
-def _int8(t: torch.Tensor, what: str) -> None:
-    if t.dtype != torch.int8:
-        raise NotImplementedError(f"{what}: codes of dtype {t.dtype} (int8)")
+    if scale.dtype is not _F32:
+        scale = scale.to(_F32)
+    return scale if scale.is_contiguous() else scale.contiguous()
 
 
 def int8_linear(codes: torch.Tensor, scale: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor,
@@ -232,39 +288,46 @@ def int8_linear(codes: torch.Tensor, scale: torch.Tensor, weight: torch.Tensor, 
     exact (int32); the scales and the bias are applied in fp32, in that order, and the result is
     rounded once to `dtype` (bf16, fp16 or fp32)."""
     what = "int8_linear"
-    _int8(codes, what), _int8(weight, what)
-    if codes.dim() < 1 or weight.dim() != 2 or weight.shape[1] != codes.shape[-1]:
+    if codes.dtype is not _INT8 or weight.dtype is not _INT8:
+        raise NotImplementedError(f"{what}: codes {codes.dtype}, weight {weight.dtype} (int8)")
+    shape = codes.shape
+    if not shape or weight.dim() != 2 or weight.shape[1] != shape[-1]:
         raise ValueError(f"{what}: codes {tuple(codes.shape)} and weight {tuple(weight.shape)}")
-    if dtype not in _FLOATS or (bias is not None and bias.dtype not in _FLOATS):
+    out_code = _CODE.get(dtype)
+    if out_code is None or (bias is not None and bias.dtype not in _CODE):
         raise NotImplementedError(f"{what}: dtype {dtype}, bias {None if bias is None else bias.dtype}")
     n, k = weight.shape
-    if k % 16 or not 0 < k < 131072 or n == 0:
-        raise NotImplementedError(f"{what}: K {k} must be a multiple of 16 below 131072 (N {n})")
-    if bias is not None and bias.shape != (n,):
-        raise ValueError(f"{what}: bias {tuple(bias.shape)} for {n} output channels")
-    dev = _lib.require_cuda(codes, scale, weight, weight_scale, bias, out, what=what)
-    rows, w = _rows(codes, 16), _aligned(weight)
-    bias = None if bias is None else bias.contiguous()
-    sx, sw = _scales(scale, rows.shape[0], what), _scales(weight_scale, n, what)
-    y = _output(out, (*codes.shape[:-1], n), dtype, dev, what)
-    flat = y.view(-1, n) if y.is_contiguous() else y
-    c = _lib.Int8LinearCall()
-    c.n_tokens, c.k, c.n = rows.shape[0], rows.shape[1], n
-    c.codes, c.codes_row_stride, c.scales = rows.data_ptr(), _stride(rows), sx.data_ptr()
-    c.weight, c.weight_scales = w.data_ptr(), sw.data_ptr()
+    if k % 16 or not 0 < k < _MAX_K or n == 0:
+        raise NotImplementedError(f"{what}: K {k} must be a multiple of 16 below {_MAX_K} (N {n})")
+    bias_code = 0
     if bias is not None:
-        c.bias, c.bias_dtype = bias.data_ptr(), _lib.DTYPE_CODE[bias.dtype]
-    c.out_dtype, c.out, c.out_row_stride = _lib.DTYPE_CODE[dtype], flat.data_ptr(), _stride(flat)
-    flags = _flags(dev, check)
-    c.flags = _lib.ptr(flags)
-    lib = _lib.lib()
-    with torch.cuda.device(dev):
-        c.workspace_bytes = lib.vy_int8_linear_workspace_size(ctypes.byref(c))
-        ws = torch.empty(c.workspace_bytes, dtype=torch.uint8, device=dev) if c.workspace_bytes else None
-        c.workspace = _lib.ptr(ws)
-        _lib.check(lib.vy_int8_linear(ctypes.byref(c), _lib.stream_of(dev)), what)
+        if bias.dim() != 1 or bias.shape[0] != n:
+            raise ValueError(f"{what}: bias {tuple(bias.shape)} for {n} output channels")
+        bias, bias_code = bias.contiguous(), _CODE[bias.dtype]
+    index = _device(what, codes, scale, weight, weight_scale, bias, out)
+    rows, w = _rows(codes, 16), _aligned(weight)
+    tokens = rows.shape[0]
+    sx, sw = _scales(scale, tokens, what), _scales(weight_scale, n, what)
+    y, flat = _output(out, codes, (*shape[:-1], n), dtype, what)
+    flags = _flags(codes, check)
+    call = _LINEAR.pack(tokens, k, n, rows.data_ptr(), _stride(rows), sx.data_ptr(), w.data_ptr(), sw.data_ptr(),
+                        _ptr(bias), bias_code, out_code, flat.data_ptr(), _stride(flat), 0, 0, _ptr(flags))
+    _enqueue(_lib.lib().vy_int8_linear, call, index, what)
     _raise_on(flags, what)
     return y
+
+
+_INT8_FFN_SIZES: dict = {}      # (tokens, hidden, inter) -> workspace bytes
+
+
+def _int8_ffn_workspace(key: tuple) -> int:
+    size = _INT8_FFN_SIZES.get(key)
+    if size is None:
+        if len(_INT8_FFN_SIZES) >= 4096:
+            _INT8_FFN_SIZES.clear()
+        size = _INT8_FFN_SIZES[key] = _lib.lib().vy_int8_gated_ffn_workspace_size(
+            _INT8_FFN.pack(0, 0, *key, *(0,) * 13))
+    return size
 
 
 def int8_gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, gate_scale: torch.Tensor, w_up: torch.Tensor,
@@ -277,37 +340,25 @@ def int8_gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, gate_scale: torch.Tens
     hidden and inter multiples of 16; scales [rows] or [rows, 1].  Returns [..., hidden] in x's type.
     No gradients."""
     what = "int8_gated_ffn"
-    code = _act_code(act, what)
-    for w in (w_gate, w_up, w_down):
-        _int8(w, what)
-    _check_ffn(x, w_gate, w_up, w_down, what)
-    if x.dtype not in (torch.bfloat16, torch.float16):
-        raise NotImplementedError(f"{what}: x dtype {x.dtype} (bf16 or fp16)")
-    if any(d % 16 or not 0 < d < 131072 for d in w_gate.shape):
-        raise NotImplementedError(f"{what}: inter and hidden {tuple(w_gate.shape)} must be multiples of 16 below 131072")
-    dev = _lib.require_cuda(x, w_gate, gate_scale, w_up, up_scale, w_down, down_scale, out, what=what)
-    rows = x.reshape(-1, x.shape[-1])
-    if rows.stride(1) != 1:
-        rows = rows.contiguous()
-    wg, wu, wd = _aligned(w_gate), _aligned(w_up), _aligned(w_down)
-    inter, hidden = wg.shape
+    code = _activation(act, what)
+    if not (w_gate.dtype is w_up.dtype is w_down.dtype is _INT8):
+        raise NotImplementedError(f"{what}: weights {w_gate.dtype}, {w_up.dtype}, {w_down.dtype} (int8)")
+    hidden, inter = _check_ffn(x, w_gate, w_up, w_down, what)
+    dtype = x.dtype
+    if dtype is not _BF16 and dtype is not _F16:
+        raise NotImplementedError(f"{what}: x dtype {dtype} (bf16 or fp16)")
+    if hidden % 16 or inter % 16 or not 0 < hidden < _MAX_K or not 0 < inter < _MAX_K:
+        raise NotImplementedError(f"{what}: hidden {hidden} and inter {inter} must be multiples of 16 below {_MAX_K}")
+    index = _device(what, x, w_gate, gate_scale, w_up, up_scale, w_down, down_scale, out)
+    rows, wg, wu, wd = _unit_rows(x), _aligned(w_gate), _aligned(w_up), _aligned(w_down)
     sg, su, sd = _scales(gate_scale, inter, what), _scales(up_scale, inter, what), _scales(down_scale, hidden, what)
-    y = _output(out, x.shape, x.dtype, dev, what)
-    flat = y.view(-1, hidden) if y.is_contiguous() else y
-    c = _lib.Int8FfnCall()
-    c.act_dtype, c.activation = _lib.DTYPE_CODE[x.dtype], code
-    c.n_tokens, c.hidden, c.inter = rows.shape[0], hidden, inter
-    c.x, c.x_row_stride = rows.data_ptr(), _stride(rows)
-    c.w_gate, c.w_up, c.w_down = wg.data_ptr(), wu.data_ptr(), wd.data_ptr()
-    c.gate_scales, c.up_scales, c.down_scales = sg.data_ptr(), su.data_ptr(), sd.data_ptr()
-    c.out, c.out_row_stride = flat.data_ptr(), _stride(flat)
-    flags = _flags(dev, check)
-    c.flags = _lib.ptr(flags)
-    lib = _lib.lib()
-    with torch.cuda.device(dev):
-        c.workspace_bytes = lib.vy_int8_gated_ffn_workspace_size(ctypes.byref(c))
-        ws = torch.empty(c.workspace_bytes, dtype=torch.uint8, device=dev)
-        c.workspace = ws.data_ptr()
-        _lib.check(lib.vy_int8_gated_ffn(ctypes.byref(c), _lib.stream_of(dev)), what)
+    y, flat = _output(out, x, x.shape, dtype, what)
+    tokens = rows.shape[0]
+    size = _int8_ffn_workspace((tokens, hidden, inter))
+    ws, flags = _workspace(size, rows), _flags(rows, check)
+    call = _INT8_FFN.pack(_CODE[dtype], code, tokens, hidden, inter, rows.data_ptr(), _stride(rows), wg.data_ptr(),
+                          wu.data_ptr(), wd.data_ptr(), sg.data_ptr(), su.data_ptr(), sd.data_ptr(), flat.data_ptr(),
+                          _stride(flat), _ptr(ws), size, _ptr(flags))
+    _enqueue(_lib.lib().vy_int8_gated_ffn, call, index, what)
     _raise_on(flags, what)
     return y
