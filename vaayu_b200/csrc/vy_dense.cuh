@@ -8,27 +8,22 @@ namespace vy {
 
 // ── activations of a gated block and their derivatives (fp32) ───────────────────────────────
 
-__device__ __forceinline__ float gelu_inner(float g) {
-    // tanh is +-1 to the last bit well inside +-16; the clamp keeps g^3 finite
-    const float c = fminf(fmaxf(g, -16.f), 16.f);
-    return 0.7978845608028654f * (c + 0.044715f * c * c * c);
+// Both are g times a sigmoid: silu(g) = g s(g), and since (1 + tanh v) / 2 = s(2v), gelu_tanh(g) =
+// g s(2 sqrt(2/pi) (g + 0.044715 g^3)).  One exponential and one approximate division (2 ulp): no
+// branch, so the loads of a tile's other columns are not held up behind it.
+__device__ __forceinline__ float sigmoid(float z) { return __fdividef(1.f, 1.f + expf(-z)); }
+__device__ __forceinline__ float gate_arg(float g, int act) {
+    return act == VY_ACT_SILU ? g : 1.5957691216057308f * (g + 0.044715f * g * g * g);
 }
-// silu(g) = g / (1 + e^-g); gelu_tanh(g) = g (1 + tanh(sqrt(2/pi) (g + 0.044715 g^3))) / 2
-__device__ __forceinline__ float gate_act(float g, int act) {
-    if (act == VY_ACT_SILU) return g / (1.f + expf(-g));
-    return 0.5f * g * (1.f + tanhf(gelu_inner(g)));
-}
-// (value, derivative)
+__device__ __forceinline__ float gate_act(float g, int act) { return g * sigmoid(gate_arg(g, act)); }
+// (value, derivative): d(g s(z)) = s + g s (1 - s) z'
 __device__ __forceinline__ float2 gate_act_grad(float g, int act) {
-    if (act == VY_ACT_SILU) {
-        const float s = 1.f / (1.f + expf(-g));
-        return make_float2(g * s, s * (1.f + g * (1.f - s)));
-    }
-    const float t = tanhf(gelu_inner(g));
+    const float s = sigmoid(gate_arg(g, act));
+    // beyond +-16 gelu's s (1 - s) is zero; the clamp keeps z' finite there
     const float c = fminf(fmaxf(g, -16.f), 16.f);
-    // beyond the clamp 1 - t^2 is zero, so the clamped factor beside it changes nothing
-    const float d = 0.5f * (1.f + t) + 0.5f * c * (1.f - t * t) * 0.7978845608028654f * (1.f + 0.134145f * c * c);
-    return make_float2(0.5f * g * (1.f + t), (g != g) ? g : d);
+    const float dz = act == VY_ACT_SILU ? 1.f : 1.5957691216057308f + 0.21406859462151464f * c * c;
+    const float gs = g * s;
+    return make_float2(gs, s + gs * (1.f - s) * dz);
 }
 
 template <int ACT>

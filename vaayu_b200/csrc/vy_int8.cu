@@ -11,9 +11,6 @@ namespace vy {
 namespace {
 
 constexpr int kMaxK = 131072;      // 128 * 128 * k stays below 2^31
-constexpr int kQuantThreads = 256;
-constexpr int kQuantVecs = 4;      // 16-value pieces of a row a thread holds in registers
-
 size_t align256(size_t v) { return (v + 255) & ~size_t(255); }
 
 // ── quantisation ────────────────────────────────────────────────────────────────────────────
@@ -23,128 +20,205 @@ struct QuantParams {
     int64_t x_stride, rows, cols;
     int8_t* codes;
     float* scales;
-    bool vec;      // rows and codes take 16-byte accesses
+    bool vec;      // rows take 16-byte loads, codes the stores that go with them
 };
 
-// Nearest integer of the exact quotient x / s, ties to even.  t = x * (1/s) is within 2.3e-5 of
-// x / s (two roundings of a value up to 127.5), so it decides every value that is not that near a
-// tie; the rest (about one in 10^4) are divided in fp64, which separates any quotient of two fp32
-// numbers from a tie.  `tiny`: 1 / s is out of range, fp64 for all.
-__device__ __forceinline__ int quant_code(float x, float s, float inv, bool tiny) {
-    float t = x * inv;
-    float r = rintf(t);
-    if (tiny || fabsf(fabsf(t - r) - 0.5f) < 1e-4f) r = static_cast<float>(rint(double(x) / double(s)));
-    return static_cast<int>(fminf(fmaxf(r, -127.f), 127.f));
-}
+// A code is the nearest integer of the exact quotient x / s, ties to even.  t = x * (1/s) is off by
+// at most 2^-23 relative (two roundings), 1.6e-5 for |t| <= 127.5, so rounding t decides every value
+// that is not that near a tie c; for the rest (about one in 20,000) the sign of x - c s decides, which
+// one fused multiply-add gives exactly (c s and the difference are exact before its one rounding, and
+// nothing underflows at these scales).  Adding 1.5 * 2^23 rounds t to the nearest integer, even on
+// ties, and leaves its two's complement in the low bits: no conversion instruction, whose rate would
+// bound the kernel (rint and float-to-int run at an eighth of the adds' rate).
+constexpr float kRound = 12582912.f;
+constexpr float kNearTie = 0.5f - 3e-5f;
 
-template <int DT>
-__device__ __forceinline__ void load16(const void* x, int64_t at, float (&v)[16]) {
-    if constexpr (DT == VY_F32) {
-        const float4* p = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(x) + at);
+struct RowScale {
+    float s, inv;
+    float up;       // 1, or 2^100 where 1 / s is out of range: x and s are scaled by it, exactly
+    bool zero;      // a zero row, or a NaN scale: all codes 0
+};
+
+// The codes of N values, N / 4 words.
+template <int N>
+__device__ __forceinline__ void quant_words(const float (&v)[N], const RowScale& r, uint32_t (&w)[N / 4]) {
+    float far = 0.f;
+    float m[N];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            const float4 f = p[q];
-            v[4 * q] = f.x, v[4 * q + 1] = f.y, v[4 * q + 2] = f.z, v[4 * q + 3] = f.w;
-        }
-    } else {
-        const uint4* p = reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(x) + at);
+    for (int j = 0; j < N; ++j) {
+        const float t = v[j] * r.inv;
+        m[j] = t + kRound;
+        far = fmaxf(far, fabsf(t - (m[j] - kRound)));
+    }
+    if (far > kNearTie || r.up != 1.f) {
 #pragma unroll
-        for (int q = 0; q < 2; ++q) {
-            const uint4 u = p[q];
-            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                v[8 * q + 2 * j] = act_from_bits<DT>(w[j] & 0xFFFFu);
-                v[8 * q + 2 * j + 1] = act_from_bits<DT>(w[j] >> 16);
+        for (int j = 0; j < N; ++j) {
+            const float x = v[j] * r.up, s = r.s * r.up;
+            const float t = r.up != 1.f ? x * __frcp_rn(s) : v[j] * r.inv;
+            const float near = (t + kRound) - kRound, d = t - near;
+            float q = near;
+            if (fabsf(d) > kNearTie) {
+                const float c = near + copysignf(0.5f, d);
+                const float e = fmaf(-c, s, x);
+                q = e > 0.f ? c + 0.5f : e < 0.f ? c - 0.5f : c;     // c + kRound goes to the even one
             }
+            // a subnormal s may be so coarse that amax / s passes 127
+            m[j] = fminf(fmaxf(q, -127.f), 127.f) + kRound;
         }
+    }
+#pragma unroll
+    for (int q = 0; q < N / 4; ++q) {
+        const uint32_t lo = __byte_perm(__float_as_uint(m[4 * q]), __float_as_uint(m[4 * q + 1]), 0x0040);
+        const uint32_t hi = __byte_perm(__float_as_uint(m[4 * q + 2]), __float_as_uint(m[4 * q + 3]), 0x0040);
+        w[q] = r.zero ? 0u : __byte_perm(lo, hi, 0x5410);
     }
 }
 
-// One block per row.
+// Plain (coherent) 16-byte load: x may come from the kernel in front, which this one overlaps.
+__device__ __forceinline__ uint4 ld_piece(const uint4* p) {
+    uint4 v;
+    asm volatile("ld.global.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+
+// Values of one 16-byte piece, and their largest magnitude's bit pattern (magnitudes order like
+// their patterns, NaN above infinity: an integer maximum).
 template <int DT>
-__global__ void __launch_bounds__(kQuantThreads) quantize_kernel(QuantParams p) {
-    __shared__ uint32_t part[kQuantThreads / 32];
+struct Piece {
+    static constexpr int N = DT == VY_F32 ? 4 : 8;
+    static __device__ __forceinline__ void values(const uint4& u, float (&v)[N]) {
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if constexpr (DT == VY_F32) {
+                v[j] = __uint_as_float(w[j]);
+            } else if constexpr (DT == VY_BF16) {
+                v[2 * j] = __uint_as_float(w[j] << 16);
+                v[2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u);
+            } else {
+                v[2 * j] = act_from_bits<VY_F16>(w[j] & 0xFFFFu);
+                v[2 * j + 1] = act_from_bits<VY_F16>(w[j] >> 16);
+            }
+        }
+    }
+    // 16-bit types: of each half in place (the two maxima of a word never mix), fp32: of the word
+    static __device__ __forceinline__ uint32_t top(uint32_t t, const uint4& u) {
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if constexpr (DT == VY_F32)
+                t = max(t, w[j] & 0x7FFFFFFFu);
+            else
+                t = __vmaxu2(t, w[j] & 0x7FFF7FFFu);
+        }
+        return t;
+    }
+    // the fp32 magnitude's pattern from top's
+    static __device__ __forceinline__ uint32_t wide(uint32_t t) {
+        if constexpr (DT == VY_F32) return t;
+        const uint32_t h = max(t & 0xFFFFu, t >> 16);
+        return __float_as_uint(act_from_bits<DT>(h)) & 0x7FFFFFFFu;
+    }
+};
+
+// One block per row; the row stays in registers between its maximum and its codes.
+template <int DT, int THREADS, int UNITS>
+__global__ void __launch_bounds__(THREADS) quantize_kernel(QuantParams p) {
+    using P = Piece<DT>;
+    __shared__ uint32_t part[THREADS / 32];
     grid_dependency_wait();
     grid_dependents_launch();
     const int64_t row = blockIdx.x;
-    const int64_t base = row * p.x_stride;
     const int tid = threadIdx.x;
-    // magnitudes order like their bit patterns, NaN above infinity: one integer maximum
+    const int64_t size = DT == VY_F32 ? 4 : 2;
+    const unsigned char* src = reinterpret_cast<const unsigned char*>(p.x) + row * p.x_stride * size;
+    const uint4* pieces = reinterpret_cast<const uint4*>(src);
+    const int64_t n = p.vec ? p.cols / P::N : 0;
+    const bool fits = n <= int64_t(UNITS) * THREADS;
+    uint4 keep[UNITS];
     uint32_t top = 0;
-    float keep[kQuantVecs][16];
-    const int64_t pieces = p.vec ? p.cols / 16 : 0;
-    const bool fits = pieces <= int64_t(kQuantVecs) * kQuantThreads;
     if (fits) {
 #pragma unroll
-        for (int i = 0; i < kQuantVecs; ++i) {
-            const int64_t at = tid + int64_t(i) * kQuantThreads;
-            if (at < pieces) {
-                load16<DT>(p.x, base + at * 16, keep[i]);
-#pragma unroll
-                for (int j = 0; j < 16; ++j) top = max(top, __float_as_uint(keep[i][j]) & 0x7FFFFFFFu);
-            }
+        for (int i = 0; i < UNITS; ++i) {
+            const int64_t at = tid + i * THREADS;
+            keep[i] = at < n ? ld_piece(pieces + at) : make_uint4(0, 0, 0, 0);
         }
+#pragma unroll
+        for (int i = 0; i < UNITS; ++i) top = P::top(top, keep[i]);
     } else {
-        for (int64_t at = tid; at < pieces; at += kQuantThreads) {
-            float v[16];
-            load16<DT>(p.x, base + at * 16, v);
-#pragma unroll
-            for (int j = 0; j < 16; ++j) top = max(top, __float_as_uint(v[j]) & 0x7FFFFFFFu);
-        }
+        for (int64_t at = tid; at < n; at += THREADS) top = P::top(top, ld_piece(pieces + at));
     }
-    for (int64_t k = pieces * 16 + tid; k < p.cols; k += kQuantThreads)
-        top = max(top, __float_as_uint(load_as_float(p.x, DT, base + k)) & 0x7FFFFFFFu);
+    top = P::wide(top);
+    for (int64_t k = n * P::N + tid; k < p.cols; k += THREADS)
+        top = max(top, __float_as_uint(load_as_float(src, DT, k)) & 0x7FFFFFFFu);
     top = __reduce_max_sync(0xffffffffu, top);
     if ((tid & 31) == 0) part[tid >> 5] = top;
     __syncthreads();
-#pragma unroll
-    for (int w = 0; w < kQuantThreads / 32; ++w) top = max(top, part[w]);
+    top = __reduce_max_sync(0xffffffffu, part[(tid & 31) % (THREADS / 32)]);
 
-    const bool finite = top < 0x7F800000u;
-    const float scale = finite ? __fdiv_rn(__uint_as_float(top), 127.f) : __uint_as_float(0x7FC00000u);
-    if (tid == 0) p.scales[row] = scale;
-    const bool zero = !(scale > 0.f);          // a zero row, or NaN
-    const bool tiny = scale < 1e-30f;
-    const float inv = zero || tiny ? 0.f : __fdiv_rn(1.f, scale);
+    RowScale r;
+    r.s = top < 0x7F800000u ? __fdiv_rn(__uint_as_float(top), 127.f) : __uint_as_float(0x7FC00000u);
+    r.zero = !(r.s > 0.f);
+    r.up = r.s < 1e-30f && !r.zero ? 0x1p100f : 1.f;
+    r.inv = r.zero || r.up != 1.f ? 0.f : __frcp_rn(r.s);
+    if (tid == 0) p.scales[row] = r.s;
     int8_t* out = p.codes + row * p.cols;
-    auto put16 = [&](int64_t at, const float (&v)[16]) {
-        uint32_t w[4];
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            w[q] = 0;
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                w[q] |= (zero ? 0u : uint32_t(quant_code(v[4 * q + j], scale, inv, tiny)) & 0xFFu) << (8 * j);
-        }
-        *reinterpret_cast<uint4*>(out + at * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+    auto put = [&](int64_t at, const uint4& u) {
+        float v[P::N];
+        uint32_t w[P::N / 4];
+        P::values(u, v);
+        quant_words<P::N>(v, r, w);
+        if constexpr (P::N == 8)
+            reinterpret_cast<uint2*>(out)[at] = make_uint2(w[0], w[1]);
+        else
+            reinterpret_cast<uint32_t*>(out)[at] = w[0];
     };
     if (fits) {
 #pragma unroll
-        for (int i = 0; i < kQuantVecs; ++i) {
-            const int64_t at = tid + int64_t(i) * kQuantThreads;
-            if (at < pieces) put16(at, keep[i]);
+        for (int i = 0; i < UNITS; ++i) {
+            const int64_t at = tid + i * THREADS;
+            if (at < n) put(at, keep[i]);
         }
     } else {
-        for (int64_t at = tid; at < pieces; at += kQuantThreads) {
-            float v[16];
-            load16<DT>(p.x, base + at * 16, v);
-            put16(at, v);
-        }
+        for (int64_t at = tid; at < n; at += THREADS) put(at, ld_piece(pieces + at));
     }
-    for (int64_t k = pieces * 16 + tid; k < p.cols; k += kQuantThreads)
-        out[k] = static_cast<int8_t>(zero ? 0 : quant_code(load_as_float(p.x, DT, base + k), scale, inv, tiny));
+    for (int64_t k = n * P::N + tid; k < p.cols; k += THREADS) {
+        const float v[4] = {load_as_float(src, DT, k), 0.f, 0.f, 0.f};
+        uint32_t w[1];
+        quant_words<4>(v, r, w);
+        out[k] = static_cast<int8_t>(w[0] & 0xFFu);
+    }
+}
+
+template <int DT>
+int launch_quantize_as(const QuantParams& p, int sm_count, cudaStream_t s) {
+    const int64_t n = p.cols / Piece<DT>::N;
+    // Threads of a row's block, and 16-byte pieces each keeps in registers: enough that the row fits;
+    // with fewer rows than SMs, as many threads as the row can use, since one block's latency is the
+    // call's.  (A row past 8192 pieces is read twice.)
+    const bool few = p.rows <= sm_count;
+    void (*kern)(QuantParams) = quantize_kernel<DT, 1024, 8>;
+    int threads = 1024;
+    if (few ? n <= 64 : n <= 128)
+        kern = quantize_kernel<DT, 64, 2>, threads = 64;
+    else if (few ? n <= 256 : n <= 512)
+        kern = quantize_kernel<DT, 256, 2>, threads = 256;
+    else if (few && n <= 2048)
+        kern = quantize_kernel<DT, 1024, 2>, threads = 1024;
+    else if (n <= 2048)
+        kern = quantize_kernel<DT, 512, 4>, threads = 512;
+    const cudaError_t e = launch_chained(kern, dim3(static_cast<unsigned>(p.rows)), dim3(threads), 0, s, p);
+    return e == cudaSuccess ? VY_OK : fail(VY_ERR_CUDA, "int8 quantise launch: %s", cudaGetErrorString(e));
 }
 
 int launch_quantize(const void* x, int dtype, int64_t stride, int64_t rows, int64_t cols, int8_t* codes, float* scales,
-                    cudaStream_t s) {
+                    int sm_count, cudaStream_t s) {
     QuantParams p{x, stride, rows, cols, codes, scales, false};
     const int64_t size = dtype == VY_F32 ? 4 : 2;
-    p.vec = aligned16(x) && (rows == 1 || (stride * size) % 16 == 0) && aligned16(codes) && (rows == 1 || cols % 16 == 0);
-    auto kern = dtype == VY_F32 ? quantize_kernel<VY_F32> : dtype == VY_F16 ? quantize_kernel<VY_F16> : quantize_kernel<VY_BF16>;
-    const cudaError_t e = launch_chained(kern, dim3(static_cast<unsigned>(rows)), dim3(kQuantThreads), 0, s, p);
-    if (e != cudaSuccess) return fail(VY_ERR_CUDA, "int8 quantise launch: %s", cudaGetErrorString(e));
-    return VY_OK;
+    p.vec = aligned16(x) && (rows == 1 || (stride * size) % 16 == 0) && aligned16(codes) && (rows == 1 || cols % 8 == 0);
+    return dtype == VY_F32   ? launch_quantize_as<VY_F32>(p, sm_count, s)
+           : dtype == VY_F16 ? launch_quantize_as<VY_F16>(p, sm_count, s)
+                             : launch_quantize_as<VY_BF16>(p, sm_count, s);
 }
 
 // ── products ────────────────────────────────────────────────────────────────────────────────
@@ -287,8 +361,9 @@ extern "C" int vy_int8_quantize(const void* x, int32_t x_dtype, int64_t x_row_st
     if (rows > 0x7FFFFFFFll) return fail(VY_ERR_UNSUPPORTED, "rows %lld", (long long)rows);
     if (rows == 0) return ok();
     if (!x || !codes || !scales) return fail(VY_ERR_INVALID, "null operand");
-    if (!device_info(&st)) return st;
-    st = launch_quantize(x, x_dtype, x_row_stride, rows, cols, codes, scales, as_stream(stream));
+    const DeviceInfo* dev = device_info(&st);
+    if (!dev) return st;
+    st = launch_quantize(x, x_dtype, x_row_stride, rows, cols, codes, scales, dev->sm_count, as_stream(stream));
     return st != VY_OK ? st : check_launch("vy_int8_quantize");
 }
 
@@ -320,11 +395,11 @@ extern "C" int vy_int8_gated_ffn(const vy_int8_ffn_call* c, void* stream) {
     cudaStream_t s = as_stream(stream);
     const FfnLayout L = ffn_layout(
         c, reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(c->workspace) + 255) & ~uintptr_t(255)));
-    VY_TRY(launch_quantize(c->x, c->act_dtype, c->x_row_stride, c->n_tokens, c->hidden, L.x_codes, L.x_scales, s));
+    VY_TRY(launch_quantize(c->x, c->act_dtype, c->x_row_stride, c->n_tokens, c->hidden, L.x_codes, L.x_scales, dev->sm_count, s));
     Product gu{L.x_codes, c->hidden, L.x_scales, {c->w_gate, c->w_up}, {c->gate_scales, c->up_scales}, c->n_tokens,
                c->hidden, c->inter, L.h, c->inter, VY_F32, c->activation, nullptr, 0, c->flags};
     VY_TRY(launch_product<true>(gu, false, dev, s));
-    VY_TRY(launch_quantize(L.h, VY_F32, c->inter, c->n_tokens, c->inter, L.h_codes, L.h_scales, s));
+    VY_TRY(launch_quantize(L.h, VY_F32, c->inter, c->n_tokens, c->inter, L.h_codes, L.h_scales, dev->sm_count, s));
     Product down{L.h_codes, c->inter, L.h_scales, {c->w_down, nullptr}, {c->down_scales, nullptr}, c->n_tokens, c->inter,
                  c->hidden, c->out, c->out_row_stride, c->act_dtype, 0, nullptr, 0, c->flags};
     VY_TRY(launch_product<false>(down, false, dev, s));

@@ -5,15 +5,14 @@
 // its N, rounded up to 16.  Weight tiles arrive by TMA in a ring deep enough to keep about 100 KB in
 // flight per CTA, two CTAs on an SM; HBM needs about 45 KB an SM in flight at its latency.
 //
-// K is split over the CTAs of a cluster: each accumulates its share in TMEM, leaves the sums in its
-// shared memory, and after one cluster barrier every CTA adds a slice of the rows over all shares, in
-// rank order, through distributed shared memory.  No workspace, no atomics, one order of summation.
+// K is split over the CTAs of a cluster: each accumulates its share in TMEM and writes the sums of
+// every slice of the rows into the shared memory of the CTA that owns the slice; after one cluster
+// barrier each CTA adds its slice over all shares, in rank order.  No workspace, no atomics, one
+// order of summation, and no remote read to wait for.
 //
 // A kernel that is not the first of its call starts loading weights before the kernel in front of it
 // has finished (they do not depend on it); its token tiles wait for it.
 #pragma once
-
-#include <cstdlib>
 
 #include "vy_dense.cuh"
 
@@ -23,12 +22,14 @@ constexpr int kStreamRows = 128;        // weight rows of a unit (of each matrix
 constexpr int kStreamMaxTokens = 128;
 constexpr int kStreamThreads = 192;     // warps 0-3 read the sums, 4 loads, 5 issues the MMAs
 constexpr int kStreamMaxStages = 12;
+constexpr int kSmemMost = 226 * 1024, kSmemHalf = 112 * 1024;   // dynamic bytes of one CTA, of two on an SM
 
 struct StreamParams {
     CUtensorMap w[2], x;
     int tokens, n, nk;      // nk: K blocks of 128 bytes
     int cols;               // MMA N: tokens rounded up to 16
     int stages, tmem_cols;
+    int sums_at;            // offset of the received sums in dynamic shared memory
     int early;              // weights may be loaded before the previous kernel has finished
     EpiParams epi;
     int32_t* flags;
@@ -56,21 +57,19 @@ __device__ __forceinline__ void stream_put(const StreamParams& p, int row, int t
     } else if constexpr (EPI == EPI_STORE) {
         reinterpret_cast<uint16_t*>(e.out)[at] = static_cast<uint16_t>(act_bits<ACT>(__uint_as_float(s0)));
     } else if constexpr (EPI == EPI_I8GATE) {
-        const float rs = __ldg(e.row_scale + t);
-        const float g = __fmul_rn(__fmul_rn(float(int(s0)), rs), __ldg(e.col_scale[0] + row));
-        const float u = __fmul_rn(__fmul_rn(float(int(s1)), rs), __ldg(e.col_scale[1] + row));
+        const float rs = e.row_scale[t];
+        const float g = __fmul_rn(__fmul_rn(float(int(s0)), rs), e.col_scale[0][row]);
+        const float u = __fmul_rn(__fmul_rn(float(int(s1)), rs), e.col_scale[1][row]);
         reinterpret_cast<float*>(e.out)[at] = gate_act(g, e.act) * u;
     } else {
-        float v = __fmul_rn(__fmul_rn(float(int(s0)), __ldg(e.row_scale + t)), __ldg(e.col_scale[0] + row));
+        float v = __fmul_rn(__fmul_rn(float(int(s0)), e.row_scale[t]), e.col_scale[0][row]);
         if (e.bias) v = __fadd_rn(v, load_as_float(e.bias, e.bias_dtype, row));
         store_as(e.out, e.out_dtype, at, v);
     }
 }
 
-__device__ __forceinline__ uint32_t ld_cluster(uint32_t addr) {
-    uint32_t v;
-    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr));
-    return v;
+__device__ __forceinline__ void st_cluster(uint32_t addr, uint32_t v) {
+    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
 }
 
 template <int EPI, int ACT>
@@ -101,9 +100,16 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(const __grid_con
         S.abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    if (warp == 4 && lane == 0) {
+        prefetch_map(&p.w[0]);
+        if (NW == 2) prefetch_map(&p.w[1]);
+        prefetch_map(&p.x);
+    }
     if (warp == 0) tmem_alloc_n<0>(&S.tmem_base, p.tmem_cols);
     tc_fence_before();
     __syncthreads();
+    // waited for before the first write into another CTA's shared memory: it has started by then
+    if (splits > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
     tc_fence_after();
     const uint32_t tmem = S.tmem_base;
     volatile int* abort_flag = &S.abort_flag;
@@ -171,14 +177,17 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(const __grid_con
     }
     __syncwarp();
 
-    // sums [matrix][token][row] in shared memory, rows fastest (a warp's lanes are rows)
-    uint32_t* part = reinterpret_cast<uint32_t*>(ring);
-    bool ready = true;
+    // received sums [share][matrix][token][row of my slice], rows fastest
+    const int rows = kStreamRows / splits;      // 1, 2, 4 or 8 shares
+    uint32_t* sums = reinterpret_cast<uint32_t*>(ring + p.sums_at);
+    if (splits > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
     if (warp < 4) {
-        ready = __all_sync(0xffffffffu, mbar_wait(&S.done, 0, abort_flag, p.flags));
+        const bool ready = __all_sync(0xffffffffu, mbar_wait(&S.done, 0, abort_flag, p.flags));
         tc_fence_after();
         const uint32_t lanes = uint32_t(warp * 32) << 16;
         const int row = warp * 32 + lane;
+        const uint32_t owner = map_to_rank(smem_u32(sums), row / rows) +
+                               4u * (rank * NW * p.tokens * rows + row % rows);
         if (ready) {
             for (int c = 0; c < p.cols; c += 16) {
                 uint32_t v[NW][16];
@@ -186,12 +195,6 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(const __grid_con
                 for (int m = 0; m < NW; ++m) tmem_ld16(tmem + lanes + m * p.cols + c, v[m]);
 #pragma unroll
                 for (int m = 0; m < NW; ++m) tmem_wait16(v[m]);
-                if (nk == 0) {      // a share of no K blocks: TMEM holds nothing of this call
-#pragma unroll
-                    for (int m = 0; m < NW; ++m)
-#pragma unroll
-                        for (int j = 0; j < 16; ++j) v[m][j] = 0;
-                }
                 if (splits == 1) {
                     if (row0 + row < p.n) {
 #pragma unroll
@@ -203,37 +206,32 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(const __grid_con
                     for (int m = 0; m < NW; ++m)
 #pragma unroll
                         for (int j = 0; j < 16; ++j)
-                            if (c + j < p.tokens) part[(m * p.cols + c + j) * kStreamRows + row] = v[m][j];
+                            if (c + j < p.tokens) st_cluster(owner + 4u * ((m * p.tokens + c + j) * rows), v[m][j]);
                 }
             }
         }
         tc_fence_before();
     }
+    __syncwarp();
     if (splits > 1) {
         cluster_sync();
-        const int rows = kStreamRows / splits, first = rank * rows;      // 2, 4 or 8 shares: a power of two
-        const uint32_t base = smem_u32(part);
+        const int share = NW * p.tokens * rows;
         for (int q = tid; q < rows * p.tokens; q += kStreamThreads) {
-            const int row = first + q % rows, t = q / rows;
+            const int row = int(rank) * rows + q % rows, t = q / rows;
             if (row0 + row >= p.n) continue;
             uint32_t sum[NW];
 #pragma unroll
             for (int m = 0; m < NW; ++m) {
-                const uint32_t at = base + 4u * ((m * p.cols + t) * kStreamRows + row);
-                uint32_t v[8];
-#pragma unroll
-                for (uint32_t r = 0; r < 8; ++r)
-                    if (r < splits) v[r] = ld_cluster(map_to_rank(at, r));
-                uint32_t acc = v[0];
-#pragma unroll
-                for (uint32_t r = 1; r < 8; ++r)
-                    if (r < splits)
-                        acc = I8 ? acc + v[r] : __float_as_uint(__fadd_rn(__uint_as_float(acc), __uint_as_float(v[r])));
+                const uint32_t* at = sums + (m * p.tokens + t) * rows + q % rows;
+                uint32_t acc = at[0];
+                for (uint32_t r = 1; r < splits; ++r) {
+                    const uint32_t v = at[r * share];
+                    acc = I8 ? acc + v : __float_as_uint(__fadd_rn(__uint_as_float(acc), __uint_as_float(v)));
+                }
                 sum[m] = acc;
             }
             stream_put<EPI, ACT>(p, row0 + row, t, sum[0], sum[NW - 1]);
         }
-        cluster_sync();      // no CTA leaves while another still reads its sums
     } else {
         __syncthreads();
     }
@@ -243,13 +241,30 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(const __grid_con
 
 // ── host ────────────────────────────────────────────────────────────────────────────────────
 
-// CTAs that share a unit's K.
-inline int stream_splits(int64_t n, int nk, int sm_count) {
-    const int64_t units = (n + kStreamRows - 1) / kStreamRows;
-    int s = 1;
-    while (s < 8 && units * s < sm_count && nk >= 4 * s) s *= 2;
-    if (const char* e = getenv("VY_SPLITS")) s = atoi(e);
-    return s;
+// How a call is laid out on the machine: CTAs that share a unit's K, ring stages, shared memory.
+struct StreamPlan {
+    int splits, stages, sums, stage;
+};
+// The most shares (up to 8) whose CTAs are all resident at once: a second round would leave the
+// memory system idle while its CTAs start and join.  Two CTAs run on an SM (and the next kernel's
+// first ones start under this kernel's last) while ring and received sums take half its shared
+// memory.  Up to 32 tokens two stages a CTA are enough for that (16 x 7168 x 2048, bf16: 27.5 us
+// against 32.3 with one deep ring an SM); with more, the token tiles crowd the ring, and one CTA with
+// five stages is faster than two with two (64 x 4096 x 14336: 82 us against 99).
+inline StreamPlan stream_plan(int nw, int tokens, int n, int nk, int sm_count) {
+    const int units = (n + kStreamRows - 1) / kStreamRows;
+    StreamPlan p{};
+    p.stage = nw * 16384 + (tokens + 15) / 16 * 16 * 128;
+    for (p.splits = 8; p.splits >= 1; p.splits /= 2) {
+        p.sums = p.splits > 1 ? (nw * tokens * kStreamRows * 4 + 1023) / 1024 * 1024 : 0;
+        const int half = (kSmemHalf - 1024 - p.sums) / p.stage, whole = (kSmemMost - 1024 - p.sums) / p.stage;
+        const bool two = half >= (tokens <= 32 ? 2 : 3);
+        p.stages = two ? half : whole;
+        if (p.splits == 1) break;
+        if (p.stages >= 2 && nk >= 2 * p.splits && units * p.splits <= (two ? 2 : 1) * sm_count) break;
+    }
+    if (p.stages > kStreamMaxStages) p.stages = kStreamMaxStages;
+    return p;
 }
 
 // w: NW weight matrices [n, k], contiguous; x: [tokens, k].
@@ -274,27 +289,20 @@ int stream_launch(const void* w0, const void* w1, const void* x, int64_t x_ld, i
     if ((st = make_map_2d(&p.w[0], dtype, w0, n, k, k, block, kStreamRows)) != VY_OK) return st;
     if (NW == 2 && (st = make_map_2d(&p.w[1], dtype, w1, n, k, k, block, kStreamRows)) != VY_OK) return st;
     if ((st = make_map_2d(&p.x, dtype, x, tokens, k, x_ld, block, p.cols)) != VY_OK) return st;
-    const int splits = stream_splits(n, p.nk, dev->sm_count);
-    const int stage = NW * 16384 + p.cols * 128;
-    const int sums = splits > 1 ? NW * p.cols * kStreamRows * 4 : 0;
-    // about 100 KB of stages: two CTAs on an SM; more only where the sums to be joined ask for it
-    p.stages = 100 * 1024 / stage;
-    if (p.stages > kStreamMaxStages) p.stages = kStreamMaxStages;
-    if (p.stages < 2) p.stages = 2;
-    int bytes = p.stages * stage;
-    if (bytes < sums) bytes = sums;
-    bytes += 1024;
+    const StreamPlan plan = stream_plan(NW, tokens, n, p.nk, dev->sm_count);
+    if (plan.stages < 2) return fail(VY_ERR_UNSUPPORTED, "dense stream: %d tokens", tokens);
+    p.stages = plan.stages;
+    p.sums_at = plan.stages * plan.stage;
+    const int bytes = p.sums_at + plan.sums + 1024;
     auto kern = stream_kernel<EPI, ACT>;
-    constexpr int kMost = 2 * 128 * kStreamRows * 4 + 2 * 1024 + 32768;
     st = once_per_device(reinterpret_cast<const void*>(kern), [](int, void* f) {
-        const cudaError_t e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost);
+        const cudaError_t e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMost);
         return e == cudaSuccess ? VY_OK : fail(VY_ERR_CUDA, "dense stream shared memory: %s", cudaGetErrorString(e));
     }, reinterpret_cast<void*>(kern));
     if (st != VY_OK) return st;
-    if (bytes > kMost) return fail(VY_ERR_UNSUPPORTED, "dense stream: %d bytes of shared memory", bytes);
     const unsigned units = (n + kStreamRows - 1) / kStreamRows;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(units * splits);
+    cfg.gridDim = dim3(units * plan.splits);
     cfg.blockDim = dim3(kStreamThreads);
     cfg.dynamicSmemBytes = bytes;
     cfg.stream = s;
@@ -302,7 +310,7 @@ int stream_launch(const void* w0, const void* w1, const void* x, int64_t x_ld, i
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = splits;
+    attr[1].val.clusterDim.x = plan.splits;
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 2;

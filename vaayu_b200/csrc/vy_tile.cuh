@@ -88,8 +88,8 @@ __device__ __forceinline__ void tile_epilogue(const TileProblem& q, int row, int
 #pragma unroll
                 for (int j = 0; j < 16; ++j) {
                     const int cc = j < valid ? col + j : col;
-                    const float gf = __fmul_rn(__fmul_rn(float(int(g[j])), rs), __ldg(e.col_scale[0] + cc));
-                    const float uf = __fmul_rn(__fmul_rn(float(int(u[j])), rs), __ldg(e.col_scale[1] + cc));
+                    const float gf = __fmul_rn(__fmul_rn(float(int(g[j])), rs), e.col_scale[0][cc]);
+                    const float uf = __fmul_rn(__fmul_rn(float(int(u[j])), rs), e.col_scale[1][cc]);
                     h[j] = gate_act(gf, e.act) * uf;
                 }
                 store16_dyn(e.out, VY_F32, int64_t(row) * e.ldo + col, h, valid, true);
@@ -124,7 +124,7 @@ __device__ __forceinline__ void tile_epilogue(const TileProblem& q, int row, int
 #pragma unroll
                 for (int j = 0; j < 16; ++j) {
                     const int cc = j < valid ? col + j : col;
-                    v[j] = __fmul_rn(__fmul_rn(float(int(r[j])), rs), __ldg(e.col_scale[0] + cc));
+                    v[j] = __fmul_rn(__fmul_rn(float(int(r[j])), rs), e.col_scale[0][cc]);
                     if (e.bias) v[j] = __fadd_rn(v[j], load_as_float(e.bias, e.bias_dtype, cc));
                 }
                 store16_dyn(e.out, e.out_dtype, int64_t(row) * e.ldo + col, v, valid, e.vec != 0);
@@ -132,24 +132,54 @@ __device__ __forceinline__ void tile_epilogue(const TileProblem& q, int row, int
 #pragma unroll
                 for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(r[j]);
                 store16<ACT>(reinterpret_cast<uint16_t*>(e.out) + int64_t(row) * e.ldo + col, v, valid);
-            } else {
-                const float* s = e.saved + int64_t(col) * e.ld_saved + row;
-                float du[16], h[16];
-#pragma unroll
-                for (int j = 0; j < 16; ++j) {
-                    const int64_t o = (j < valid ? j : 0) * e.ld_saved;
-                    const float g = s[o], u = s[e.saved_u + o], dh = __uint_as_float(r[j]);
-                    const float2 a = gate_act_grad(g, e.act);
-                    v[j] = dh * u * a.y;
-                    du[j] = dh * a.x;
-                    h[j] = a.x * u;
-                }
-                const int64_t at = int64_t(row) * e.ldo + col;
-                store16<ACT>(e.dg + at, v, valid);
-                store16<ACT>(e.du + at, du, valid);
-                store16<ACT>(e.h + at, h, valid);
             }
         }
+    }
+}
+
+// dg, du and h of a tile from its dh and the saved g and u.  The tile's g and u are read a chunk of 16
+// columns ahead, the first one before the tile's sums are awaited: their latency is paid under the
+// MMAs and the previous chunk's arithmetic.
+struct GateChunk {
+    float g[16], u[16];
+};
+__device__ __forceinline__ void load_gate(GateChunk& k, const EpiParams& e, int row, int col, bool live, int n) {
+    const float* s = e.saved + int64_t(col) * e.ld_saved + row;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+        const bool in = live && col + j < n;
+        k.g[j] = in ? s[j * e.ld_saved] : 0.f;
+        k.u[j] = in ? s[e.saved_u + j * e.ld_saved] : 0.f;
+    }
+}
+template <int ACT>
+__device__ __forceinline__ void dgate_epilogue(const TileProblem& q, GateChunk& next, int row, int n_tile, uint32_t tmem,
+                                               int half) {
+    const EpiParams& e = q.epi;
+    const bool live = row < q.m;
+    const int c0 = half * (q.bn / 2), c1 = c0 + q.bn / 2;
+    for (int c = c0; c < c1; c += 16) {
+        const GateChunk k = next;
+        const int col = n_tile * q.bn + c;
+        if (c + 16 < c1) load_gate(next, e, row, col + 16, live, q.n);
+        uint32_t r[16];
+        tmem_ld16(tmem + c, r);
+        tmem_wait16(r);
+        const int valid = min(16, q.n - col);
+        if (!live || valid <= 0) continue;
+        float dg[16], du[16], h[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+            const float dh = __uint_as_float(r[j]);
+            const float2 a = gate_act_grad(k.g[j], e.act);
+            dg[j] = dh * k.u[j] * a.y;
+            du[j] = dh * a.x;
+            h[j] = a.x * k.u[j];
+        }
+        const int64_t at = int64_t(row) * e.ldo + col;
+        store16<ACT>(e.dg + at, dg, valid);
+        store16<ACT>(e.du + at, du, valid);
+        store16<ACT>(e.h + at, h, valid);
     }
 }
 
@@ -268,11 +298,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTileThreads, 1)
         for (int tile = cluster; tile < p.n_tiles; tile += n_clusters, ++n) {
             const TileAt t = tile_at(p, tile);
             const uint32_t buf = n & 1;
+            const TileProblem& q = p.prob[t.prob];
+            const int row = t.m * 256 + int(rank) * 128 + quarter * 32 + lane;
+            const uint32_t acc = tmem + buf * 256 + (uint32_t(quarter * 32) << 16);
+            GateChunk first;
+            if constexpr (EPI == EPI_DGATE)
+                load_gate(first, q.epi, row, t.n * q.bn + half * (q.bn / 2), row < q.m, q.n);
             const bool ready = mbar_wait(&S.acc_full[buf], (n >> 1) & 1, abort_flag, p.flags);
             if (!__all_sync(0xffffffffu, ready)) break;
             tc_fence_after();
-            tile_epilogue<EPI, ACT>(p.prob[t.prob], t.m * 256 + int(rank) * 128 + quarter * 32 + lane, t.n,
-                                    tmem + buf * 256 + (uint32_t(quarter * 32) << 16), half);
+            if constexpr (EPI == EPI_DGATE)
+                dgate_epilogue<ACT>(q, first, row, t.n, acc, half);
+            else
+                tile_epilogue<EPI, ACT>(q, row, t.n, acc, half);
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive_remote(map_to_rank(smem_u32(&S.acc_empty[buf]), 0));

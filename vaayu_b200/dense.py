@@ -46,7 +46,7 @@ def _device(what: str, first: torch.Tensor, *others) -> int:
         if t is not None and t.get_device() != index:
             index = -1
     if index < 0:
-        _lib.require_cuda(first, *others, what=what)
+        _lib.require_cuda(first, *others, what=what)      # raises: CPU tensors, or two devices
     return index
 
 
@@ -68,38 +68,38 @@ def _activation(act: str, what: str) -> int:
     return code
 
 
-def _rows(x: torch.Tensor, unit: int) -> torch.Tensor:
-    """x as [tokens, width] rows that start on 16-byte boundaries (`unit` elements): a view where the
-    strides allow it, else a copy."""
+def _rows(x: torch.Tensor, unit: int) -> tuple:
+    """(x as [tokens, width] with rows that start on 16-byte boundaries (`unit` elements), its row
+    stride): a view where the strides allow it, else a copy."""
     if x.dim() != 2:
         x = x.reshape(-1, x.shape[-1])
-    if x.data_ptr() % 16 == 0:
-        if x.is_contiguous():
-            if x.shape[1] % unit == 0 or x.shape[0] <= 1:
-                return x
-        else:
-            row, col = x.stride()
-            if col == 1 and (x.shape[0] <= 1 or (row % unit == 0 and row >= x.shape[1])):
-                return x
-    return x.clone(memory_format=torch.contiguous_format)
-
-
-def _unit_rows(x: torch.Tensor) -> torch.Tensor:
-    """x as [tokens, width] with a unit column stride."""
-    if x.dim() != 2:
-        x = x.reshape(-1, x.shape[-1])
-    return x if x.stride(1) == 1 else x.contiguous()
-
-
-def _stride(x: torch.Tensor) -> int:
     tokens, width = x.shape
-    return x.stride(0) if tokens > 1 else width
+    if x.data_ptr() & 15 == 0:
+        row, col = x.stride()
+        if tokens <= 1:
+            if col == 1 or width == 1:
+                return x, -(-width // unit) * unit
+        elif col == 1 and row % unit == 0 and row >= width:
+            return x, row
+    return x.clone(memory_format=torch.contiguous_format), width
+
+
+def _unit_rows(x: torch.Tensor) -> tuple:
+    """(x as [tokens, width] with a unit column stride, its row stride)."""
+    if x.dim() != 2:
+        x = x.reshape(-1, x.shape[-1])
+    row, col = x.stride()
+    if col != 1:
+        x = x.contiguous()
+        row = x.shape[1]
+    return x, (row if x.shape[0] > 1 else x.shape[1])
 
 
 def _aligned(w: torch.Tensor) -> torch.Tensor:
+    """w itself when it is contiguous and starts on a 16-byte boundary, else a copy that does."""
     if not w.is_contiguous():
-        w = w.contiguous()
-    return w.clone() if w.data_ptr() % 16 else w
+        return w.contiguous()
+    return w.clone() if w.data_ptr() & 15 else w
 
 
 def _check_ffn(x, w_gate, w_up, w_down, what: str) -> tuple:
@@ -114,14 +114,16 @@ def _check_ffn(x, w_gate, w_up, w_down, what: str) -> tuple:
 
 
 def _output(out, like, shape, dtype, what: str) -> tuple:
-    """(`out` checked or a new tensor on like's device, it as [tokens, width])."""
+    """(`out` checked or a new tensor on like's device, it as [tokens, width], its row stride)."""
     if out is None:
         out = torch.empty(shape, dtype=dtype, device=like.device)
     elif out.shape != shape or out.dtype != dtype:
         raise ValueError(f"{what}: out {tuple(out.shape)} {out.dtype}, expected {tuple(shape)} {dtype}")
-    elif not out.is_contiguous() and (out.dim() != 2 or out.stride(1) != 1 or out.stride(0) < out.shape[1]):
-        raise ValueError(f"{what}: out must be contiguous, or a 2-D view with unit column stride")
-    return out, (out if out.dim() == 2 else out.view(-1, shape[-1]))
+    elif not out.is_contiguous():
+        if out.dim() != 2 or out.stride(1) != 1 or out.stride(0) < out.shape[1]:
+            raise ValueError(f"{what}: out must be contiguous, or a 2-D view with unit column stride")
+        return out, out, out.stride(0)
+    return out, (out if out.dim() == 2 else out.view(-1, shape[-1])), shape[-1]
 
 
 def _workspace(size: int, like: torch.Tensor) -> "torch.Tensor | None":
@@ -136,8 +138,8 @@ def _ptr(t: "torch.Tensor | None") -> int:
     return 0 if t is None else t.data_ptr()
 
 
-def _raise_on(flags: "torch.Tensor | None", what: str) -> None:
-    if flags is not None and (v := int(flags.item())):
+def _raise_on(flags: torch.Tensor, what: str) -> None:
+    if v := int(flags.item()):
         raise RuntimeError(f"{what}: device error flags {v:#x} (a device-side wait ran out); the output is not valid")
 
 
@@ -157,31 +159,33 @@ def _ffn_workspace(tokens: int, hidden: int, inter: int, backward: int) -> int:
     return size
 
 
-def _ffn_forward(rows, wg, wu, wd, act: int, flat, index: int, save: bool, check: bool):
-    """The forward call on 2-D rows into `flat`; returns what the backward pass needs when `save`."""
-    tokens, hidden = rows.shape
-    inter = wg.shape[0]
+def _ffn_forward(x, w_gate, w_up, w_down, hidden: int, inter: int, act: int, flat, out_stride: int, index: int,
+                 save: bool, check: bool):
+    """The forward call into `flat`; returns what the backward pass needs when `save`."""
+    rows, x_stride = _rows(x, 8)
+    wg, wu, wd = _aligned(w_gate), _aligned(w_up), _aligned(w_down)
+    tokens = rows.shape[0]
     size = _ffn_workspace(tokens, hidden, inter, 0)
     ws = _workspace(size, rows)
     saved = None
     if save:
         saved = torch.empty(_lib.lib().vy_gated_ffn_saved_floats(tokens, inter), dtype=_F32, device=rows.device)
     flags = _flags(rows, check)
-    call = _FFN.pack(_CODE[rows.dtype], act, tokens, hidden, inter, rows.data_ptr(), _stride(rows), wg.data_ptr(),
-                     wu.data_ptr(), wd.data_ptr(), flat.data_ptr(), _stride(flat), _ptr(saved), _ptr(ws), size,
+    call = _FFN.pack(_CODE[rows.dtype], act, tokens, hidden, inter, rows.data_ptr(), x_stride, wg.data_ptr(),
+                     wu.data_ptr(), wd.data_ptr(), flat.data_ptr(), out_stride, _ptr(saved), _ptr(ws), size,
                      _ptr(flags), 0, 0, 0, 0, 0, 0, 0)
     _enqueue(_lib.lib().vy_gated_ffn_forward, call, index, "gated_ffn")
-    _raise_on(flags, "gated_ffn")
+    if check:
+        _raise_on(flags, "gated_ffn")
     return saved
 
 
 class _GatedFfn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w_gate, w_up, w_down, act, check):
-        rows, wg, wu, wd = _rows(x, 8), _aligned(w_gate), _aligned(w_up), _aligned(w_down)
+        inter, hidden = w_gate.shape
         out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        flat = out if out.dim() == 2 else out.view(-1, x.shape[-1])
-        saved = _ffn_forward(rows, wg, wu, wd, act, flat, x.get_device(), True, check)
+        saved = _ffn_forward(x, w_gate, w_up, w_down, hidden, inter, act, out, hidden, x.get_device(), True, check)
         ctx.save_for_backward(x, w_gate, w_up, w_down, saved)
         ctx.act, ctx.check = act, check
         return out
@@ -190,24 +194,21 @@ class _GatedFfn(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, d_out):
         x, w_gate, w_up, w_down, saved = ctx.saved_tensors
-        rows, dy = _rows(x, 8), _rows(d_out, 8)
+        (rows, x_stride), (dy, dy_stride) = _rows(x, 8), _rows(d_out, 8)
         wg, wu, wd = _aligned(w_gate), _aligned(w_up), _aligned(w_down)
-        tokens, hidden = rows.shape
-        inter = wg.shape[0]
+        tokens, (inter, hidden) = rows.shape[0], wg.shape
         need = ctx.needs_input_grad
-        like = torch.empty_like
-        keep = torch.contiguous_format
-        d_x = like(x, memory_format=keep) if need[0] else None
-        d_wg, d_wu, d_wd = (like(w, memory_format=keep) if n else None for w, n in zip((wg, wu, wd), need[1:4]))
+        grads = [torch.empty(t.shape, dtype=t.dtype, device=t.device) if n else None
+                 for t, n in zip((x, w_gate, w_up, w_down), need)]
         size = _ffn_workspace(tokens, hidden, inter, 1)
         ws, flags = _workspace(size, rows), _flags(rows, ctx.check)
-        call = _FFN.pack(_CODE[rows.dtype], ctx.act, tokens, hidden, inter, rows.data_ptr(), _stride(rows),
+        call = _FFN.pack(_CODE[rows.dtype], ctx.act, tokens, hidden, inter, rows.data_ptr(), x_stride,
                          wg.data_ptr(), wu.data_ptr(), wd.data_ptr(), 0, 0, saved.data_ptr(), _ptr(ws), size,
-                         _ptr(flags), dy.data_ptr(), _stride(dy), _ptr(d_x), hidden, _ptr(d_wg), _ptr(d_wu),
-                         _ptr(d_wd))
+                         _ptr(flags), dy.data_ptr(), dy_stride, _ptr(grads[0]), hidden, *map(_ptr, grads[1:]))
         _enqueue(_lib.lib().vy_gated_ffn_backward, call, x.get_device(), "gated_ffn backward")
-        _raise_on(flags, "gated_ffn backward")
-        return d_x, d_wg, d_wu, d_wd, None, None
+        if ctx.check:
+            _raise_on(flags, "gated_ffn backward")
+        return (*grads, None, None)
 
 
 def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor,
@@ -235,10 +236,10 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
         if out is not None:
             raise RuntimeError(f"{what}: out= with gradients")
         return _GatedFfn.apply(x, w_gate, w_up, w_down, code, check)
-    y, flat = _output(out, x, x.shape, dtype, what)
-    if flat.data_ptr() % 16 or (flat.shape[0] > 1 and flat.stride(0) % 8):
+    y, flat, stride = _output(out, x, x.shape, dtype, what)
+    if out is not None and (flat.data_ptr() & 15 or stride % 8):
         raise ValueError(f"{what}: out rows must start on 16-byte boundaries")
-    _ffn_forward(_rows(x, 8), _aligned(w_gate), _aligned(w_up), _aligned(w_down), code, flat, index, False, check)
+    _ffn_forward(x, w_gate, w_up, w_down, hidden, inter, code, flat, stride, index, False, check)
     return y
 
 
@@ -259,14 +260,17 @@ def quantize_int8(x: torch.Tensor) -> tuple:
     if not shape or shape[-1] == 0:
         raise ValueError(f"{what}: x {tuple(shape)} has no values in a row")
     index = _device(what, x)
-    rows = _unit_rows(x)
-    codes = torch.empty(shape, dtype=_INT8, device=x.device)
-    scale = torch.empty((*shape[:-1], 1), dtype=_F32, device=x.device)
+    rows, stride = _unit_rows(x)
     tokens, width = rows.shape
-    fn = _lib.lib().vy_int8_quantize
-    _enqueue(lambda call, stream: fn(*call, stream),
-             (rows.data_ptr(), code, rows.stride(0) if tokens > 1 else width, tokens, width, codes.data_ptr(),
-              scale.data_ptr()), index, what)
+    dev = x.device
+    codes = torch.empty(shape, dtype=_INT8, device=dev)
+    scale = torch.empty((tokens, 1) if len(shape) == 2 else (*shape[:-1], 1), dtype=_F32, device=dev)
+
+    def call(_none, stream):
+        return _lib.lib().vy_int8_quantize(rows.data_ptr(), code, stride, tokens, width, codes.data_ptr(),
+                                           scale.data_ptr(), stream)
+
+    _enqueue(call, None, index, what)
     return codes, scale
 
 
@@ -305,15 +309,16 @@ def int8_linear(codes: torch.Tensor, scale: torch.Tensor, weight: torch.Tensor, 
             raise ValueError(f"{what}: bias {tuple(bias.shape)} for {n} output channels")
         bias, bias_code = bias.contiguous(), _CODE[bias.dtype]
     index = _device(what, codes, scale, weight, weight_scale, bias, out)
-    rows, w = _rows(codes, 16), _aligned(weight)
+    (rows, stride), w = _rows(codes, 16), _aligned(weight)
     tokens = rows.shape[0]
     sx, sw = _scales(scale, tokens, what), _scales(weight_scale, n, what)
-    y, flat = _output(out, codes, (*shape[:-1], n), dtype, what)
+    y, flat, out_stride = _output(out, codes, (tokens, n) if len(shape) == 2 else (*shape[:-1], n), dtype, what)
     flags = _flags(codes, check)
-    call = _LINEAR.pack(tokens, k, n, rows.data_ptr(), _stride(rows), sx.data_ptr(), w.data_ptr(), sw.data_ptr(),
-                        _ptr(bias), bias_code, out_code, flat.data_ptr(), _stride(flat), 0, 0, _ptr(flags))
+    call = _LINEAR.pack(tokens, k, n, rows.data_ptr(), stride, sx.data_ptr(), w.data_ptr(), sw.data_ptr(),
+                        _ptr(bias), bias_code, out_code, flat.data_ptr(), out_stride, 0, 0, _ptr(flags))
     _enqueue(_lib.lib().vy_int8_linear, call, index, what)
-    _raise_on(flags, what)
+    if check:
+        _raise_on(flags, what)
     return y
 
 
@@ -350,15 +355,16 @@ def int8_gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, gate_scale: torch.Tens
     if hidden % 16 or inter % 16 or not 0 < hidden < _MAX_K or not 0 < inter < _MAX_K:
         raise NotImplementedError(f"{what}: hidden {hidden} and inter {inter} must be multiples of 16 below {_MAX_K}")
     index = _device(what, x, w_gate, gate_scale, w_up, up_scale, w_down, down_scale, out)
-    rows, wg, wu, wd = _unit_rows(x), _aligned(w_gate), _aligned(w_up), _aligned(w_down)
+    (rows, stride), wg, wu, wd = _unit_rows(x), _aligned(w_gate), _aligned(w_up), _aligned(w_down)
     sg, su, sd = _scales(gate_scale, inter, what), _scales(up_scale, inter, what), _scales(down_scale, hidden, what)
-    y, flat = _output(out, x, x.shape, dtype, what)
+    y, flat, out_stride = _output(out, x, x.shape, dtype, what)
     tokens = rows.shape[0]
     size = _int8_ffn_workspace((tokens, hidden, inter))
     ws, flags = _workspace(size, rows), _flags(rows, check)
-    call = _INT8_FFN.pack(_CODE[dtype], code, tokens, hidden, inter, rows.data_ptr(), _stride(rows), wg.data_ptr(),
+    call = _INT8_FFN.pack(_CODE[dtype], code, tokens, hidden, inter, rows.data_ptr(), stride, wg.data_ptr(),
                           wu.data_ptr(), wd.data_ptr(), sg.data_ptr(), su.data_ptr(), sd.data_ptr(), flat.data_ptr(),
-                          _stride(flat), _ptr(ws), size, _ptr(flags))
+                          out_stride, _ptr(ws), size, _ptr(flags))
     _enqueue(_lib.lib().vy_int8_gated_ffn, call, index, what)
-    _raise_on(flags, what)
+    if check:
+        _raise_on(flags, what)
     return y
