@@ -68,64 +68,54 @@ void epi_store(TileProblem* q, void* out, int64_t ldo) {
         if (vy_st != VY_OK) return vy_st;    \
     } while (0)
 
+int k_blocks(int64_t k) { return static_cast<int>((k + 63) / 64); }
+
 template <int ACT>
 int forward(const vy_ffn_call* c, const DeviceInfo* dev, cudaStream_t s) {
     const int64_t T = c->n_tokens, H = c->hidden, I = c->inter;
-    const int clusters = dev->sm_count / 2;
     uint16_t* h = reinterpret_cast<uint16_t*>((reinterpret_cast<uintptr_t>(c->workspace) + 255) & ~uintptr_t(255));
+    EpiParams e{};
+    e.out = h;
+    e.ldo = I;
+    e.act = c->activation;
+    e.saved = c->saved;
+    e.ld_saved = saved_ld(T);
+    e.saved_u = saved_ld(T) * I;
+    EpiParams d{};
+    d.out = c->out;
+    d.ldo = c->out_row_stride;
     if (T <= kStreamMaxTokens) {
-        EpiParams e{};
-        e.out = h;
-        e.ldo = I;
-        e.act = c->activation;
-        e.saved = c->saved;
-        e.ld_saved = saved_ld(T);
-        e.saved_u = saved_ld(T) * I;
         VY_TRY((stream_launch<EPI_GATE, ACT>(c->w_gate, c->w_up, c->x, c->x_row_stride, static_cast<int>(T), c->inter,
                                              c->hidden, false, e, c->flags, dev, s)));
-        EpiParams d{};
-        d.out = c->out;
-        d.ldo = c->out_row_stride;
         return stream_launch<EPI_STORE, ACT>(c->w_down, nullptr, h, I, static_cast<int>(T), c->hidden, c->inter, true, d,
                                              c->flags, dev, s);
     }
+    const int pairs = dev->sm_count / 2;
     {
         TileParams p{};
-        TileProblem& q = p.prob[0];
-        q.m = static_cast<int>(T);
-        q.n = c->inter;
-        q.bn = tile_columns(T, 2 * I, clusters);
-        q.nk[0] = static_cast<int>((H + 63) / 64);
+        TileProblem& q = tile_add(&p, T, I, k_blocks(H));
+        tile_layout(&p, true, pairs);
         VY_TRY(tile_operand(&q.a[0], ACT, c->x, T, H, c->x_row_stride, false, 128));
         VY_TRY(tile_operand(&q.b[0], ACT, c->w_gate, I, H, H, false, q.bn / 2));
         VY_TRY(tile_operand(&q.b[1], ACT, c->w_up, I, H, H, false, q.bn / 2));
-        epi_store(&q, h, I);
-        q.epi.act = c->activation;
-        q.epi.saved = c->saved;
-        q.epi.ld_saved = saved_ld(T);
-        q.epi.saved_u = saved_ld(T) * I;
+        q.epi = e;
         p.flags = c->flags;
-        tile_place(&p, 0, true);
-        VY_TRY((tile_launch<EPI_GATE, ACT>(p, dev, s)));
+        VY_TRY((tile_launch<EPI_GATE, ACT>(p, pairs, s)));
     }
     TileParams p{};
-    TileProblem& q = p.prob[0];
-    q.m = static_cast<int>(T);
-    q.n = c->hidden;
-    q.bn = tile_columns(T, H, clusters);
-    q.nk[0] = static_cast<int>((I + 63) / 64);
+    TileProblem& q = tile_add(&p, T, H, k_blocks(I));
+    tile_layout(&p, false, pairs);
     VY_TRY(tile_operand(&q.a[0], ACT, h, T, I, I, false, 128));
     VY_TRY(tile_operand(&q.b[0], ACT, c->w_down, H, I, I, false, q.bn / 2));
-    epi_store(&q, c->out, c->out_row_stride);
+    q.epi = d;
     p.flags = c->flags;
-    tile_place(&p, 0, false);
-    return tile_launch<EPI_STORE, ACT>(p, dev, s);
+    return tile_launch<EPI_STORE, ACT>(p, pairs, s);
 }
 
 template <int ACT>
 int backward(const vy_ffn_call* c, const DeviceInfo* dev, cudaStream_t s) {
     const int64_t T = c->n_tokens, H = c->hidden, I = c->inter;
-    const int clusters = dev->sm_count / 2;
+    const int pairs = dev->sm_count / 2;
     char* base = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(c->workspace) + 255) & ~uintptr_t(255));
     const size_t each = align256(size_t(h_elems(c)) * 2);
     uint16_t* dg = reinterpret_cast<uint16_t*>(base);
@@ -133,11 +123,8 @@ int backward(const vy_ffn_call* c, const DeviceInfo* dev, cudaStream_t s) {
     uint16_t* h = reinterpret_cast<uint16_t*>(base + 2 * each);
     {
         TileParams p{};
-        TileProblem& q = p.prob[0];
-        q.m = static_cast<int>(T);
-        q.n = c->inter;
-        q.bn = tile_columns(T, I, clusters);
-        q.nk[0] = static_cast<int>((H + 63) / 64);
+        TileProblem& q = tile_add(&p, T, I, k_blocks(H));
+        tile_layout(&p, false, pairs);
         q.b_mn = 1;
         VY_TRY(tile_operand(&q.a[0], ACT, c->d_out, T, H, c->d_out_row_stride, false, 128));
         VY_TRY(tile_operand(&q.b[0], ACT, c->w_down, I, H, I, true, 0));
@@ -150,25 +137,18 @@ int backward(const vy_ffn_call* c, const DeviceInfo* dev, cudaStream_t s) {
         q.epi.du = du;
         q.epi.h = h;
         p.flags = c->flags;
-        tile_place(&p, 0, false);
-        VY_TRY((tile_launch<EPI_DGATE, ACT>(p, dev, s)));
+        VY_TRY((tile_launch<EPI_DGATE, ACT>(p, pairs, s)));
     }
     TileParams p{};
     p.flags = c->flags;
-    int n = 0;
     if (c->d_x) {      // two K segments: dg Wg + du Wu
-        TileProblem& q = p.prob[n];
-        q.m = static_cast<int>(T);
-        q.n = c->hidden;
-        q.bn = tile_columns(T, H, clusters);
-        q.nk[0] = q.nk[1] = static_cast<int>((I + 63) / 64);
+        TileProblem& q = tile_add(&p, T, H, k_blocks(I), k_blocks(I));
         q.b_mn = 1;
         VY_TRY(tile_operand(&q.a[0], ACT, dg, T, I, I, false, 128));
         VY_TRY(tile_operand(&q.a[1], ACT, du, T, I, I, false, 128));
         VY_TRY(tile_operand(&q.b[0], ACT, c->w_gate, H, I, H, true, 0));
         VY_TRY(tile_operand(&q.b[1], ACT, c->w_up, H, I, H, true, 0));
         epi_store(&q, c->d_x, c->d_x_row_stride);
-        tile_place(&p, n++, false);
     }
     struct Grad {
         void* out;
@@ -180,19 +160,15 @@ int backward(const vy_ffn_call* c, const DeviceInfo* dev, cudaStream_t s) {
                            {c->d_w_down, c->d_out, h, H, I, c->d_out_row_stride, I}};
     for (const Grad& g : grads) {
         if (!g.out) continue;
-        TileProblem& q = p.prob[n];
-        q.m = static_cast<int>(g.m);
-        q.n = static_cast<int>(g.n);
-        q.bn = tile_columns(g.m, g.n, clusters);
-        q.nk[0] = static_cast<int>((T + 63) / 64);
+        TileProblem& q = tile_add(&p, g.m, g.n, k_blocks(T));
         q.a_mn = q.b_mn = 1;
         VY_TRY(tile_operand(&q.a[0], ACT, g.a, g.m, T, g.lda, true, 0));
         VY_TRY(tile_operand(&q.b[0], ACT, g.b, g.n, T, g.ldb, true, 0));
         epi_store(&q, g.out, g.n);
-        tile_place(&p, n++, false);
     }
-    if (n == 0) return VY_OK;
-    return tile_launch<EPI_STORE, ACT>(p, dev, s);
+    if (p.n_problems == 0) return VY_OK;
+    tile_layout(&p, false, pairs);
+    return tile_launch<EPI_STORE, ACT>(p, pairs, s);
 }
 
 }  // namespace

@@ -263,19 +263,16 @@ int launch_product(const Product& a, bool first, const DeviceInfo* dev, cudaStre
     if (a.tokens <= kStreamMaxTokens)
         return stream_launch<EPI, VY_BF16>(a.w[0], a.w[1], a.codes, a.codes_ld, static_cast<int>(a.tokens), a.n, a.k,
                                            !first, e, a.flags, dev, s);
+    const int pairs = dev->sm_count / 2;
     TileParams p{};
-    TileProblem& q = p.prob[0];
-    q.m = static_cast<int>(a.tokens);
-    q.n = a.n;
-    q.bn = tile_columns(a.tokens, GATE ? 2 * int64_t(a.n) : a.n, dev->sm_count / 2);
-    q.nk[0] = (a.k + 127) / 128;
+    TileProblem& q = tile_add(&p, a.tokens, a.n, (a.k + 127) / 128);
+    tile_layout(&p, GATE, pairs);
     VY_TRY(tile_operand(&q.a[0], VY_E4M3, a.codes, a.tokens, a.k, a.codes_ld, false, 128));
     VY_TRY(tile_operand(&q.b[0], VY_E4M3, a.w[0], a.n, a.k, a.k, false, q.bn / 2));
     if (GATE) VY_TRY(tile_operand(&q.b[1], VY_E4M3, a.w[1], a.n, a.k, a.k, false, q.bn / 2));
     q.epi = e;
     p.flags = a.flags;
-    tile_place(&p, 0, GATE);
-    return tile_launch<EPI, VY_BF16>(p, dev, s);
+    return tile_launch<EPI, VY_BF16>(p, pairs, s);
 }
 
 bool float_dtype(int d) { return d == VY_BF16 || d == VY_F16 || d == VY_F32; }

@@ -37,13 +37,34 @@ struct StreamParams {
 
 struct StreamBars {
     uint64_t full[kStreamMaxStages], empty[kStreamMaxStages], done;
+    float token_scale[kStreamMaxTokens];
     uint32_t tmem_base;
     int abort_flag;
 };
 
 // One output value (weight row `row`, token `t`) from its sums.
+// What an output needs besides its sums, fetched while they are still being formed.
+struct ColumnScale {
+    float a, b;      // int8: scale of the weight row, and of its up row or its bias
+};
+template <int EPI>
+__device__ __forceinline__ ColumnScale column_scale(const StreamParams& p, int row) {
+    ColumnScale c{0.f, 0.f};
+    if constexpr (epi_is_i8(EPI)) {
+        const EpiParams& e = p.epi;
+        if (row < p.n) {
+            c.a = e.col_scale[0][row];
+            if constexpr (EPI == EPI_I8GATE)
+                c.b = e.col_scale[1][row];
+            else if (e.bias)
+                c.b = load_as_float(e.bias, e.bias_dtype, row);
+        }
+    }
+    return c;
+}
 template <int EPI, int ACT>
-__device__ __forceinline__ void stream_put(const StreamParams& p, int row, int t, uint32_t s0, uint32_t s1) {
+__device__ __forceinline__ void stream_put(const StreamParams& p, int row, int t, uint32_t s0, uint32_t s1,
+                                           const ColumnScale& cs, const float* token_scale) {
     const EpiParams& e = p.epi;
     const int64_t at = int64_t(t) * e.ldo + row;
     if constexpr (EPI == EPI_GATE) {
@@ -57,13 +78,12 @@ __device__ __forceinline__ void stream_put(const StreamParams& p, int row, int t
     } else if constexpr (EPI == EPI_STORE) {
         reinterpret_cast<uint16_t*>(e.out)[at] = static_cast<uint16_t>(act_bits<ACT>(__uint_as_float(s0)));
     } else if constexpr (EPI == EPI_I8GATE) {
-        const float rs = e.row_scale[t];
-        const float g = __fmul_rn(__fmul_rn(float(int(s0)), rs), e.col_scale[0][row]);
-        const float u = __fmul_rn(__fmul_rn(float(int(s1)), rs), e.col_scale[1][row]);
+        const float g = __fmul_rn(__fmul_rn(float(int(s0)), token_scale[t]), cs.a);
+        const float u = __fmul_rn(__fmul_rn(float(int(s1)), token_scale[t]), cs.b);
         reinterpret_cast<float*>(e.out)[at] = gate_act(g, e.act) * u;
     } else {
-        float v = __fmul_rn(__fmul_rn(float(int(s0)), e.row_scale[t]), e.col_scale[0][row]);
-        if (e.bias) v = __fadd_rn(v, load_as_float(e.bias, e.bias_dtype, row));
+        float v = __fmul_rn(__fmul_rn(float(int(s0)), token_scale[t]), cs.a);
+        if (e.bias) v = __fadd_rn(v, cs.b);
         store_as(e.out, e.out_dtype, at, v);
     }
 }
@@ -180,6 +200,14 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(const __grid_con
     // received sums [share][matrix][token][row of my slice], rows fastest
     const int rows = kStreamRows / splits;      // 1, 2, 4 or 8 shares
     uint32_t* sums = reinterpret_cast<uint32_t*>(ring + p.sums_at);
+    // the weight row of this thread: its lane's when it reads all sums itself, else of my slice
+    // (kStreamThreads is a multiple of a slice's rows, so every output it adds has the same one)
+    const int my_row = row0 + (splits == 1 ? tid & (kStreamRows - 1) : int(rank) * rows + tid % rows);
+    const ColumnScale cs = column_scale<EPI>(p, my_row);
+    if constexpr (epi_is_i8(EPI)) {
+        for (int t = tid; t < p.tokens; t += kStreamThreads) S.token_scale[t] = p.epi.row_scale[t];
+        __syncthreads();
+    }
     if (splits > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
     if (warp < 4) {
         const bool ready = __all_sync(0xffffffffu, mbar_wait(&S.done, 0, abort_flag, p.flags));
@@ -199,7 +227,8 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(const __grid_con
                     if (row0 + row < p.n) {
 #pragma unroll
                         for (int j = 0; j < 16; ++j)
-                            if (c + j < p.tokens) stream_put<EPI, ACT>(p, row0 + row, c + j, v[0][j], v[NW - 1][j]);
+                            if (c + j < p.tokens) stream_put<EPI, ACT>(p, row0 + row, c + j, v[0][j], v[NW - 1][j], cs,
+                                                     S.token_scale);
                     }
                 } else {
 #pragma unroll
@@ -217,8 +246,8 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(const __grid_con
         cluster_sync();
         const int share = NW * p.tokens * rows;
         for (int q = tid; q < rows * p.tokens; q += kStreamThreads) {
-            const int row = int(rank) * rows + q % rows, t = q / rows;
-            if (row0 + row >= p.n) continue;
+            const int t = q / rows;
+            if (my_row >= p.n) continue;
             uint32_t sum[NW];
 #pragma unroll
             for (int m = 0; m < NW; ++m) {
@@ -230,7 +259,7 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(const __grid_con
                 }
                 sum[m] = acc;
             }
-            stream_put<EPI, ACT>(p, row0 + row, t, sum[0], sum[NW - 1]);
+            stream_put<EPI, ACT>(p, my_row, t, sum[0], sum[NW - 1], cs, S.token_scale);
         }
     } else {
         __syncthreads();

@@ -10,6 +10,12 @@
 // come in two segments from two tensor pairs (dx = dg Wg + du Wu).  One launch takes up to four
 // GEMMs, whose tiles fill the machine together.
 //
+// Few tiles.  Pairs are persistent, one for two SMs, and take tiles in turn.  A launch with at most half
+// as many tiles as pairs instead gives each tile a cluster of 2 or 4 pairs, which split its K: every
+// pair sends each other pair the sums of the columns that one owns, into shared memory, and adds its
+// own columns over all shares in K order.  (Joining through global memory, the last of the pairs adding
+// all shares, measured 59 us where this takes 21 and no split 27: 1003 x 2048 x 768 forward.)
+//
 // Roles of a CTA (12 warps): warp 0 loads, warp 1 of the pair's first CTA issues the MMAs, warp 2
 // owns TMEM, warps 4-11 run the epilogue.  Every wait is bounded: on a timeout the CTA records the
 // error, leaves its loop, and the pair still meets at its final barrier.
@@ -38,6 +44,7 @@ struct TileProblem {
 struct TileParams {
     TileProblem prob[kTileProblems];
     int n_problems, n_tiles;
+    int splits;              // pairs of a cluster, which share a tile's K: 1, 2 or 4
     int32_t* flags;
 };
 
@@ -46,6 +53,7 @@ struct __align__(1024) TileSmem {
     unsigned char b[kTileStages][kHalfBytes];
     uint64_t full[kTileStages], empty[kTileStages];
     uint64_t acc_full[2], acc_empty[2];
+    float cols[8][2][128];       // int8: an epilogue warp's column scales (gate, up) or scale and bias
     uint32_t tmem_base;
     int abort_flag;
 };
@@ -66,20 +74,85 @@ __device__ __forceinline__ TileAt tile_at(const TileParams& p, int tile) {
     return t;
 }
 
+// Sums of 16 columns of a tile: from TMEM, or (splits > 1) all shares of my columns, received in
+// shared memory as [share][4 columns][row][4], added in K order.
+struct TileSums {
+    uint32_t tmem;
+    const float4* recv;      // at my row
+    int splits, first, own;  // my columns [first, first + own) of each matrix
+    int mats, width;         // matrices of a tile (2: gate and up) and columns of each
+    template <bool I8>
+    __device__ __forceinline__ void get(int mat, int c, uint32_t (&r)[16]) const {
+        if (splits == 1) {
+            tmem_ld16(tmem + mat * width + c, r);
+            tmem_wait16(r);
+            return;
+        }
+        const float4* s = recv + (mat * own + c - first) / 4 * 128;
+        for (int i = 0; i < splits; ++i, s += mats * own / 4 * 128) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const float4 f = s[q * 128];
+                const float v[4] = {f.x, f.y, f.z, f.w};
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    uint32_t& d = r[4 * q + j];
+                    const uint32_t u = __float_as_uint(v[j]);
+                    d = i == 0 ? u : I8 ? d + u : __float_as_uint(__fadd_rn(__uint_as_float(d), __uint_as_float(u)));
+                }
+            }
+        }
+    }
+    // Sends my share of the tile (half of its columns a warp) to the pairs that own the columns.
+    __device__ __forceinline__ void send(uint32_t recv_base, uint32_t rank, int share, int half) const {
+        const int cols = mats * width;
+        for (int c = half * (cols / 2); c < (half + 1) * (cols / 2); c += 16) {
+            uint32_t r[16];
+            tmem_ld16(tmem + c, r);
+            tmem_wait16(r);
+            const int mat = c / width, in = c % width, owner = in / own;
+            const int local = (share * mats + mat) * own + in % own;
+            const uint32_t to = map_to_rank(recv_base, owner * 2 + rank) + local / 4 * 2048;
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                asm volatile("st.shared::cluster.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(to + q * 2048), "r"(r[4 * q]),
+                             "r"(r[4 * q + 1]), "r"(r[4 * q + 2]), "r"(r[4 * q + 3])
+                             : "memory");
+        }
+    }
+};
+
+// The scales (and bias) of a warp's columns [c0, c1) of a tile, fetched while the sums are still being
+// formed; a column at a time beside its sums costs a memory latency per 16 columns (1.1 us each).
+template <int EPI>
+__device__ __forceinline__ void load_cols(float (&cols)[2][128], const TileProblem& q, int n_tile, int c0, int c1) {
+    if constexpr (epi_is_i8(EPI)) {
+        const EpiParams& e = q.epi;
+        const int width = epi_is_gate(EPI) ? q.bn / 2 : q.bn, first = n_tile * width + c0;
+        __syncwarp();
+        for (int i = threadIdx.x & 31; i < c1 - c0; i += 32) {
+            const int c = min(first + i, q.n - 1);
+            cols[0][i] = e.col_scale[0][c];
+            if constexpr (EPI == EPI_I8GATE)
+                cols[1][i] = e.col_scale[1][c];
+            else if (e.bias)
+                cols[1][i] = load_as_float(e.bias, e.bias_dtype, c);
+        }
+        __syncwarp();
+    }
+}
+
 template <int EPI, int ACT>
-__device__ __forceinline__ void tile_epilogue(const TileProblem& q, int row, int n_tile, uint32_t tmem, int half) {
+__device__ __forceinline__ void tile_epilogue(const TileProblem& q, int row, int n_tile, const TileSums& sums, int c0,
+                                              int c1, float rs, const float (&cols)[2][128]) {
     const EpiParams& e = q.epi;
     const bool live = row < q.m;
     if constexpr (epi_is_gate(EPI)) {
         const int width = q.bn / 2;                  // output columns of the tile
-        const int c0 = half * (width / 2), c1 = c0 + width / 2;
-        const float rs = EPI == EPI_I8GATE && live ? e.row_scale[row] : 0.f;
         for (int c = c0; c < c1; c += 16) {
             uint32_t g[16], u[16];
-            tmem_ld16(tmem + c, g);
-            tmem_ld16(tmem + width + c, u);
-            tmem_wait16(g);
-            tmem_wait16(u);
+            sums.get<epi_is_i8(EPI)>(0, c, g);
+            sums.get<epi_is_i8(EPI)>(1, c, u);
             const int col = n_tile * width + c;
             const int valid = min(16, q.n - col);
             if (!live || valid <= 0) continue;
@@ -87,9 +160,8 @@ __device__ __forceinline__ void tile_epilogue(const TileProblem& q, int row, int
             if constexpr (EPI == EPI_I8GATE) {
 #pragma unroll
                 for (int j = 0; j < 16; ++j) {
-                    const int cc = j < valid ? col + j : col;
-                    const float gf = __fmul_rn(__fmul_rn(float(int(g[j])), rs), e.col_scale[0][cc]);
-                    const float uf = __fmul_rn(__fmul_rn(float(int(u[j])), rs), e.col_scale[1][cc]);
+                    const float gf = __fmul_rn(__fmul_rn(float(int(g[j])), rs), cols[0][c - c0 + j]);
+                    const float uf = __fmul_rn(__fmul_rn(float(int(u[j])), rs), cols[1][c - c0 + j]);
                     h[j] = gate_act(gf, e.act) * uf;
                 }
                 store16_dyn(e.out, VY_F32, int64_t(row) * e.ldo + col, h, valid, true);
@@ -110,12 +182,9 @@ __device__ __forceinline__ void tile_epilogue(const TileProblem& q, int row, int
             }
         }
     } else {
-        const int c0 = half * (q.bn / 2), c1 = c0 + q.bn / 2;
-        const float rs = EPI == EPI_I8 && live ? e.row_scale[row] : 0.f;
         for (int c = c0; c < c1; c += 16) {
             uint32_t r[16];
-            tmem_ld16(tmem + c, r);
-            tmem_wait16(r);
+            sums.get<epi_is_i8(EPI)>(0, c, r);
             const int col = n_tile * q.bn + c;
             const int valid = min(16, q.n - col);
             if (!live || valid <= 0) continue;
@@ -123,9 +192,8 @@ __device__ __forceinline__ void tile_epilogue(const TileProblem& q, int row, int
             if constexpr (EPI == EPI_I8) {
 #pragma unroll
                 for (int j = 0; j < 16; ++j) {
-                    const int cc = j < valid ? col + j : col;
-                    v[j] = __fmul_rn(__fmul_rn(float(int(r[j])), rs), e.col_scale[0][cc]);
-                    if (e.bias) v[j] = __fadd_rn(v[j], load_as_float(e.bias, e.bias_dtype, cc));
+                    v[j] = __fmul_rn(__fmul_rn(float(int(r[j])), rs), cols[0][c - c0 + j]);
+                    if (e.bias) v[j] = __fadd_rn(v[j], cols[1][c - c0 + j]);
                 }
                 store16_dyn(e.out, e.out_dtype, int64_t(row) * e.ldo + col, v, valid, e.vec != 0);
             } else if constexpr (EPI == EPI_STORE) {
@@ -153,18 +221,16 @@ __device__ __forceinline__ void load_gate(GateChunk& k, const EpiParams& e, int 
     }
 }
 template <int ACT>
-__device__ __forceinline__ void dgate_epilogue(const TileProblem& q, GateChunk& next, int row, int n_tile, uint32_t tmem,
-                                               int half) {
+__device__ __forceinline__ void dgate_epilogue(const TileProblem& q, GateChunk& next, int row, int n_tile,
+                                               const TileSums& sums, int c0, int c1) {
     const EpiParams& e = q.epi;
     const bool live = row < q.m;
-    const int c0 = half * (q.bn / 2), c1 = c0 + q.bn / 2;
     for (int c = c0; c < c1; c += 16) {
         const GateChunk k = next;
         const int col = n_tile * q.bn + c;
         if (c + 16 < c1) load_gate(next, e, row, col + 16, live, q.n);
         uint32_t r[16];
-        tmem_ld16(tmem + c, r);
-        tmem_wait16(r);
+        sums.get<false>(0, c, r);
         const int valid = min(16, q.n - col);
         if (!live || valid <= 0) continue;
         float dg[16], du[16], h[16];
@@ -184,15 +250,15 @@ __device__ __forceinline__ void dgate_epilogue(const TileProblem& q, GateChunk& 
 }
 
 template <int EPI, int ACT>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTileThreads, 1)
-    tile_kernel(const __grid_constant__ TileParams p) {
+__global__ void __launch_bounds__(kTileThreads, 1) tile_kernel(const __grid_constant__ TileParams p) {
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     TileSmem& S = *reinterpret_cast<TileSmem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     constexpr bool I8 = epi_is_i8(EPI);
     constexpr int kBlockK = I8 ? 128 : 64;      // elements of a 128-byte K block
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const uint32_t rank = cluster_rank();
-    const int cluster = blockIdx.x >> 1, n_clusters = gridDim.x >> 1;
+    const uint32_t place = cluster_rank(), rank = place & 1, leader = place & ~1u;
+    const int splits = p.splits, share = int(place >> 1);
+    const int cluster = blockIdx.x / (2 * splits), n_clusters = gridDim.x / (2 * splits);
 
     if (tid == 0) {
         for (int i = 0; i < kTileStages; ++i) {
@@ -217,29 +283,30 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTileThreads, 1)
     grid_dependents_launch();
 
     if (warp == 0) {
-        if (lane == 0) {
-            uint32_t it = 0;
-            bool go = true;
-            for (int tile = cluster; go && tile < p.n_tiles; tile += n_clusters) {
-                const TileAt t = tile_at(p, tile);
-                const TileProblem& q = p.prob[t.prob];
-                const int m0 = t.m * 256 + int(rank) * 128;
-                // a gated product's pair holds the same columns of gate (first CTA) and up
-                const int n0 = epi_is_gate(EPI) ? t.n * (q.bn / 2) : t.n * q.bn + int(rank) * (q.bn / 2);
-                const uint32_t bytes = 2u * (kHalfBytes + uint32_t(q.bn) * 64u);
-                for (int seg = 0; go && seg < 2; ++seg) {
-                    const CUtensorMap* ma = &q.a[epi_is_gate(EPI) ? 0 : seg];
-                    const CUtensorMap* mb = &q.b[epi_is_gate(EPI) ? rank : seg];
-                    for (int kb = 0; kb < q.nk[seg]; ++kb, ++it) {
-                        const uint32_t s = it % kTileStages;
-                        if (!mbar_wait(&S.empty[s], ((it / kTileStages) & 1) ^ 1, abort_flag, p.flags)) {
-                            go = false;
-                            break;
-                        }
-                        const uint32_t bar = map_to_rank(smem_u32(&S.full[s]), 0);
-                        if (rank == 0) mbar_expect_tx(&S.full[s], bytes);
+        uint32_t it = 0, stage = 0, phase = 1;      // phase: parity the ring's next pass waits for
+        bool go = true;
+        for (int tile = cluster; go && tile < p.n_tiles; tile += n_clusters) {
+            const TileAt t = tile_at(p, tile);
+            const TileProblem& q = p.prob[t.prob];
+            const int m0 = t.m * 256 + int(rank) * 128;
+            // a gated product's pair holds the same columns of gate (first CTA) and up
+            const int n0 = epi_is_gate(EPI) ? t.n * (q.bn / 2) : t.n * q.bn + int(rank) * (q.bn / 2);
+            const uint32_t bytes = 2u * (kHalfBytes + uint32_t(q.bn) * 64u);
+            const int nk = q.nk[0] + q.nk[1], k_first = nk * share / splits, k_last = nk * (share + 1) / splits;
+            for (int seg = 0; go && seg < 2; ++seg) {
+                const CUtensorMap* ma = &q.a[epi_is_gate(EPI) ? 0 : seg];
+                const CUtensorMap* mb = &q.b[epi_is_gate(EPI) ? rank : seg];
+                const int before = seg ? q.nk[0] : 0, last = min(q.nk[seg], k_last - before);
+                for (int kb = max(0, k_first - before); kb < last; ++kb, ++it) {
+                    if (!mbar_wait_warp(&S.empty[stage], phase, abort_flag, p.flags)) {
+                        go = false;
+                        break;
+                    }
+                    if (elect_one()) {
+                        const uint32_t bar = map_to_rank(smem_u32(&S.full[stage]), leader);
+                        if (rank == 0) mbar_expect_tx(&S.full[stage], bytes);
                         const int k0 = kb * kBlockK;
-                        const uint32_t da = smem_u32(S.a[s]), db = smem_u32(S.b[s]);
+                        const uint32_t da = smem_u32(S.a[stage]), db = smem_u32(S.b[stage]);
                         if (!I8 && q.a_mn) {
                             tma_load_2d_pair(da, ma, m0, k0, bar);
                             tma_load_2d_pair(da + 8192, ma, m0 + 64, k0, bar);
@@ -253,46 +320,53 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTileThreads, 1)
                             tma_load_2d_pair(db, mb, k0, n0, bar);
                         }
                     }
+                    __syncwarp();
+                    if (++stage == kTileStages) stage = 0, phase ^= 1;
                 }
             }
-            // every stage this loader filled is read before the CTA may leave (bounded)
+        }
+        // every stage this loader filled is read before the CTA may leave (bounded)
+        if (lane == 0) {
             for (uint32_t i = 0; i < kTileStages && i < it; ++i) {
                 const uint32_t last = it - 1 - i;
                 mbar_drain(&S.empty[last % kTileStages], (last / kTileStages) & 1, p.flags);
             }
         }
     } else if (warp == 1) {
-        if (lane == 0 && rank == 0) {
-            uint32_t it = 0, n = 0;
+        if (rank == 0) {
+            uint32_t n = 0, stage = 0, phase = 0;
             bool go = true;
             for (int tile = cluster; go && tile < p.n_tiles; tile += n_clusters, ++n) {
                 const TileProblem& q = p.prob[tile_at(p, tile).prob];
                 const uint32_t idesc = umma_idesc(I8, ACT == VY_BF16, q.a_mn, q.b_mn, 256, q.bn);
-                const uint32_t a_lbo = q.a_mn ? 8192 : 16, b_lbo = q.b_mn ? 8192 : 16;
                 // one MMA's K (32 bytes): along the swizzled row, or 16 rows of 128 bytes
                 const uint32_t a_step = q.a_mn ? 128 : 2, b_step = q.b_mn ? 128 : 2;
+                const uint64_t a_desc = umma_desc(smem_u32(S.a[0]), q.a_mn ? 8192 : 16, 1024);
+                const uint64_t b_desc = umma_desc(smem_u32(S.b[0]), q.b_mn ? 8192 : 16, 1024);
                 const uint32_t buf = n & 1, d = tmem + buf * 256;
-                const int nk = q.nk[0] + q.nk[1];
-                if (!mbar_wait(&S.acc_empty[buf], ((n >> 1) & 1) ^ 1, abort_flag, p.flags)) break;
+                const int nk = q.nk[0] + q.nk[1], blocks = nk * (share + 1) / splits - nk * share / splits;
+                if (!mbar_wait_warp(&S.acc_empty[buf], ((n >> 1) & 1) ^ 1, abort_flag, p.flags)) break;
                 tc_fence_after();
-                for (int kb = 0; kb < nk; ++kb, ++it) {
-                    const uint32_t s = it % kTileStages;
-                    if (!mbar_wait(&S.full[s], (it / kTileStages) & 1, abort_flag, p.flags)) {
+                for (int kb = 0; kb < blocks; ++kb) {
+                    if (!mbar_wait_warp(&S.full[stage], phase, abort_flag, p.flags)) {
                         go = false;
                         break;
                     }
                     tc_fence_after();
-                    const uint64_t da = umma_desc(smem_u32(S.a[s]), a_lbo, 1024);
-                    const uint64_t db = umma_desc(smem_u32(S.b[s]), b_lbo, 1024);
+                    if (elect_one()) {
+                        const uint64_t da = a_desc + stage * (kHalfBytes >> 4), db = b_desc + stage * (kHalfBytes >> 4);
 #pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        mma_ss<I8, 1>(d, da + k * a_step, db + k * b_step, idesc, (kb | k) != 0);
-                    mma_commit_pair(&S.empty[s]);
+                        for (int k = 0; k < 4; ++k)
+                            mma_ss<I8, 1>(d, da + k * a_step, db + k * b_step, idesc, kb != 0 || k != 0);
+                        mma_commit_pair(&S.empty[stage], leader);
+                        if (kb == blocks - 1) mma_commit_pair(&S.acc_full[buf], leader);
+                    }
+                    __syncwarp();
+                    if (++stage == kTileStages) stage = 0, phase ^= 1;
                 }
-                if (go) mma_commit_pair(&S.acc_full[buf]);
             }
         }
-    } else if (warp >= 4) {
+    } else if (warp >= 4 && splits == 1) {
         const int quarter = warp & 3, half = (warp - 4) >> 2;
         uint32_t n = 0;
         for (int tile = cluster; tile < p.n_tiles; tile += n_clusters, ++n) {
@@ -300,20 +374,55 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTileThreads, 1)
             const uint32_t buf = n & 1;
             const TileProblem& q = p.prob[t.prob];
             const int row = t.m * 256 + int(rank) * 128 + quarter * 32 + lane;
-            const uint32_t acc = tmem + buf * 256 + (uint32_t(quarter * 32) << 16);
+            const int width = epi_is_gate(EPI) ? q.bn / 2 : q.bn, c0 = half * (width / 2), c1 = c0 + width / 2;
+            const TileSums sums{tmem + buf * 256 + (uint32_t(quarter * 32) << 16), nullptr, 1, 0, width,
+                                epi_is_gate(EPI) ? 2 : 1, width};
             GateChunk first;
-            if constexpr (EPI == EPI_DGATE)
-                load_gate(first, q.epi, row, t.n * q.bn + half * (q.bn / 2), row < q.m, q.n);
+            if constexpr (EPI == EPI_DGATE) load_gate(first, q.epi, row, t.n * q.bn + c0, row < q.m, q.n);
+            load_cols<EPI>(S.cols[warp & 7], q, t.n, c0, c1);
+            const float rs = epi_is_i8(EPI) && row < q.m ? q.epi.row_scale[row] : 0.f;
             const bool ready = mbar_wait(&S.acc_full[buf], (n >> 1) & 1, abort_flag, p.flags);
             if (!__all_sync(0xffffffffu, ready)) break;
             tc_fence_after();
             if constexpr (EPI == EPI_DGATE)
-                dgate_epilogue<ACT>(q, first, row, t.n, acc, half);
+                dgate_epilogue<ACT>(q, first, row, t.n, sums, c0, c1);
             else
-                tile_epilogue<EPI, ACT>(q, row, t.n, acc, half);
+                tile_epilogue<EPI, ACT>(q, row, t.n, sums, c0, c1, rs, S.cols[warp & 7]);
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive_remote(map_to_rank(smem_u32(&S.acc_empty[buf]), 0));
+            if (lane == 0) mbar_arrive_remote(map_to_rank(smem_u32(&S.acc_empty[buf]), leader));
+        }
+    }
+    if (splits > 1) {
+        // one tile a cluster: send, meet, add my columns
+        const int quarter = warp & 3, half = (warp - 4) >> 2;
+        const TileAt t = tile_at(p, cluster);
+        const TileProblem& q = p.prob[t.prob];
+        const int row = t.m * 256 + int(rank) * 128 + quarter * 32 + lane;
+        const int width = epi_is_gate(EPI) ? q.bn / 2 : q.bn, own = width / splits;
+        const int c0 = share * own + half * (own / 2), c1 = c0 + own / 2;
+        const TileSums sums{tmem + (uint32_t(quarter * 32) << 16),
+                            reinterpret_cast<const float4*>(S.a) + quarter * 32 + lane, splits, share * own, own,
+                            epi_is_gate(EPI) ? 2 : 1, width};
+        GateChunk first;
+        bool ready = false;
+        const float rs = epi_is_i8(EPI) && row < q.m ? q.epi.row_scale[row] : 0.f;
+        __syncwarp();
+        if (warp >= 4) {
+            load_cols<EPI>(S.cols[warp & 7], q, t.n, c0, c1);
+            if constexpr (EPI == EPI_DGATE) load_gate(first, q.epi, row, t.n * q.bn + c0, row < q.m, q.n);
+            ready = __all_sync(0xffffffffu, mbar_wait(&S.acc_full[0], 0, abort_flag, p.flags));
+            tc_fence_after();
+        }
+        cluster_sync();      // every pair's MMAs are done: the rings may be written over
+        if (ready) sums.send(smem_u32(S.a) + (quarter * 32 + lane) * 16, rank, share, half);
+        __syncwarp();
+        cluster_sync();
+        if (ready) {
+            if constexpr (EPI == EPI_DGATE)
+                dgate_epilogue<ACT>(q, first, row, t.n, sums, c0, c1);
+            else
+                tile_epilogue<EPI, ACT>(q, row, t.n, sums, c0, c1, rs, S.cols[warp & 7]);
         }
     }
     __syncwarp();
@@ -334,26 +443,45 @@ inline int tile_operand(CUtensorMap* map, int dtype, const void* base, int64_t r
               : make_map_2d(map, dtype, base, rows, k, ld, block, box_rows);
 }
 
-// Tile columns: 256, unless that leaves most of the clusters without a tile.
-inline int tile_columns(int64_t m, int64_t n, int clusters) {
-    const int64_t wide = ((m + 255) / 256) * ((n + 255) / 256);
-    return wide * 2 <= clusters ? 128 : 256;
+// Lays a launch's problems out (sizes and K blocks set): tile columns, tiles, K shares.  A gated
+// product's tile has bn / 2 output columns.  `pairs`: CTA pairs the device runs at once.
+constexpr int kShareLeast = 16;      // K blocks a pair's share is worth joining for
+inline void tile_layout(TileParams* p, bool gate, int pairs) {
+    int least = 1 << 30, wide = 0;
+    for (int i = 0; i < p->n_problems; ++i) {
+        const TileProblem& q = p->prob[i];
+        const int n = gate ? 2 * q.n : q.n;
+        if (q.nk[0] + q.nk[1] < least) least = q.nk[0] + q.nk[1];
+        wide += (q.m + 255) / 256 * ((n + 255) / 256);
+    }
+    p->splits = 1;
+    while (p->splits < 4 && wide * p->splits * 2 <= pairs && least >= kShareLeast * p->splits * 2) p->splits *= 2;
+    const bool narrow = p->splits == 1 && wide * 2 <= pairs;
+    p->n_tiles = 0;
+    for (int i = 0; i < p->n_problems; ++i) {
+        TileProblem& q = p->prob[i];
+        q.bn = narrow || (gate ? 2 * q.n : q.n) <= 128 ? 128 : 256;
+        if (q.bn == 128 && p->splits > 2) p->splits = 2;      // an epilogue warp takes 16 columns at least
+        const int width = gate ? q.bn / 2 : q.bn;
+        q.m_tiles = (q.m + 255) / 256;
+        q.n_tiles = (q.n + width - 1) / width;
+        q.first = p->n_tiles;
+        p->n_tiles += q.m_tiles * q.n_tiles;
+    }
 }
 
-// Gives problem i (its sizes and bn set, problems before it placed) its tiles; a gated product's
-// tile has bn / 2 output columns.
-inline void tile_place(TileParams* p, int i, bool gate) {
-    TileProblem& q = p->prob[i];
-    const int width = gate ? q.bn / 2 : q.bn;
-    q.m_tiles = (q.m + 255) / 256;
-    q.n_tiles = (q.n + width - 1) / width;
-    q.first = p->n_tiles;
-    p->n_tiles += q.m_tiles * q.n_tiles;
-    p->n_problems = i + 1;
+// Adds a problem to a launch: m x n, K blocks of its two segments.
+inline TileProblem& tile_add(TileParams* p, int64_t m, int64_t n, int nk0, int nk1 = 0) {
+    TileProblem& q = p->prob[p->n_problems++];
+    q.m = static_cast<int>(m);
+    q.n = static_cast<int>(n);
+    q.nk[0] = nk0;
+    q.nk[1] = nk1;
+    return q;
 }
 
 template <int EPI, int ACT>
-int tile_launch(TileParams& p, const DeviceInfo* dev, cudaStream_t s) {
+int tile_launch(const TileParams& p, int pairs, cudaStream_t s) {
     auto kern = tile_kernel<EPI, ACT>;
     constexpr int smem = sizeof(TileSmem) + 1024;
     int st = once_per_device(reinterpret_cast<const void*>(kern), [](int, void* k) {
@@ -361,9 +489,21 @@ int tile_launch(TileParams& p, const DeviceInfo* dev, cudaStream_t s) {
         return e == cudaSuccess ? VY_OK : fail(VY_ERR_CUDA, "dense GEMM shared memory: %s", cudaGetErrorString(e));
     }, reinterpret_cast<void*>(kern));
     if (st != VY_OK) return st;
-    const int pairs = dev->sm_count / 2;
     const int clusters = p.n_tiles < pairs ? p.n_tiles : pairs;
-    const cudaError_t e = launch_chained(kern, dim3(2 * clusters), dim3(kTileThreads), smem, s, p);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(2 * p.splits * clusters);
+    cfg.blockDim = dim3(kTileThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = 2 * p.splits;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, p);
     if (e != cudaSuccess) return fail(VY_ERR_CUDA, "dense GEMM launch: %s", cudaGetErrorString(e));
     return VY_OK;
 }

@@ -102,6 +102,19 @@ __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.a
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
+// True in one lane of a converged warp.  The loops that feed the tensor core run in whole warps and only
+// the issue itself in the elected lane: around code of one lane the compiler cannot keep descriptors
+// and coordinates in uniform registers, which TMA and MMA instructions take them from.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t r;
+    asm volatile("{ .reg .pred p; elect.sync _|p, 0xffffffff; selp.u32 %0, 1, 0, p; }" : "=r"(r));
+    return r != 0;
+}
+// A whole warp's bounded wait.
+__device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int32_t* err) {
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, err));
+}
+
 // ── tcgen05 on a CTA pair ───────────────────────────────────────────────────────────────────
 
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -171,13 +184,13 @@ __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint3
     else VY_MMA_SS("cta_group::1", "f16");
 #undef VY_MMA_SS
 }
-// Arrives on `bar` (of both CTAs of the pair, the same offset in each) once every MMA this thread
-// issued before it has completed.
-__device__ __forceinline__ void mma_commit_pair(uint64_t* bar) {
+// Arrives on `bar` (of both CTAs of the pair whose first has cluster rank `leader`, the same offset in
+// each) once every MMA this thread issued before it has completed.
+__device__ __forceinline__ void mma_commit_pair(uint64_t* bar, uint32_t leader) {
     asm volatile(
         "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
             smem_u32(bar)),
-        "h"(static_cast<uint16_t>(3))
+        "h"(static_cast<uint16_t>(3u << leader))
         : "memory");
 }
 __device__ __forceinline__ void mma_commit_one(uint64_t* bar) {
