@@ -139,60 +139,58 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(const __grid_con
     }
 
     if (warp == 4) {
-        if (lane == 0) {
-            auto load_w = [&](int i) {
-                const uint32_t s = i % p.stages;
-                const int k = (k_first + i) * kBlockK;
-                unsigned char* at = ring + s * stage_bytes;
-                mbar_expect_tx(&S.full[s], stage_bytes);
-                tma_load_2d(at, &p.w[0], k, row0, &S.full[s]);
-                if (NW == 2) tma_load_2d(at + 16384, &p.w[1], k, row0, &S.full[s]);
-            };
-            auto load_x = [&](int i) {
-                const uint32_t s = i % p.stages;
-                tma_load_2d(ring + s * stage_bytes + NW * 16384, &p.x, (k_first + i) * kBlockK, 0, &S.full[s]);
-            };
-            int ahead = 0;
-            if (p.early)
-                for (; ahead < p.stages && ahead < nk; ++ahead) load_w(ahead);
-            grid_dependency_wait();
-            grid_dependents_launch();
-            for (int i = 0; i < ahead; ++i) load_x(i);
-            int i = ahead;
-            for (; i < nk; ++i) {
-                if (i >= p.stages && !mbar_wait(&S.empty[i % p.stages], ((i / p.stages) & 1) ^ 1, abort_flag, p.flags)) break;
-                load_w(i);
-                load_x(i);
+        auto load_w = [&](int i, uint32_t s) {
+            const int k = (k_first + i) * kBlockK;
+            unsigned char* at = ring + s * stage_bytes;
+            mbar_expect_tx(&S.full[s], stage_bytes);
+            tma_load_2d(at, &p.w[0], k, row0, &S.full[s]);
+            if (NW == 2) tma_load_2d(at + 16384, &p.w[1], k, row0, &S.full[s]);
+        };
+        auto load_x = [&](int i, uint32_t s) {
+            tma_load_2d(ring + s * stage_bytes + NW * 16384, &p.x, (k_first + i) * kBlockK, 0, &S.full[s]);
+        };
+        const int ahead = p.early ? min(p.stages, nk) : 0;
+        if (elect_one())
+            for (int i = 0; i < ahead; ++i) load_w(i, i);
+        __syncwarp();
+        grid_dependency_wait();
+        grid_dependents_launch();
+        if (elect_one())
+            for (int i = 0; i < ahead; ++i) load_x(i, i);
+        __syncwarp();
+        int i = ahead, stage = ahead == p.stages ? 0 : ahead;
+        uint32_t phase = ahead == p.stages ? 0 : 1;      // parity the ring's next pass waits for
+        for (; i < nk; ++i) {
+            if (!mbar_wait_warp(&S.empty[stage], phase, abort_flag, p.flags)) break;
+            if (elect_one()) {
+                load_w(i, stage);
+                load_x(i, stage);
             }
-            // all loads have landed and been read before the ring is used again or the CTA leaves
-            for (int j = max(0, i - p.stages); j < i; ++j) mbar_drain(&S.empty[j % p.stages], (j / p.stages) & 1, p.flags);
-        } else {
-            grid_dependency_wait();
-            grid_dependents_launch();
+            __syncwarp();
+            if (++stage == p.stages) stage = 0, phase ^= 1;
         }
+        // all loads have landed and been read before the ring is used again or the CTA leaves
+        if (lane == 0)
+            for (int j = max(0, i - p.stages); j < i; ++j) mbar_drain(&S.empty[j % p.stages], (j / p.stages) & 1, p.flags);
     } else if (warp == 5) {
-        if (lane == 0) {
-            const uint32_t idesc = umma_idesc(I8, ACT == VY_BF16, 0, 0, kStreamRows, p.cols);
-            bool go = true;
-            for (int i = 0; i < nk; ++i) {
-                const uint32_t s = i % p.stages;
-                if (!mbar_wait(&S.full[s], (i / p.stages) & 1, abort_flag, p.flags)) {
-                    go = false;
-                    break;
-                }
-                tc_fence_after();
-                const uint32_t at = smem_u32(ring) + s * stage_bytes;
-                const uint64_t dx = umma_desc(at + NW * 16384, 16, 1024);
+        const uint32_t idesc = umma_idesc(I8, ACT == VY_BF16, 0, 0, kStreamRows, p.cols);
+        const uint64_t first = umma_desc(smem_u32(ring), 16, 1024);
+        uint32_t stage = 0, phase = 0;
+        for (int i = 0; i < nk; ++i) {
+            if (!mbar_wait_warp(&S.full[stage], phase, abort_flag, p.flags)) break;
+            tc_fence_after();
+            if (elect_one()) {
+                const uint64_t dw = first + (stage * stage_bytes >> 4), dx = dw + NW * 1024;
 #pragma unroll
-                for (int m = 0; m < NW; ++m) {
-                    const uint64_t dw = umma_desc(at + m * 16384, 16, 1024);
+                for (int m = 0; m < NW; ++m)
 #pragma unroll
                     for (int k = 0; k < 4; ++k)
-                        mma_ss<I8, 0>(tmem + m * p.cols, dw + 2 * k, dx + 2 * k, idesc, (i | k) != 0);
-                }
-                mma_commit_one(&S.empty[s]);
+                        mma_ss<I8, 0>(tmem + m * p.cols, dw + m * 1024 + 2 * k, dx + 2 * k, idesc, i != 0 || k != 0);
+                mma_commit_one(&S.empty[stage]);
+                if (i == nk - 1) mma_commit_one(&S.done);
             }
-            if (go) mma_commit_one(&S.done);
+            __syncwarp();
+            if (++stage == uint32_t(p.stages)) stage = 0, phase ^= 1;
         }
     }
     __syncwarp();
