@@ -23,54 +23,55 @@ struct QuantParams {
     bool vec;      // rows take 16-byte loads, codes the stores that go with them
 };
 
-// A code is the nearest integer of the exact quotient x / s, ties to even.  t = x * (1/s) is off by
-// at most 2^-23 relative (two roundings), 1.6e-5 for |t| <= 127.5, so rounding t decides every value
-// that is not that near a tie c; for the rest (about one in 20,000) the sign of x - c s decides, which
-// one fused multiply-add gives exactly (c s and the difference are exact before its one rounding, and
-// nothing underflows at these scales).  Adding 1.5 * 2^23 rounds t to the nearest integer, even on
-// ties, and leaves its two's complement in the low bits: no conversion instruction, whose rate would
-// bound the kernel (rint and float-to-int run at an eighth of the adds' rate).
+// A code is the nearest integer of the exact quotient x / s, ties to even.  With 1 / s rounded down
+// and up, one fused multiply-add each rounds x lo and x hi to the nearest integer (adding 1.5 * 2^23,
+// which leaves the integer's two's complement in the low bits); x / s lies between the two products
+// and rounding is monotone, so where both give one integer it is the code.  Where they differ (about
+// one value in 10^5: a tie c lies between), the sign of x - c s decides, exact under one fused
+// multiply-add.  Two FFMAs and a LOP3 a value; rint and float-to-int conversions run at an eighth of
+// that rate and would bound the kernel; following the distance to the nearest tie instead took some 20
+// instructions a value in all (4096 x 14336, bf16: 46 us, 36 this way).
 constexpr float kRound = 12582912.f;
-constexpr float kNearTie = 0.5f - 3e-5f;
 
 struct RowScale {
-    float s, inv;
-    float up;       // 1, or 2^100 where 1 / s is out of range: x and s are scaled by it, exactly
-    bool zero;      // a zero row, or a NaN scale: all codes 0
+    float s, lo, hi;
+    float up;           // 1, or 2^100 where 1 / s is out of range: x and s are scaled by it, exactly
+    uint32_t odd;       // not zero when up is not 1: every value takes the long way
+    uint32_t keep;      // 0 for a zero row or a NaN scale: all codes 0; else all ones
 };
+
+__device__ __forceinline__ float quant_long(float v, const RowScale& r) {
+    const float x = v * r.up, s = r.s * r.up;
+    const float t = x * __frcp_rn(s);
+    const float near = (t + kRound) - kRound, d = t - near;
+    float q = near;
+    if (fabsf(d) > 0.499f) {                      // t is off by 2^-23 relative at most
+        const float c = near + copysignf(0.5f, d);
+        const float e = fmaf(-c, s, x);           // c s has 32 bits, nothing underflows: the sign is exact
+        q = e > 0.f ? c + 0.5f : e < 0.f ? c - 0.5f : c;     // c + kRound goes to the even one
+    }
+    // a subnormal s may be so coarse that amax / s passes 127
+    return fminf(fmaxf(q, -127.f), 127.f) + kRound;
+}
 
 // The codes of N values, N / 4 words.
 template <int N>
 __device__ __forceinline__ void quant_words(const float (&v)[N], const RowScale& r, uint32_t (&w)[N / 4]) {
-    float far = 0.f;
-    float m[N];
+    uint32_t m[N], differ = r.odd;
 #pragma unroll
     for (int j = 0; j < N; ++j) {
-        const float t = v[j] * r.inv;
-        m[j] = t + kRound;
-        far = fmaxf(far, fabsf(t - (m[j] - kRound)));
+        m[j] = __float_as_uint(fmaf(v[j], r.lo, kRound));
+        differ |= m[j] ^ __float_as_uint(fmaf(v[j], r.hi, kRound));
     }
-    if (far > kNearTie || r.up != 1.f) {
+    if (differ) {
 #pragma unroll
-        for (int j = 0; j < N; ++j) {
-            const float x = v[j] * r.up, s = r.s * r.up;
-            const float t = r.up != 1.f ? x * __frcp_rn(s) : v[j] * r.inv;
-            const float near = (t + kRound) - kRound, d = t - near;
-            float q = near;
-            if (fabsf(d) > kNearTie) {
-                const float c = near + copysignf(0.5f, d);
-                const float e = fmaf(-c, s, x);
-                q = e > 0.f ? c + 0.5f : e < 0.f ? c - 0.5f : c;     // c + kRound goes to the even one
-            }
-            // a subnormal s may be so coarse that amax / s passes 127
-            m[j] = fminf(fmaxf(q, -127.f), 127.f) + kRound;
-        }
+        for (int j = 0; j < N; ++j) m[j] = __float_as_uint(quant_long(v[j], r));
     }
 #pragma unroll
     for (int q = 0; q < N / 4; ++q) {
-        const uint32_t lo = __byte_perm(__float_as_uint(m[4 * q]), __float_as_uint(m[4 * q + 1]), 0x0040);
-        const uint32_t hi = __byte_perm(__float_as_uint(m[4 * q + 2]), __float_as_uint(m[4 * q + 3]), 0x0040);
-        w[q] = r.zero ? 0u : __byte_perm(lo, hi, 0x5410);
+        const uint32_t lo = __byte_perm(m[4 * q], m[4 * q + 1], 0x0040);
+        const uint32_t hi = __byte_perm(m[4 * q + 2], m[4 * q + 3], 0x0040);
+        w[q] = __byte_perm(lo, hi, 0x5410) & r.keep;
     }
 }
 
@@ -101,29 +102,67 @@ struct Piece {
             }
         }
     }
-    // 16-bit types: of each half in place (the two maxima of a word never mix), fp32: of the word
+    // 16-bit types: of each half in place, fp32: of the word
     static __device__ __forceinline__ uint32_t top(uint32_t t, const uint4& u) {
         const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             if constexpr (DT == VY_F32)
                 t = max(t, w[j] & 0x7FFFFFFFu);
+            else if constexpr (DT == VY_BF16)
+                asm("max.NaN.bf16x2 %0, %0, %1;" : "+r"(t) : "r"(w[j] & 0x7FFF7FFFu));
             else
-                t = __vmaxu2(t, w[j] & 0x7FFF7FFFu);
+                asm("max.NaN.f16x2 %0, %0, %1;" : "+r"(t) : "r"(w[j] & 0x7FFF7FFFu));
         }
         return t;
     }
     // the fp32 magnitude's pattern from top's
     static __device__ __forceinline__ uint32_t wide(uint32_t t) {
         if constexpr (DT == VY_F32) return t;
-        const uint32_t h = max(t & 0xFFFFu, t >> 16);
-        return __float_as_uint(act_from_bits<DT>(h)) & 0x7FFFFFFFu;
+        const uint32_t a = __float_as_uint(act_from_bits<DT>(t & 0xFFFFu)) & 0x7FFFFFFFu;
+        return max(a, __float_as_uint(act_from_bits<DT>(t >> 16)) & 0x7FFFFFFFu);
     }
 };
 
+// The scale of a row whose largest magnitude has the pattern `top`.
+__device__ __forceinline__ RowScale row_scale(uint32_t top) {
+    RowScale r;
+    r.s = top < 0x7F800000u ? __fdiv_rn(__uint_as_float(top), 127.f) : __uint_as_float(0x7FC00000u);
+    const bool zero = !(r.s > 0.f), tiny = r.s < 1e-30f && !zero;
+    r.up = tiny ? 0x1p100f : 1.f;
+    r.odd = tiny;
+    r.keep = zero ? 0u : 0xFFFFFFFFu;
+    r.lo = zero || tiny ? 0.f : __frcp_rd(r.s);
+    r.hi = zero || tiny ? 0.f : __frcp_ru(r.s);
+    return r;
+}
+// Codes of a row's 16-byte piece `at`.
+template <int DT>
+__device__ __forceinline__ void put_piece(int8_t* out, int64_t at, const uint4& u, const RowScale& r) {
+    using P = Piece<DT>;
+    float v[P::N];
+    uint32_t w[P::N / 4];
+    P::values(u, v);
+    quant_words<P::N>(v, r, w);
+    if constexpr (P::N == 8)
+        reinterpret_cast<uint2*>(out)[at] = make_uint2(w[0], w[1]);
+    else
+        reinterpret_cast<uint32_t*>(out)[at] = w[0];
+}
+// Codes of single values k, k + step, ... below cols (rows that are no whole pieces, or not aligned).
+template <int DT>
+__device__ __forceinline__ void put_tail(int8_t* out, const void* src, int64_t k, int64_t cols, int step, const RowScale& r) {
+    for (; k < cols; k += step) {
+        const float v[4] = {load_as_float(src, DT, k), 0.f, 0.f, 0.f};
+        uint32_t w[1];
+        quant_words<4>(v, r, w);
+        out[k] = static_cast<int8_t>(w[0] & 0xFFu);
+    }
+}
+
 // One block per row; the row stays in registers between its maximum and its codes.
-template <int DT, int THREADS, int UNITS>
-__global__ void __launch_bounds__(THREADS) quantize_kernel(QuantParams p) {
+template <int DT, int THREADS, int UNITS, int BLOCKS>
+__global__ void __launch_bounds__(THREADS, BLOCKS) quantize_kernel(QuantParams p) {
     using P = Piece<DT>;
     __shared__ uint32_t part[THREADS / 32];
     grid_dependency_wait();
@@ -156,57 +195,43 @@ __global__ void __launch_bounds__(THREADS) quantize_kernel(QuantParams p) {
     __syncthreads();
     top = __reduce_max_sync(0xffffffffu, part[(tid & 31) % (THREADS / 32)]);
 
-    RowScale r;
-    r.s = top < 0x7F800000u ? __fdiv_rn(__uint_as_float(top), 127.f) : __uint_as_float(0x7FC00000u);
-    r.zero = !(r.s > 0.f);
-    r.up = r.s < 1e-30f && !r.zero ? 0x1p100f : 1.f;
-    r.inv = r.zero || r.up != 1.f ? 0.f : __frcp_rn(r.s);
+    const RowScale r = row_scale(top);
     if (tid == 0) p.scales[row] = r.s;
     int8_t* out = p.codes + row * p.cols;
-    auto put = [&](int64_t at, const uint4& u) {
-        float v[P::N];
-        uint32_t w[P::N / 4];
-        P::values(u, v);
-        quant_words<P::N>(v, r, w);
-        if constexpr (P::N == 8)
-            reinterpret_cast<uint2*>(out)[at] = make_uint2(w[0], w[1]);
-        else
-            reinterpret_cast<uint32_t*>(out)[at] = w[0];
-    };
     if (fits) {
 #pragma unroll
         for (int i = 0; i < UNITS; ++i) {
             const int64_t at = tid + i * THREADS;
-            if (at < n) put(at, keep[i]);
+            if (at < n) put_piece<DT>(out, at, keep[i], r);
         }
     } else {
-        for (int64_t at = tid; at < n; at += THREADS) put(at, ld_piece(pieces + at));
+        for (int64_t at = tid; at < n; at += THREADS) put_piece<DT>(out, at, ld_piece(pieces + at), r);
     }
-    for (int64_t k = n * P::N + tid; k < p.cols; k += THREADS) {
-        const float v[4] = {load_as_float(src, DT, k), 0.f, 0.f, 0.f};
-        uint32_t w[1];
-        quant_words<4>(v, r, w);
-        out[k] = static_cast<int8_t>(w[0] & 0xFFu);
-    }
+    put_tail<DT>(out, src, n * P::N + tid, p.cols, THREADS, r);
 }
 
 template <int DT>
 int launch_quantize_as(const QuantParams& p, int sm_count, cudaStream_t s) {
     const int64_t n = p.cols / Piece<DT>::N;
-    // Threads of a row's block, and 16-byte pieces each keeps in registers: enough that the row fits;
-    // with fewer rows than SMs, as many threads as the row can use, since one block's latency is the
-    // call's.  (A row past 8192 pieces is read twice.)
+    // Threads of a row's block, and 16-byte pieces each keeps in registers.  Many rows: few threads
+    // with many pieces, so that several blocks share an SM and one's loads run under another's
+    // arithmetic.  Fewer rows than SMs: as many threads as the row can use, since one block's latency
+    // is the call's.  (A row past 8192 pieces is read twice.)
     const bool few = p.rows <= sm_count;
-    void (*kern)(QuantParams) = quantize_kernel<DT, 1024, 8>;
+    void (*kern)(QuantParams) = quantize_kernel<DT, 1024, 8, 1>;
     int threads = 1024;
     if (few ? n <= 64 : n <= 128)
-        kern = quantize_kernel<DT, 64, 2>, threads = 64;
-    else if (few ? n <= 256 : n <= 512)
-        kern = quantize_kernel<DT, 256, 2>, threads = 256;
+        kern = quantize_kernel<DT, 64, 2, 8>, threads = 64;
+    else if (few && n <= 256)
+        kern = quantize_kernel<DT, 256, 2, 4>, threads = 256;
+    else if (!few && n <= 512)
+        kern = quantize_kernel<DT, 128, 4, 8>, threads = 128;
     else if (few && n <= 2048)
-        kern = quantize_kernel<DT, 1024, 2>, threads = 1024;
+        kern = quantize_kernel<DT, 1024, 2, 1>, threads = 1024;
     else if (n <= 2048)
-        kern = quantize_kernel<DT, 512, 4>, threads = 512;
+        kern = quantize_kernel<DT, 256, 8, 4>, threads = 256;
+    else if (n <= 4096)
+        kern = quantize_kernel<DT, 512, 8, 2>, threads = 512;
     const cudaError_t e = launch_chained(kern, dim3(static_cast<unsigned>(p.rows)), dim3(threads), 0, s, p);
     return e == cudaSuccess ? VY_OK : fail(VY_ERR_CUDA, "int8 quantise launch: %s", cudaGetErrorString(e));
 }
