@@ -423,9 +423,9 @@ int64_t vy_gated_ffn_saved_floats(int64_t n_tokens, int32_t inter);
 size_t vy_gated_ffn_workspace_size(const vy_ffn_call* call, int32_t backward);
 
 /*
- * out = (act(x Wg^T) * (x Wu^T)) Wd^T with fp32 sums; g and u stay in fp32, the hidden row
- * h = act(g) * u is rounded once to the activation type (it is a tensor-core operand of the second
- * product), and so is out.
+ * out = (act(x Wg^T) * (x Wu^T)) Wd^T with fp32 sums; g and u stay in fp32.  The hidden row
+ * h = act(g) * u is a tensor-core operand of the second product: it is rounded once to the activation
+ * type, or with up to 32 tokens to a sum of two such values.  out is rounded once.
  */
 int vy_gated_ffn_forward(const vy_ffn_call* call, void* stream);
 
@@ -433,7 +433,7 @@ int vy_gated_ffn_forward(const vy_ffn_call* call, void* stream);
  * The gradients of that block from d_out and the forward call's `saved`:
  *   dh = d_out Wd;  dg = dh * u * act'(g);  du = dh * act(g)
  *   d_x = dg Wg + du Wu;  d_w_gate = dg^T x;  d_w_up = du^T x;  d_w_down = d_out^T h
- * fp32 sums; dg, du and h are rounded once to the activation type (tensor-core operands).
+ * fp32 sums; dg, du and h are rounded like the forward call's h.
  */
 int vy_gated_ffn_backward(const vy_ffn_call* call, void* stream);
 

@@ -81,6 +81,29 @@ __device__ __forceinline__ void store16_dyn(void* p, int dtype, int64_t at, cons
         if (j < valid) store_as(p, dtype, at + j, v[j]);
 }
 
+// g and u in fp32 between the passes, in the order the tile epilogues move them: blocks of 32 tokens x
+// 16 channels, g before u, each [4 channels][32 tokens][4 channels], so that a warp (a token per lane)
+// reads and writes its chunk of 16 columns as eight whole 512-byte lines.  (One column after another
+// over all tokens, 32 separate 128-byte lines a chunk: 235 us for dh at 2048 x 4096 x 14336, 214
+// this way.)
+constexpr int kSavedBlock = 2 * 16 * 32;
+__host__ __device__ constexpr int64_t saved_bands(int64_t tokens) { return (tokens + 31) / 32; }
+__device__ __forceinline__ int64_t saved_at(int64_t bands, int64_t token, int channel) {
+    return ((channel >> 4) * bands + (token >> 5)) * kSavedBlock + ((channel >> 2) & 3) * 128 + (token & 31) * 4 +
+           (channel & 3);
+}
+
+// Calls of up to this many tokens keep the hidden row h (and dg, du) as two 16-bit parts, high and low,
+// and run both through the next product: rounding it to one part adds as much error as rounding the
+// result does, and with few tokens the few roundings do not average out.  The products there cost
+// their weights' bytes, so the second part is free.
+constexpr int kPartTokens = 32;
+template <int ACT>
+__device__ __forceinline__ float low_part(float v) {
+    const float rest = v - round_act<ACT>(v);
+    return fabsf(rest) < INFINITY ? rest : 0.f;      // an overflowed or NaN high part says it all
+}
+
 // What a GEMM's epilogue does with its sums.
 enum Epilogue {
     EPI_STORE = 0,   // out = sum, in the activation type
@@ -98,11 +121,12 @@ struct EpiParams {
     int out_dtype;
     int vec;                 // out rows take 16-byte stores
     int act;                 // vy_activation
-    // g and u as [2][inter][ld_saved]: a column of the tile is contiguous over the tokens, so a
-    // warp (one token per lane) moves it in one 128-byte line both ways
-    float* saved;
-    int64_t ld_saved, saved_u;      // token stride, offset of u
-    uint16_t *dg, *du, *h;          // EPI_DGATE, rows `ldo` apart
+    float* saved;            // g and u, see saved_at
+    int64_t saved_bands;     // groups of 32 tokens in it
+    uint16_t *dg, *du, *h;   // EPI_DGATE, rows `ldo` apart
+    // When not 0, a hidden row (h, dg, du) is kept as a sum of two 16-bit parts, the second this many
+    // elements behind the first: see kPartTokens.
+    int64_t part;
     const float* row_scale;
     const float* col_scale[2];
     const void* bias;

@@ -12,12 +12,12 @@
 namespace vy {
 namespace {
 
-// Tokens of a column of `saved`: whole 128-byte lines of fp32.
-int64_t saved_ld(int64_t tokens) { return (tokens + 31) / 32 * 32; }
-
 size_t align256(size_t v) { return (v + 255) & ~size_t(255); }
 
+// Elements of one part of a hidden row's matrix, and bytes of the matrix.
 int64_t h_elems(const vy_ffn_call* c) { return c->n_tokens * int64_t(c->inter); }
+int h_parts(const vy_ffn_call* c) { return c->n_tokens <= kPartTokens ? 2 : 1; }
+size_t h_bytes(const vy_ffn_call* c) { return align256(size_t(h_elems(c)) * 2 * h_parts(c)); }
 
 int check_ffn(const vy_ffn_call* c, bool backward) {
     if (!c) return fail(VY_ERR_INVALID, "null call");
@@ -79,16 +79,17 @@ int forward(const vy_ffn_call* c, const DeviceInfo* dev, cudaStream_t s) {
     e.ldo = I;
     e.act = c->activation;
     e.saved = c->saved;
-    e.ld_saved = saved_ld(T);
-    e.saved_u = saved_ld(T) * I;
+    e.saved_bands = saved_bands(T);
+    e.part = h_parts(c) == 2 ? h_elems(c) : 0;
     EpiParams d{};
     d.out = c->out;
     d.ldo = c->out_row_stride;
     if (T <= kStreamMaxTokens) {
-        VY_TRY((stream_launch<EPI_GATE, ACT>(c->w_gate, c->w_up, c->x, c->x_row_stride, static_cast<int>(T), c->inter,
+        VY_TRY((stream_launch<EPI_GATE, ACT>(c->w_gate, c->w_up, c->x, c->x_row_stride, static_cast<int>(T), 1, c->inter,
                                              c->hidden, false, e, c->flags, dev, s)));
-        return stream_launch<EPI_STORE, ACT>(c->w_down, nullptr, h, I, static_cast<int>(T), c->hidden, c->inter, true, d,
-                                             c->flags, dev, s);
+        const int parts = h_parts(c);
+        return stream_launch<EPI_STORE, ACT>(c->w_down, nullptr, h, I, static_cast<int>(T) * parts, parts, c->hidden,
+                                             c->inter, true, d, c->flags, dev, s);
     }
     const int pairs = dev->sm_count / 2;
     {
@@ -117,7 +118,9 @@ int backward(const vy_ffn_call* c, const DeviceInfo* dev, cudaStream_t s) {
     const int64_t T = c->n_tokens, H = c->hidden, I = c->inter;
     const int pairs = dev->sm_count / 2;
     char* base = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(c->workspace) + 255) & ~uintptr_t(255));
-    const size_t each = align256(size_t(h_elems(c)) * 2);
+    const size_t each = h_bytes(c);
+    const int parts = h_parts(c);
+    const int64_t part = parts == 2 ? h_elems(c) : 0;
     uint16_t* dg = reinterpret_cast<uint16_t*>(base);
     uint16_t* du = reinterpret_cast<uint16_t*>(base + each);
     uint16_t* h = reinterpret_cast<uint16_t*>(base + 2 * each);
@@ -130,8 +133,8 @@ int backward(const vy_ffn_call* c, const DeviceInfo* dev, cudaStream_t s) {
         VY_TRY(tile_operand(&q.b[0], ACT, c->w_down, I, H, I, true, 0));
         q.epi.act = c->activation;
         q.epi.saved = c->saved;
-        q.epi.ld_saved = saved_ld(T);
-        q.epi.saved_u = saved_ld(T) * I;
+        q.epi.saved_bands = saved_bands(T);
+        q.epi.part = part;
         q.epi.ldo = I;
         q.epi.dg = dg;
         q.epi.du = du;
@@ -141,11 +144,14 @@ int backward(const vy_ffn_call* c, const DeviceInfo* dev, cudaStream_t s) {
     }
     TileParams p{};
     p.flags = c->flags;
-    if (c->d_x) {      // two K segments: dg Wg + du Wu
-        TileProblem& q = tile_add(&p, T, H, k_blocks(I), k_blocks(I));
+    if (c->d_x) {      // K segments: the parts of dg with Wg, those of du with Wu
+        TileProblem& q = tile_add(&p, T, H, k_blocks(I), 2 * parts);
         q.b_mn = 1;
-        VY_TRY(tile_operand(&q.a[0], ACT, dg, T, I, I, false, 128));
-        VY_TRY(tile_operand(&q.a[1], ACT, du, T, I, I, false, 128));
+        for (int i = 0; i < 2 * parts; ++i) {
+            q.a_of[i] = static_cast<uint8_t>(i);
+            q.b_of[i] = static_cast<uint8_t>(i / parts);
+            VY_TRY(tile_operand(&q.a[i], ACT, (i / parts ? du : dg) + i % parts * part, T, I, I, false, 128));
+        }
         VY_TRY(tile_operand(&q.b[0], ACT, c->w_gate, H, I, H, true, 0));
         VY_TRY(tile_operand(&q.b[1], ACT, c->w_up, H, I, H, true, 0));
         epi_store(&q, c->d_x, c->d_x_row_stride);
@@ -154,16 +160,24 @@ int backward(const vy_ffn_call* c, const DeviceInfo* dev, cudaStream_t s) {
         void* out;
         const void *a, *b;
         int64_t m, n, lda, ldb;
+        bool b_parts;      // the hidden row's matrix is b (else a)
     };
-    const Grad grads[3] = {{c->d_w_gate, dg, c->x, I, H, I, c->x_row_stride},
-                           {c->d_w_up, du, c->x, I, H, I, c->x_row_stride},
-                           {c->d_w_down, c->d_out, h, H, I, c->d_out_row_stride, I}};
+    const Grad grads[3] = {{c->d_w_gate, dg, c->x, I, H, I, c->x_row_stride, false},
+                           {c->d_w_up, du, c->x, I, H, I, c->x_row_stride, false},
+                           {c->d_w_down, c->d_out, h, H, I, c->d_out_row_stride, I, true}};
     for (const Grad& g : grads) {
         if (!g.out) continue;
-        TileProblem& q = tile_add(&p, g.m, g.n, k_blocks(T));
+        TileProblem& q = tile_add(&p, g.m, g.n, k_blocks(T), parts);
         q.a_mn = q.b_mn = 1;
-        VY_TRY(tile_operand(&q.a[0], ACT, g.a, g.m, T, g.lda, true, 0));
-        VY_TRY(tile_operand(&q.b[0], ACT, g.b, g.n, T, g.ldb, true, 0));
+        for (int i = 0; i < parts; ++i) {
+            uint8_t* of = g.b_parts ? q.b_of : q.a_of;
+            of[i] = static_cast<uint8_t>(i);
+            const int64_t at = i * part;
+            if (i == 0 || !g.b_parts)
+                VY_TRY(tile_operand(&q.a[i], ACT, static_cast<const uint16_t*>(g.a) + at, g.m, T, g.lda, true, 0));
+            if (i == 0 || g.b_parts)
+                VY_TRY(tile_operand(&q.b[i], ACT, static_cast<const uint16_t*>(g.b) + at, g.n, T, g.ldb, true, 0));
+        }
         epi_store(&q, g.out, g.n);
     }
     if (p.n_problems == 0) return VY_OK;
@@ -177,13 +191,12 @@ int backward(const vy_ffn_call* c, const DeviceInfo* dev, cudaStream_t s) {
 using namespace vy;
 
 extern "C" int64_t vy_gated_ffn_saved_floats(int64_t n_tokens, int32_t inter) {
-    return n_tokens < 0 || inter < 0 ? 0 : 2 * saved_ld(n_tokens) * int64_t(inter);
+    return n_tokens < 0 || inter < 0 ? 0 : saved_bands(n_tokens) * ((int64_t(inter) + 15) / 16) * kSavedBlock;
 }
 
 extern "C" size_t vy_gated_ffn_workspace_size(const vy_ffn_call* c, int32_t backward) {
     if (!c || c->n_tokens <= 0 || c->inter <= 0) return 0;
-    const size_t each = align256(size_t(h_elems(c)) * 2);
-    return (backward ? 3 * each : each) + 256;
+    return (backward ? 3 : 1) * h_bytes(c) + 256;
 }
 
 extern "C" int vy_gated_ffn_forward(const vy_ffn_call* c, void* stream) {

@@ -286,7 +286,7 @@ int launch_product(const Product& a, bool first, const DeviceInfo* dev, cudaStre
     e.bias_dtype = a.bias_dtype;
     constexpr int EPI = GATE ? EPI_I8GATE : EPI_I8;
     if (a.tokens <= kStreamMaxTokens)
-        return stream_launch<EPI, VY_BF16>(a.w[0], a.w[1], a.codes, a.codes_ld, static_cast<int>(a.tokens), a.n, a.k,
+        return stream_launch<EPI, VY_BF16>(a.w[0], a.w[1], a.codes, a.codes_ld, static_cast<int>(a.tokens), 1, a.n, a.k,
                                            !first, e, a.flags, dev, s);
     const int pairs = dev->sm_count / 2;
     TileParams p{};

@@ -26,11 +26,12 @@ constexpr int kSmemMost = 226 * 1024, kSmemHalf = 112 * 1024;   // dynamic bytes
 
 struct StreamParams {
     CUtensorMap w[2], x;
-    int tokens, n, nk;      // nk: K blocks of 128 bytes
+    int tokens, n, nk;      // rows of x; nk: K blocks of 128 bytes
     int cols;               // MMA N: tokens rounded up to 16
     int stages, tmem_cols;
     int sums_at;            // offset of the received sums in dynamic shared memory
     int early;              // weights may be loaded before the previous kernel has finished
+    int parts;              // 2: x holds high parts, then low parts; an output is the sum of both
     EpiParams epi;
     int32_t* flags;
 };
@@ -69,11 +70,13 @@ __device__ __forceinline__ void stream_put(const StreamParams& p, int row, int t
     const int64_t at = int64_t(t) * e.ldo + row;
     if constexpr (EPI == EPI_GATE) {
         const float g = __uint_as_float(s0), u = __uint_as_float(s1);
-        reinterpret_cast<uint16_t*>(e.out)[at] = static_cast<uint16_t>(act_bits<ACT>(gate_act(g, e.act) * u));
+        const float h = gate_act(g, e.act) * u;
+        reinterpret_cast<uint16_t*>(e.out)[at] = static_cast<uint16_t>(act_bits<ACT>(h));
+        if (e.part) reinterpret_cast<uint16_t*>(e.out)[at + e.part] = static_cast<uint16_t>(act_bits<ACT>(low_part<ACT>(h)));
         if (e.saved) {
-            float* s = e.saved + int64_t(row) * e.ld_saved + t;
+            float* s = e.saved + saved_at(e.saved_bands, t, row);
             s[0] = g;
-            s[e.saved_u] = u;
+            s[kSavedBlock / 2] = u;
         }
     } else if constexpr (EPI == EPI_STORE) {
         reinterpret_cast<uint16_t*>(e.out)[at] = static_cast<uint16_t>(act_bits<ACT>(__uint_as_float(s0)));
@@ -199,8 +202,10 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(const __grid_con
     const int rows = kStreamRows / splits;      // 1, 2, 4 or 8 shares
     uint32_t* sums = reinterpret_cast<uint32_t*>(ring + p.sums_at);
     // the weight row of this thread: its lane's when it reads all sums itself, else of my slice
-    // (kStreamThreads is a multiple of a slice's rows, so every output it adds has the same one)
-    const int my_row = row0 + (splits == 1 ? tid & (kStreamRows - 1) : int(rank) * rows + tid % rows);
+    // (whole multiples of a slice's rows take part, so every output a thread adds has the same row)
+    const int step = kStreamThreads / rows * rows;
+    const bool direct = splits == 1 && p.parts == 1;      // nothing to join: outputs straight from TMEM
+    const int my_row = row0 + (direct ? tid & (kStreamRows - 1) : int(rank) * rows + tid % rows);
     const ColumnScale cs = column_scale<EPI>(p, my_row);
     if constexpr (epi_is_i8(EPI)) {
         for (int t = tid; t < p.tokens; t += kStreamThreads) S.token_scale[t] = p.epi.row_scale[t];
@@ -221,7 +226,7 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(const __grid_con
                 for (int m = 0; m < NW; ++m) tmem_ld16(tmem + lanes + m * p.cols + c, v[m]);
 #pragma unroll
                 for (int m = 0; m < NW; ++m) tmem_wait16(v[m]);
-                if (splits == 1) {
+                if (direct) {
                     if (row0 + row < p.n) {
 #pragma unroll
                         for (int j = 0; j < 16; ++j)
@@ -240,10 +245,10 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(const __grid_con
         tc_fence_before();
     }
     __syncwarp();
-    if (splits > 1) {
+    if (!direct) {
         cluster_sync();
         const int share = NW * p.tokens * rows;
-        for (int q = tid; q < rows * p.tokens; q += kStreamThreads) {
+        for (int q = tid < step ? tid : rows * p.tokens; q < rows * (p.tokens / p.parts); q += step) {
             const int t = q / rows;
             if (my_row >= p.n) continue;
             uint32_t sum[NW];
@@ -254,6 +259,12 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(const __grid_con
                 for (uint32_t r = 1; r < splits; ++r) {
                     const uint32_t v = at[r * share];
                     acc = I8 ? acc + v : __float_as_uint(__fadd_rn(__uint_as_float(acc), __uint_as_float(v)));
+                }
+                if (EPI == EPI_STORE && p.parts == 2) {
+                    at += p.tokens / 2 * rows;
+                    float low = __uint_as_float(at[0]);
+                    for (uint32_t r = 1; r < splits; ++r) low = __fadd_rn(low, __uint_as_float(at[r * share]));
+                    acc = __float_as_uint(__fadd_rn(__uint_as_float(acc), low));
                 }
                 sum[m] = acc;
             }
@@ -278,12 +289,12 @@ struct StreamPlan {
 // memory.  Up to 32 tokens two stages a CTA are enough for that (16 x 7168 x 2048, bf16: 27.5 us
 // against 32.3 with one deep ring an SM); with more, the token tiles crowd the ring, and one CTA with
 // five stages is faster than two with two (64 x 4096 x 14336: 82 us against 99).
-inline StreamPlan stream_plan(int nw, int tokens, int n, int nk, int sm_count) {
+inline StreamPlan stream_plan(int nw, int tokens, int parts, int n, int nk, int sm_count) {
     const int units = (n + kStreamRows - 1) / kStreamRows;
     StreamPlan p{};
     p.stage = nw * 16384 + (tokens + 15) / 16 * 16 * 128;
     for (p.splits = 8; p.splits >= 1; p.splits /= 2) {
-        p.sums = p.splits > 1 ? (nw * tokens * kStreamRows * 4 + 1023) / 1024 * 1024 : 0;
+        p.sums = p.splits > 1 || parts > 1 ? (nw * tokens * kStreamRows * 4 + 1023) / 1024 * 1024 : 0;
         const int half = (kSmemHalf - 1024 - p.sums) / p.stage, whole = (kSmemMost - 1024 - p.sums) / p.stage;
         const bool two = half >= (tokens <= 32 ? 2 : 3);
         p.stages = two ? half : whole;
@@ -294,10 +305,10 @@ inline StreamPlan stream_plan(int nw, int tokens, int n, int nk, int sm_count) {
     return p;
 }
 
-// w: NW weight matrices [n, k], contiguous; x: [tokens, k].
+// w: NW weight matrices [n, k], contiguous; x: [tokens, k] (parts == 2: high parts, then low parts).
 template <int EPI, int ACT>
-int stream_launch(const void* w0, const void* w1, const void* x, int64_t x_ld, int tokens, int n, int k, bool early,
-                  const EpiParams& epi, int32_t* flags, const DeviceInfo* dev, cudaStream_t s) {
+int stream_launch(const void* w0, const void* w1, const void* x, int64_t x_ld, int tokens, int parts, int n, int k,
+                  bool early, const EpiParams& epi, int32_t* flags, const DeviceInfo* dev, cudaStream_t s) {
     constexpr bool I8 = epi_is_i8(EPI);
     constexpr int NW = epi_is_gate(EPI) ? 2 : 1;
     constexpr int block = I8 ? 128 : 64;
@@ -308,6 +319,7 @@ int stream_launch(const void* w0, const void* w1, const void* x, int64_t x_ld, i
     p.nk = (k + block - 1) / block;
     p.cols = (tokens + 15) / 16 * 16;
     p.early = early;
+    p.parts = parts;
     p.epi = epi;
     p.flags = flags;
     p.tmem_cols = 32;
@@ -316,7 +328,7 @@ int stream_launch(const void* w0, const void* w1, const void* x, int64_t x_ld, i
     if ((st = make_map_2d(&p.w[0], dtype, w0, n, k, k, block, kStreamRows)) != VY_OK) return st;
     if (NW == 2 && (st = make_map_2d(&p.w[1], dtype, w1, n, k, k, block, kStreamRows)) != VY_OK) return st;
     if ((st = make_map_2d(&p.x, dtype, x, tokens, k, x_ld, block, p.cols)) != VY_OK) return st;
-    const StreamPlan plan = stream_plan(NW, tokens, n, p.nk, dev->sm_count);
+    const StreamPlan plan = stream_plan(NW, tokens, parts, n, p.nk, dev->sm_count);
     if (plan.stages < 2) return fail(VY_ERR_UNSUPPORTED, "dense stream: %d tokens", tokens);
     p.stages = plan.stages;
     p.sums_at = plan.stages * plan.stage;

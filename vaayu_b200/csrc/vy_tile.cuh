@@ -7,7 +7,7 @@
 // elements or 128 int8) through a ring of TMA-filled stages; accumulators are double-buffered in
 // TMEM, so the epilogue of one tile runs under the MMAs of the next.  Both operands may be K-major
 // or MN-major (the weight gradients contract over tokens, the activations' slow axis), and K may
-// come in two segments from two tensor pairs (dx = dg Wg + du Wu).  One launch takes up to four
+// come in segments from several tensors (dx = dg Wg + du Wu).  One launch takes up to four
 // GEMMs, whose tiles fill the machine together.
 //
 // Few tiles.  Pairs are persistent, one for two SMs, and take tiles in turn.  A launch with at most half
@@ -32,9 +32,10 @@ constexpr int kHalfBytes = 128 * 128;          // one operand's share of a stage
 constexpr uint32_t kTileTmemCols = 512;
 
 struct TileProblem {
-    CUtensorMap a[2], b[2];      // per K segment (per CTA for a gated product: gate, up)
+    CUtensorMap a[4], b[2];      // operands of the K segments (a gated product: b is gate, up)
     int m, n;                    // rows, output columns
-    int nk[2];                   // K blocks of each segment
+    int nk[4];                   // K blocks of each segment
+    uint8_t a_of[4], b_of[4];    // each segment's operands
     int a_mn, b_mn;              // 1: that operand is MN-major (memory [K, M] / [K, N])
     int bn;                      // tile columns, 256 or 128
     int m_tiles, n_tiles, first; // tiles [first, first + m_tiles * n_tiles)
@@ -45,6 +46,7 @@ struct TileParams {
     TileProblem prob[kTileProblems];
     int n_problems, n_tiles;
     int splits;              // pairs of a cluster, which share a tile's K: 1, 2 or 4
+    int n_long, extra;       // see TileTurn
     int32_t* flags;
 };
 
@@ -58,6 +60,23 @@ struct __align__(1024) TileSmem {
     int abort_flag;
 };
 
+__host__ __device__ __forceinline__ int k_total(const TileProblem& q) { return q.nk[0] + q.nk[1] + q.nk[2] + q.nk[3]; }
+
+// A pair's tiles: first, first + pairs, ...  When the first problem's tiles are long ones (dx: its K is
+// both halves' channels), they come first, n_long of them, and the pairs that get one fewer of them
+// take `extra` of the others each before all go on in turn.
+__device__ __forceinline__ int tile_of_turn(const TileParams& p, int turn, int pair, int pairs) {
+    if (p.extra == 0) return pair + turn * pairs;
+    const int odd = p.n_long % pairs, rounds = p.n_long / pairs + (pair < odd);      // my long tiles
+    if (turn < rounds) return pair + turn * pairs;
+    turn -= rounds;
+    const int light = pairs - odd;
+    if (pair >= odd) {
+        if (turn < p.extra) return p.n_long + turn * light + pair - odd;
+        turn -= p.extra;
+    }
+    return p.n_long + p.extra * light + turn * pairs + pair;
+}
 struct TileAt {
     int prob, m, n;   // tile's problem, row tile, column tile
 };
@@ -169,13 +188,13 @@ __device__ __forceinline__ void tile_epilogue(const TileProblem& q, int row, int
 #pragma unroll
                 for (int j = 0; j < 16; ++j) h[j] = gate_act(__uint_as_float(g[j]), e.act) * __uint_as_float(u[j]);
                 if (e.saved) {
-                    float* s = e.saved + int64_t(col) * e.ld_saved + row;
+                    float4* s = reinterpret_cast<float4*>(e.saved + saved_at(e.saved_bands, row, col));
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) {
-                        if (j < valid) {
-                            s[j * e.ld_saved] = __uint_as_float(g[j]);
-                            s[e.saved_u + j * e.ld_saved] = __uint_as_float(u[j]);
-                        }
+                    for (int j = 0; j < 4; ++j) {
+                        s[j * 32] = make_float4(__uint_as_float(g[4 * j]), __uint_as_float(g[4 * j + 1]),
+                                                __uint_as_float(g[4 * j + 2]), __uint_as_float(g[4 * j + 3]));
+                        s[128 + j * 32] = make_float4(__uint_as_float(u[4 * j]), __uint_as_float(u[4 * j + 1]),
+                                                      __uint_as_float(u[4 * j + 2]), __uint_as_float(u[4 * j + 3]));
                     }
                 }
                 store16<ACT>(reinterpret_cast<uint16_t*>(e.out) + int64_t(row) * e.ldo + col, h, valid);
@@ -209,15 +228,16 @@ __device__ __forceinline__ void tile_epilogue(const TileProblem& q, int row, int
 // columns ahead, the first one before the tile's sums are awaited: their latency is paid under the
 // MMAs and the previous chunk's arithmetic.
 struct GateChunk {
-    float g[16], u[16];
+    float4 g[4], u[4];
 };
 __device__ __forceinline__ void load_gate(GateChunk& k, const EpiParams& e, int row, int col, bool live, int n) {
-    const float* s = e.saved + int64_t(col) * e.ld_saved + row;
+    // blocks are whole: columns behind n are padding of the buffer
+    const bool in = live && col < n;
+    const float4* s = reinterpret_cast<const float4*>(e.saved + (in ? saved_at(e.saved_bands, row, col) : 0));
 #pragma unroll
-    for (int j = 0; j < 16; ++j) {
-        const bool in = live && col + j < n;
-        k.g[j] = in ? s[j * e.ld_saved] : 0.f;
-        k.u[j] = in ? s[e.saved_u + j * e.ld_saved] : 0.f;
+    for (int j = 0; j < 4; ++j) {
+        k.g[j] = s[j * 32];
+        k.u[j] = s[128 + j * 32];
     }
 }
 template <int ACT>
@@ -236,16 +256,30 @@ __device__ __forceinline__ void dgate_epilogue(const TileProblem& q, GateChunk& 
         float dg[16], du[16], h[16];
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
+            const float4 g4 = k.g[j / 4], u4 = k.u[j / 4];
+            const float g = j % 4 == 0 ? g4.x : j % 4 == 1 ? g4.y : j % 4 == 2 ? g4.z : g4.w;
+            const float u = j % 4 == 0 ? u4.x : j % 4 == 1 ? u4.y : j % 4 == 2 ? u4.z : u4.w;
             const float dh = __uint_as_float(r[j]);
-            const float2 a = gate_act_grad(k.g[j], e.act);
-            dg[j] = dh * k.u[j] * a.y;
+            const float2 a = gate_act_grad(g, e.act);
+            dg[j] = dh * u * a.y;
             du[j] = dh * a.x;
-            h[j] = a.x * k.u[j];
+            h[j] = a.x * u;
         }
         const int64_t at = int64_t(row) * e.ldo + col;
         store16<ACT>(e.dg + at, dg, valid);
         store16<ACT>(e.du + at, du, valid);
         store16<ACT>(e.h + at, h, valid);
+        if (e.part) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+                dg[j] = low_part<ACT>(dg[j]);
+                du[j] = low_part<ACT>(du[j]);
+                h[j] = low_part<ACT>(h[j]);
+            }
+            store16<ACT>(e.dg + at + e.part, dg, valid);
+            store16<ACT>(e.du + at + e.part, du, valid);
+            store16<ACT>(e.h + at + e.part, h, valid);
+        }
     }
 }
 
@@ -285,18 +319,18 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_kernel(const __grid_cons
     if (warp == 0) {
         uint32_t it = 0, stage = 0, phase = 1;      // phase: parity the ring's next pass waits for
         bool go = true;
-        for (int tile = cluster; go && tile < p.n_tiles; tile += n_clusters) {
+        for (int turn = 0, tile; go && (tile = tile_of_turn(p, turn, cluster, n_clusters)) < p.n_tiles; ++turn) {
             const TileAt t = tile_at(p, tile);
             const TileProblem& q = p.prob[t.prob];
             const int m0 = t.m * 256 + int(rank) * 128;
             // a gated product's pair holds the same columns of gate (first CTA) and up
             const int n0 = epi_is_gate(EPI) ? t.n * (q.bn / 2) : t.n * q.bn + int(rank) * (q.bn / 2);
             const uint32_t bytes = 2u * (kHalfBytes + uint32_t(q.bn) * 64u);
-            const int nk = q.nk[0] + q.nk[1], k_first = nk * share / splits, k_last = nk * (share + 1) / splits;
-            for (int seg = 0; go && seg < 2; ++seg) {
-                const CUtensorMap* ma = &q.a[epi_is_gate(EPI) ? 0 : seg];
-                const CUtensorMap* mb = &q.b[epi_is_gate(EPI) ? rank : seg];
-                const int before = seg ? q.nk[0] : 0, last = min(q.nk[seg], k_last - before);
+            const int nk = k_total(q), k_first = nk * share / splits, k_last = nk * (share + 1) / splits;
+            for (int seg = 0, before = 0; go && seg < 4; before += q.nk[seg++]) {
+                const CUtensorMap* ma = &q.a[q.a_of[seg]];
+                const CUtensorMap* mb = &q.b[epi_is_gate(EPI) ? rank : q.b_of[seg]];
+                const int last = min(q.nk[seg], k_last - before);
                 for (int kb = max(0, k_first - before); kb < last; ++kb, ++it) {
                     if (!mbar_wait_warp(&S.empty[stage], phase, abort_flag, p.flags)) {
                         go = false;
@@ -336,7 +370,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_kernel(const __grid_cons
         if (rank == 0) {
             uint32_t n = 0, stage = 0, phase = 0;
             bool go = true;
-            for (int tile = cluster; go && tile < p.n_tiles; tile += n_clusters, ++n) {
+            for (int tile; go && (tile = tile_of_turn(p, n, cluster, n_clusters)) < p.n_tiles; ++n) {
                 const TileProblem& q = p.prob[tile_at(p, tile).prob];
                 const uint32_t idesc = umma_idesc(I8, ACT == VY_BF16, q.a_mn, q.b_mn, 256, q.bn);
                 // one MMA's K (32 bytes): along the swizzled row, or 16 rows of 128 bytes
@@ -344,7 +378,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_kernel(const __grid_cons
                 const uint64_t a_desc = umma_desc(smem_u32(S.a[0]), q.a_mn ? 8192 : 16, 1024);
                 const uint64_t b_desc = umma_desc(smem_u32(S.b[0]), q.b_mn ? 8192 : 16, 1024);
                 const uint32_t buf = n & 1, d = tmem + buf * 256;
-                const int nk = q.nk[0] + q.nk[1], blocks = nk * (share + 1) / splits - nk * share / splits;
+                const int nk = k_total(q), blocks = nk * (share + 1) / splits - nk * share / splits;
                 if (!mbar_wait_warp(&S.acc_empty[buf], ((n >> 1) & 1) ^ 1, abort_flag, p.flags)) break;
                 tc_fence_after();
                 for (int kb = 0; kb < blocks; ++kb) {
@@ -369,7 +403,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_kernel(const __grid_cons
     } else if (warp >= 4 && splits == 1) {
         const int quarter = warp & 3, half = (warp - 4) >> 2;
         uint32_t n = 0;
-        for (int tile = cluster; tile < p.n_tiles; tile += n_clusters, ++n) {
+        for (int tile; (tile = tile_of_turn(p, n, cluster, n_clusters)) < p.n_tiles; ++n) {
             const TileAt t = tile_at(p, tile);
             const uint32_t buf = n & 1;
             const TileProblem& q = p.prob[t.prob];
@@ -451,7 +485,7 @@ inline void tile_layout(TileParams* p, bool gate, int pairs) {
     for (int i = 0; i < p->n_problems; ++i) {
         const TileProblem& q = p->prob[i];
         const int n = gate ? 2 * q.n : q.n;
-        if (q.nk[0] + q.nk[1] < least) least = q.nk[0] + q.nk[1];
+        if (k_total(q) < least) least = k_total(q);
         wide += (q.m + 255) / 256 * ((n + 255) / 256);
     }
     p->splits = 1;
@@ -468,15 +502,21 @@ inline void tile_layout(TileParams* p, bool gate, int pairs) {
         q.first = p->n_tiles;
         p->n_tiles += q.m_tiles * q.n_tiles;
     }
+    p->n_long = p->extra = 0;
+    const TileProblem& q = p->prob[0];
+    if (p->n_problems > 1 && k_total(q) >= 2 * least && p->n_tiles > pairs) {
+        const int n = q.m_tiles * q.n_tiles, odd = n % pairs;
+        const int extra = (k_total(q) + least / 2) / least;
+        if (odd && extra * (pairs - odd) <= p->n_tiles - n) p->n_long = n, p->extra = extra;
+    }
 }
 
-// Adds a problem to a launch: m x n, K blocks of its two segments.
-inline TileProblem& tile_add(TileParams* p, int64_t m, int64_t n, int nk0, int nk1 = 0) {
+// Adds a problem to a launch: m x n, `segments` K segments of nk blocks.
+inline TileProblem& tile_add(TileParams* p, int64_t m, int64_t n, int nk, int segments = 1) {
     TileProblem& q = p->prob[p->n_problems++];
     q.m = static_cast<int>(m);
     q.n = static_cast<int>(n);
-    q.nk[0] = nk0;
-    q.nk[1] = nk1;
+    for (int i = 0; i < segments; ++i) q.nk[i] = nk;
     return q;
 }
 
