@@ -50,13 +50,13 @@ def _device(what: str, first: torch.Tensor, *others) -> int:
     return index
 
 
-def _enqueue(fn, call, index: int, what: str) -> None:
+def _enqueue(fn, what: str, index: int, *args) -> None:
     """One C call on the device's current stream, with that device current."""
     if index == _current_device():
-        status = fn(call, _raw_stream(index))
+        status = fn(*args, _raw_stream(index))
     else:
         with torch.cuda.device(index):
-            status = fn(call, _raw_stream(index))
+            status = fn(*args, _raw_stream(index))
     if status:
         _lib.check(status, what)
 
@@ -105,29 +105,42 @@ def _aligned(w: torch.Tensor) -> torch.Tensor:
 def _check_ffn(x, w_gate, w_up, w_down, what: str) -> tuple:
     """(hidden, inter) of a block whose operands fit together."""
     shape = w_gate.shape
-    if x.dim() < 1 or len(shape) != 2 or w_up.shape != shape or w_down.shape != shape[::-1]:
-        raise ValueError(f"{what}: weights {tuple(w_gate.shape)}, {tuple(w_up.shape)}, {tuple(w_down.shape)} "
-                         "are not [inter, hidden], [inter, hidden], [hidden, inter]")
-    if x.shape[-1] != shape[1]:
-        raise ValueError(f"{what}: x {tuple(x.shape)} does not fit hidden {shape[1]}")
-    return shape[1], shape[0]
+    if len(shape) == 2 and w_up.shape == shape:
+        inter, hidden = shape
+        down = w_down.shape
+        if len(down) == 2 and down[0] == hidden and down[1] == inter:
+            if x.dim() < 1 or x.shape[-1] != hidden:
+                raise ValueError(f"{what}: x {tuple(x.shape)} does not fit hidden {hidden}")
+            return hidden, inter
+    raise ValueError(f"{what}: weights {tuple(shape)}, {tuple(w_up.shape)}, {tuple(w_down.shape)} "
+                     "are not [inter, hidden], [inter, hidden], [hidden, inter]")
 
 
-def _output(out, like, shape, dtype, what: str) -> tuple:
-    """(`out` checked or a new tensor on like's device, it as [tokens, width], its row stride)."""
-    if out is None:
-        out = torch.empty(shape, dtype=dtype, device=like.device)
-    elif out.shape != shape or out.dtype != dtype:
+def _like(x: torch.Tensor) -> torch.Tensor:
+    """A new contiguous tensor of x's shape and type.  (empty_like of a contiguous tensor, and new_empty
+    with its sizes spelt out, take half the host time of torch.empty with a shape.)"""
+    return torch.empty_like(x) if x.is_contiguous() else x.new_empty(x.shape)
+
+
+def _given(out, shape, dtype, what: str) -> tuple:
+    """(the caller's out as [tokens, width], its row stride)."""
+    if out.shape != shape or out.dtype != dtype:
         raise ValueError(f"{what}: out {tuple(out.shape)} {out.dtype}, expected {tuple(shape)} {dtype}")
-    elif not out.is_contiguous():
+    if not out.is_contiguous():
         if out.dim() != 2 or out.stride(1) != 1 or out.stride(0) < out.shape[1]:
             raise ValueError(f"{what}: out must be contiguous, or a 2-D view with unit column stride")
-        return out, out, out.stride(0)
-    return out, (out if out.dim() == 2 else out.view(-1, shape[-1])), shape[-1]
+        return out, out.stride(0)
+    return out.view(-1, shape[-1]), shape[-1]
 
 
-def _workspace(size: int, like: torch.Tensor) -> "torch.Tensor | None":
-    return torch.empty(size, dtype=_INT8, device=like.device) if size else None
+_SIZES: dict = {}      # an entry point's sizes -> its workspace bytes
+
+
+def _remember(key: tuple, size: int) -> int:
+    if len(_SIZES) >= 4096:
+        _SIZES.clear()
+    _SIZES[key] = size
+    return size
 
 
 def _flags(like: torch.Tensor, check: bool) -> "torch.Tensor | None":
@@ -145,17 +158,13 @@ def _raise_on(flags: torch.Tensor, what: str) -> None:
 
 # ── gated feed-forward, 16-bit ───────────────────────────────────────────────────────────────
 
-_FFN_SIZES: dict = {}      # (tokens, hidden, inter, backward) -> workspace bytes
-
 
 def _ffn_workspace(tokens: int, hidden: int, inter: int, backward: int) -> int:
     key = (tokens, hidden, inter, backward)
-    size = _FFN_SIZES.get(key)
+    size = _SIZES.get(key)
     if size is None:
         call = _FFN.pack(0, 0, tokens, hidden, inter, *(0,) * 18)
-        if len(_FFN_SIZES) >= 4096:
-            _FFN_SIZES.clear()
-        size = _FFN_SIZES[key] = _lib.lib().vy_gated_ffn_workspace_size(call, backward)
+        size = _remember(key, _lib.lib().vy_gated_ffn_workspace_size(call, backward))
     return size
 
 
@@ -165,16 +174,15 @@ def _ffn_forward(x, w_gate, w_up, w_down, hidden: int, inter: int, act: int, fla
     rows, x_stride = _rows(x, 8)
     wg, wu, wd = _aligned(w_gate), _aligned(w_up), _aligned(w_down)
     tokens = rows.shape[0]
+    lib = _lib.lib()
     size = _ffn_workspace(tokens, hidden, inter, 0)
-    ws = _workspace(size, rows)
-    saved = None
-    if save:
-        saved = torch.empty(_lib.lib().vy_gated_ffn_saved_floats(tokens, inter), dtype=_F32, device=rows.device)
+    ws = rows.new_empty((size + 1) // 2)
+    saved = rows.new_empty(lib.vy_gated_ffn_saved_floats(tokens, inter), dtype=_F32) if save else None
     flags = _flags(rows, check)
     call = _FFN.pack(_CODE[rows.dtype], act, tokens, hidden, inter, rows.data_ptr(), x_stride, wg.data_ptr(),
-                     wu.data_ptr(), wd.data_ptr(), flat.data_ptr(), out_stride, _ptr(saved), _ptr(ws), size,
+                     wu.data_ptr(), wd.data_ptr(), flat.data_ptr(), out_stride, _ptr(saved), ws.data_ptr(), size,
                      _ptr(flags), 0, 0, 0, 0, 0, 0, 0)
-    _enqueue(_lib.lib().vy_gated_ffn_forward, call, index, "gated_ffn")
+    _enqueue(lib.vy_gated_ffn_forward, "gated_ffn", index, call)
     if check:
         _raise_on(flags, "gated_ffn")
     return saved
@@ -184,7 +192,7 @@ class _GatedFfn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w_gate, w_up, w_down, act, check):
         inter, hidden = w_gate.shape
-        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        out = _like(x)
         saved = _ffn_forward(x, w_gate, w_up, w_down, hidden, inter, act, out, hidden, x.get_device(), True, check)
         ctx.save_for_backward(x, w_gate, w_up, w_down, saved)
         ctx.act, ctx.check = act, check
@@ -198,14 +206,13 @@ class _GatedFfn(torch.autograd.Function):
         wg, wu, wd = _aligned(w_gate), _aligned(w_up), _aligned(w_down)
         tokens, (inter, hidden) = rows.shape[0], wg.shape
         need = ctx.needs_input_grad
-        grads = [torch.empty(t.shape, dtype=t.dtype, device=t.device) if n else None
-                 for t, n in zip((x, w_gate, w_up, w_down), need)]
+        grads = [_like(t) if n else None for t, n in zip((x, w_gate, w_up, w_down), need)]
         size = _ffn_workspace(tokens, hidden, inter, 1)
-        ws, flags = _workspace(size, rows), _flags(rows, ctx.check)
+        ws, flags = rows.new_empty((size + 1) // 2), _flags(rows, ctx.check)
         call = _FFN.pack(_CODE[rows.dtype], ctx.act, tokens, hidden, inter, rows.data_ptr(), x_stride,
-                         wg.data_ptr(), wu.data_ptr(), wd.data_ptr(), 0, 0, saved.data_ptr(), _ptr(ws), size,
+                         wg.data_ptr(), wu.data_ptr(), wd.data_ptr(), 0, 0, saved.data_ptr(), ws.data_ptr(), size,
                          _ptr(flags), dy.data_ptr(), dy_stride, _ptr(grads[0]), hidden, *map(_ptr, grads[1:]))
-        _enqueue(_lib.lib().vy_gated_ffn_backward, call, x.get_device(), "gated_ffn backward")
+        _enqueue(_lib.lib().vy_gated_ffn_backward, "gated_ffn backward", x.get_device(), call)
         if ctx.check:
             _raise_on(flags, "gated_ffn backward")
         return (*grads, None, None)
@@ -236,11 +243,15 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
         if out is not None:
             raise RuntimeError(f"{what}: out= with gradients")
         return _GatedFfn.apply(x, w_gate, w_up, w_down, code, check)
-    y, flat, stride = _output(out, x, x.shape, dtype, what)
-    if out is not None and (flat.data_ptr() & 15 or stride % 8):
-        raise ValueError(f"{what}: out rows must start on 16-byte boundaries")
+    if out is None:
+        out, stride = _like(x), hidden
+        flat = out                      # contiguous: only its address is used
+    else:
+        flat, stride = _given(out, x.shape, dtype, what)
+        if flat.data_ptr() & 15 or stride % 8:
+            raise ValueError(f"{what}: out rows must start on 16-byte boundaries")
     _ffn_forward(x, w_gate, w_up, w_down, hidden, inter, code, flat, stride, index, False, check)
-    return y
+    return out
 
 
 # ── int8 ─────────────────────────────────────────────────────────────────────────────────────
@@ -262,15 +273,10 @@ def quantize_int8(x: torch.Tensor) -> tuple:
     index = _device(what, x)
     rows, stride = _unit_rows(x)
     tokens, width = rows.shape
-    dev = x.device
-    codes = torch.empty(shape, dtype=_INT8, device=dev)
-    scale = torch.empty((tokens, 1) if len(shape) == 2 else (*shape[:-1], 1), dtype=_F32, device=dev)
-
-    def call(_none, stream):
-        return _lib.lib().vy_int8_quantize(rows.data_ptr(), code, stride, tokens, width, codes.data_ptr(),
-                                           scale.data_ptr(), stream)
-
-    _enqueue(call, None, index, what)
+    codes = torch.empty_like(x, dtype=_INT8) if x.is_contiguous() else x.new_empty(shape, dtype=_INT8)
+    scale = x.new_empty(tokens, 1, dtype=_F32) if len(shape) == 2 else x.new_empty((*shape[:-1], 1), dtype=_F32)
+    _enqueue(_lib.lib().vy_int8_quantize, what, index, rows.data_ptr(), code, stride, tokens, width,
+             codes.data_ptr(), scale.data_ptr())
     return codes, scale
 
 
@@ -312,26 +318,26 @@ def int8_linear(codes: torch.Tensor, scale: torch.Tensor, weight: torch.Tensor, 
     (rows, stride), w = _rows(codes, 16), _aligned(weight)
     tokens = rows.shape[0]
     sx, sw = _scales(scale, tokens, what), _scales(weight_scale, n, what)
-    y, flat, out_stride = _output(out, codes, (tokens, n) if len(shape) == 2 else (*shape[:-1], n), dtype, what)
+    if out is None:
+        out = codes.new_empty(tokens, n, dtype=dtype) if len(shape) == 2 else codes.new_empty((*shape[:-1], n), dtype=dtype)
+        flat, out_stride = out, n
+    else:
+        flat, out_stride = _given(out, (*shape[:-1], n), dtype, what)
     flags = _flags(codes, check)
     call = _LINEAR.pack(tokens, k, n, rows.data_ptr(), stride, sx.data_ptr(), w.data_ptr(), sw.data_ptr(),
                         _ptr(bias), bias_code, out_code, flat.data_ptr(), out_stride, 0, 0, _ptr(flags))
-    _enqueue(_lib.lib().vy_int8_linear, call, index, what)
+    _enqueue(_lib.lib().vy_int8_linear, what, index, call)
     if check:
         _raise_on(flags, what)
-    return y
+    return out
 
 
-_INT8_FFN_SIZES: dict = {}      # (tokens, hidden, inter) -> workspace bytes
-
-
-def _int8_ffn_workspace(key: tuple) -> int:
-    size = _INT8_FFN_SIZES.get(key)
+def _int8_ffn_workspace(tokens: int, hidden: int, inter: int) -> int:
+    key = ("int8", tokens, hidden, inter)
+    size = _SIZES.get(key)
     if size is None:
-        if len(_INT8_FFN_SIZES) >= 4096:
-            _INT8_FFN_SIZES.clear()
-        size = _INT8_FFN_SIZES[key] = _lib.lib().vy_int8_gated_ffn_workspace_size(
-            _INT8_FFN.pack(0, 0, *key, *(0,) * 13))
+        call = _INT8_FFN.pack(0, 0, tokens, hidden, inter, *(0,) * 13)
+        size = _remember(key, _lib.lib().vy_int8_gated_ffn_workspace_size(call))
     return size
 
 
@@ -357,14 +363,18 @@ def int8_gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, gate_scale: torch.Tens
     index = _device(what, x, w_gate, gate_scale, w_up, up_scale, w_down, down_scale, out)
     (rows, stride), wg, wu, wd = _unit_rows(x), _aligned(w_gate), _aligned(w_up), _aligned(w_down)
     sg, su, sd = _scales(gate_scale, inter, what), _scales(up_scale, inter, what), _scales(down_scale, hidden, what)
-    y, flat, out_stride = _output(out, x, x.shape, dtype, what)
+    if out is None:
+        out, out_stride = _like(x), hidden
+        flat = out
+    else:
+        flat, out_stride = _given(out, x.shape, dtype, what)
     tokens = rows.shape[0]
-    size = _int8_ffn_workspace((tokens, hidden, inter))
-    ws, flags = _workspace(size, rows), _flags(rows, check)
+    size = _int8_ffn_workspace(tokens, hidden, inter)
+    ws, flags = rows.new_empty((size + 1) // 2), _flags(rows, check)
     call = _INT8_FFN.pack(_CODE[dtype], code, tokens, hidden, inter, rows.data_ptr(), stride, wg.data_ptr(),
                           wu.data_ptr(), wd.data_ptr(), sg.data_ptr(), su.data_ptr(), sd.data_ptr(), flat.data_ptr(),
-                          out_stride, _ptr(ws), size, _ptr(flags))
-    _enqueue(_lib.lib().vy_int8_gated_ffn, call, index, what)
+                          out_stride, ws.data_ptr(), size, _ptr(flags))
+    _enqueue(_lib.lib().vy_int8_gated_ffn, what, index, call)
     if check:
         _raise_on(flags, what)
-    return y
+    return out
