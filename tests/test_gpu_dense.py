@@ -370,7 +370,9 @@ def test_int8_linear_layouts():
 # ── int8_gated_ffn ───────────────────────────────────────────────────────────────────────────
 
 
-@pytest.mark.parametrize("tokens,hidden,inter", [(1, 16, 16), (1, 1024, 512), (2, 144, 48), (16, 7168, 2048), (17, 64, 1040),
+@pytest.mark.parametrize("tokens,hidden,inter", [(1, 16, 16), (1, 1024, 512), (2, 144, 48), (1, 14336, 256), (2, 8192, 144),
+                                                 (3, 4096, 1040), (4, 4112, 272), (9, 1040, 4096), (15, 272, 2064),
+                                                 (16, 1024, 16), (16, 7168, 2048), (17, 64, 1040),
                                                  (33, 528, 272), (64, 256, 128), (129, 272, 80), (257, 1040, 528),
                                                  (1003, 2048, 768)])
 @pytest.mark.parametrize("dtype,act", [(BF16, "silu"), (F16, "gelu_tanh")])

@@ -85,11 +85,11 @@ int forward(const vy_ffn_call* c, const DeviceInfo* dev, cudaStream_t s) {
     d.out = c->out;
     d.ldo = c->out_row_stride;
     if (T <= kStreamMaxTokens) {
-        VY_TRY((stream_launch<EPI_GATE, ACT>(c->w_gate, c->w_up, c->x, c->x_row_stride, static_cast<int>(T), 1, c->inter,
-                                             c->hidden, false, e, c->flags, dev, s)));
-        const int parts = h_parts(c);
-        return stream_launch<EPI_STORE, ACT>(c->w_down, nullptr, h, I, static_cast<int>(T) * parts, parts, c->hidden,
-                                             c->inter, true, d, c->flags, dev, s);
+        const int t = static_cast<int>(T), parts = h_parts(c);
+        const StreamCall gate{c->w_gate, c->w_up, c->x, c->x_row_stride, t, 1, c->inter, c->hidden, false, nullptr, 0};
+        VY_TRY((stream_launch<EPI_GATE, ACT>(gate, e, c->flags, dev, s)));
+        const StreamCall down{c->w_down, nullptr, h, I, t * parts, parts, c->hidden, c->inter, true, nullptr, 0};
+        return stream_launch<EPI_STORE, ACT>(down, d, c->flags, dev, s);
     }
     const int pairs = dev->sm_count / 2;
     {

@@ -4,6 +4,7 @@
 // Bounds.  Quantisation: HBM (each value read once, kept in registers between the row maximum and
 // the rounding).  The products: the weights' bytes for few tokens, the tensor cores' int8 rate
 // (twice the bf16 rate) for many.
+#include "vy_quant.cuh"
 #include "vy_stream.cuh"
 #include "vy_tile.cuh"
 
@@ -22,143 +23,6 @@ struct QuantParams {
     float* scales;
     bool vec;      // rows take 16-byte loads, codes the stores that go with them
 };
-
-// A code is the nearest integer of the exact quotient x / s, ties to even.  With 1 / s rounded down
-// and up, one fused multiply-add each rounds x lo and x hi to the nearest integer (adding 1.5 * 2^23,
-// which leaves the integer's two's complement in the low bits); x / s lies between the two products
-// and rounding is monotone, so where both give one integer it is the code.  Where they differ (about
-// one value in 10^5: a tie c lies between), the sign of x - c s decides, exact under one fused
-// multiply-add.  Two FFMAs and a LOP3 a value; rint and float-to-int conversions run at an eighth of
-// that rate and would bound the kernel; following the distance to the nearest tie instead took some 20
-// instructions a value in all (4096 x 14336, bf16: 46 us, 36 this way).
-constexpr float kRound = 12582912.f;
-
-struct RowScale {
-    float s, lo, hi;
-    float up;           // 1, or 2^100 where 1 / s is out of range: x and s are scaled by it, exactly
-    uint32_t odd;       // not zero when up is not 1: every value takes the long way
-    uint32_t keep;      // 0 for a zero row or a NaN scale: all codes 0; else all ones
-};
-
-__device__ __forceinline__ float quant_long(float v, const RowScale& r) {
-    const float x = v * r.up, s = r.s * r.up;
-    const float t = x * __frcp_rn(s);
-    const float near = (t + kRound) - kRound, d = t - near;
-    float q = near;
-    if (fabsf(d) > 0.499f) {                      // t is off by 2^-23 relative at most
-        const float c = near + copysignf(0.5f, d);
-        const float e = fmaf(-c, s, x);           // c s has 32 bits, nothing underflows: the sign is exact
-        q = e > 0.f ? c + 0.5f : e < 0.f ? c - 0.5f : c;     // c + kRound goes to the even one
-    }
-    // a subnormal s may be so coarse that amax / s passes 127
-    return fminf(fmaxf(q, -127.f), 127.f) + kRound;
-}
-
-// The codes of N values, N / 4 words.
-template <int N>
-__device__ __forceinline__ void quant_words(const float (&v)[N], const RowScale& r, uint32_t (&w)[N / 4]) {
-    uint32_t m[N], differ = r.odd;
-#pragma unroll
-    for (int j = 0; j < N; ++j) {
-        m[j] = __float_as_uint(fmaf(v[j], r.lo, kRound));
-        differ |= m[j] ^ __float_as_uint(fmaf(v[j], r.hi, kRound));
-    }
-    if (differ) {
-#pragma unroll
-        for (int j = 0; j < N; ++j) m[j] = __float_as_uint(quant_long(v[j], r));
-    }
-#pragma unroll
-    for (int q = 0; q < N / 4; ++q) {
-        const uint32_t lo = __byte_perm(m[4 * q], m[4 * q + 1], 0x0040);
-        const uint32_t hi = __byte_perm(m[4 * q + 2], m[4 * q + 3], 0x0040);
-        w[q] = __byte_perm(lo, hi, 0x5410) & r.keep;
-    }
-}
-
-// Plain (coherent) 16-byte load: x may come from the kernel in front, which this one overlaps.
-__device__ __forceinline__ uint4 ld_piece(const uint4* p) {
-    uint4 v;
-    asm volatile("ld.global.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-    return v;
-}
-
-// Values of one 16-byte piece, and their largest magnitude's bit pattern (magnitudes order like
-// their patterns, NaN above infinity: an integer maximum).
-template <int DT>
-struct Piece {
-    static constexpr int N = DT == VY_F32 ? 4 : 8;
-    static __device__ __forceinline__ void values(const uint4& u, float (&v)[N]) {
-        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            if constexpr (DT == VY_F32) {
-                v[j] = __uint_as_float(w[j]);
-            } else if constexpr (DT == VY_BF16) {
-                v[2 * j] = __uint_as_float(w[j] << 16);
-                v[2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u);
-            } else {
-                v[2 * j] = act_from_bits<VY_F16>(w[j] & 0xFFFFu);
-                v[2 * j + 1] = act_from_bits<VY_F16>(w[j] >> 16);
-            }
-        }
-    }
-    // 16-bit types: of each half in place, fp32: of the word
-    static __device__ __forceinline__ uint32_t top(uint32_t t, const uint4& u) {
-        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            if constexpr (DT == VY_F32)
-                t = max(t, w[j] & 0x7FFFFFFFu);
-            else if constexpr (DT == VY_BF16)
-                asm("max.NaN.bf16x2 %0, %0, %1;" : "+r"(t) : "r"(w[j] & 0x7FFF7FFFu));
-            else
-                asm("max.NaN.f16x2 %0, %0, %1;" : "+r"(t) : "r"(w[j] & 0x7FFF7FFFu));
-        }
-        return t;
-    }
-    // the fp32 magnitude's pattern from top's
-    static __device__ __forceinline__ uint32_t wide(uint32_t t) {
-        if constexpr (DT == VY_F32) return t;
-        const uint32_t a = __float_as_uint(act_from_bits<DT>(t & 0xFFFFu)) & 0x7FFFFFFFu;
-        return max(a, __float_as_uint(act_from_bits<DT>(t >> 16)) & 0x7FFFFFFFu);
-    }
-};
-
-// The scale of a row whose largest magnitude has the pattern `top`.
-__device__ __forceinline__ RowScale row_scale(uint32_t top) {
-    RowScale r;
-    r.s = top < 0x7F800000u ? __fdiv_rn(__uint_as_float(top), 127.f) : __uint_as_float(0x7FC00000u);
-    const bool zero = !(r.s > 0.f), tiny = r.s < 1e-30f && !zero;
-    r.up = tiny ? 0x1p100f : 1.f;
-    r.odd = tiny;
-    r.keep = zero ? 0u : 0xFFFFFFFFu;
-    r.lo = zero || tiny ? 0.f : __frcp_rd(r.s);
-    r.hi = zero || tiny ? 0.f : __frcp_ru(r.s);
-    return r;
-}
-// Codes of a row's 16-byte piece `at`.
-template <int DT>
-__device__ __forceinline__ void put_piece(int8_t* out, int64_t at, const uint4& u, const RowScale& r) {
-    using P = Piece<DT>;
-    float v[P::N];
-    uint32_t w[P::N / 4];
-    P::values(u, v);
-    quant_words<P::N>(v, r, w);
-    if constexpr (P::N == 8)
-        reinterpret_cast<uint2*>(out)[at] = make_uint2(w[0], w[1]);
-    else
-        reinterpret_cast<uint32_t*>(out)[at] = w[0];
-}
-// Codes of single values k, k + step, ... below cols (rows that are no whole pieces, or not aligned).
-template <int DT>
-__device__ __forceinline__ void put_tail(int8_t* out, const void* src, int64_t k, int64_t cols, int step, const RowScale& r) {
-    for (; k < cols; k += step) {
-        const float v[4] = {load_as_float(src, DT, k), 0.f, 0.f, 0.f};
-        uint32_t w[1];
-        quant_words<4>(v, r, w);
-        out[k] = static_cast<int8_t>(w[0] & 0xFFu);
-    }
-}
 
 // One block per row; the row stays in registers between its maximum and its codes.
 template <int DT, int THREADS, int UNITS, int BLOCKS>
@@ -269,6 +133,8 @@ struct Product {
     const void* bias;
     int bias_dtype;
     int32_t* flags;
+    uint32_t* maxima;      // GATE, few tokens: the largest |h| of each CTA's columns, for the down product
+    int n_maxima;
 };
 
 template <bool GATE>
@@ -285,9 +151,11 @@ int launch_product(const Product& a, bool first, const DeviceInfo* dev, cudaStre
     e.bias = a.bias;
     e.bias_dtype = a.bias_dtype;
     constexpr int EPI = GATE ? EPI_I8GATE : EPI_I8;
-    if (a.tokens <= kStreamMaxTokens)
-        return stream_launch<EPI, VY_BF16>(a.w[0], a.w[1], a.codes, a.codes_ld, static_cast<int>(a.tokens), 1, a.n, a.k,
-                                           !first, e, a.flags, dev, s);
+    if (a.tokens <= kStreamMaxTokens) {
+        const StreamCall c{a.w[0], a.w[1], a.codes, a.codes_ld, static_cast<int>(a.tokens), 1, a.n, a.k, !first,
+                           a.maxima, a.n_maxima};
+        return stream_launch<EPI, VY_BF16>(c, e, a.flags, dev, s);
+    }
     const int pairs = dev->sm_count / 2;
     TileParams p{};
     TileProblem& q = tile_add(&p, a.tokens, a.n, (a.k + 127) / 128);
@@ -326,6 +194,7 @@ int check_linear(const vy_int8_linear_call* c) {
 struct FfnLayout {
     int8_t *x_codes, *h_codes;
     float *x_scales, *h_scales, *h;
+    uint32_t* maxima;
     size_t bytes;
 };
 FfnLayout ffn_layout(const vy_int8_ffn_call* c, char* base) {
@@ -342,6 +211,8 @@ FfnLayout ffn_layout(const vy_int8_ffn_call* c, char* base) {
     L.h = reinterpret_cast<float*>(take(T * c->inter * 4));
     L.h_codes = reinterpret_cast<int8_t*>(take(T * c->inter));
     L.h_scales = reinterpret_cast<float*>(take(T * 4));
+    if (c->n_tokens <= kSourceTokens)      // at most 8 CTAs a unit
+        L.maxima = reinterpret_cast<uint32_t*>(take(size_t((c->inter + kStreamRows - 1) / kStreamRows) * 8 * T * 4));
     L.bytes = at + 256;
     return L;
 }
@@ -398,7 +269,7 @@ extern "C" int vy_int8_linear(const vy_int8_linear_call* c, void* stream) {
     if (!dev) return st;
     if (c->n_tokens == 0) return ok();
     Product a{c->codes, c->codes_row_stride, c->scales, {c->weight, nullptr}, {c->weight_scales, nullptr}, c->n_tokens,
-              c->k, c->n, c->out, c->out_row_stride, c->out_dtype, 0, c->bias, c->bias_dtype, c->flags};
+              c->k, c->n, c->out, c->out_row_stride, c->out_dtype, 0, c->bias, c->bias_dtype, c->flags, nullptr, 0};
     st = launch_product<false>(a, true, dev, as_stream(stream));
     return st != VY_OK ? st : check_launch("vy_int8_linear");
 }
@@ -417,13 +288,45 @@ extern "C" int vy_int8_gated_ffn(const vy_int8_ffn_call* c, void* stream) {
     cudaStream_t s = as_stream(stream);
     const FfnLayout L = ffn_layout(
         c, reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(c->workspace) + 255) & ~uintptr_t(255)));
+    const int t = static_cast<int>(c->n_tokens);
+    EpiParams d{};
+    d.out = c->out;
+    d.ldo = c->out_row_stride;
+    d.out_dtype = c->act_dtype;
+    d.col_scale[0] = c->down_scales;
+    if (c->n_tokens <= kSourceTokens) {
+        const int nk = (c->hidden + 127) / 128;
+        const int ctas = stream_ctas(2, t, 1, c->inter, nk, dev->sm_count);
+        EpiParams g{};
+        g.out = L.h;
+        g.ldo = c->inter;
+        g.act = c->activation;
+        g.col_scale[0] = c->gate_scales;
+        g.col_scale[1] = c->up_scales;
+        // the rows' maxima taken in every CTA: worth a launch while a row set is small (32 KB)
+        const bool rows = c->n_tokens * c->hidden <= 16384 && aligned16(c->x) && (t == 1 || c->x_row_stride % 8 == 0);
+        if (rows) {
+            const StreamCall gate{c->w_gate, c->w_up, c->x, c->x_row_stride, t, 1, c->inter, c->hidden, false, L.maxima, ctas};
+            VY_TRY(c->act_dtype == VY_BF16 ? (stream_launch<EPI_I8GATE, VY_BF16, SRC_ROWS>(gate, g, c->flags, dev, s))
+                                           : (stream_launch<EPI_I8GATE, VY_F16, SRC_ROWS>(gate, g, c->flags, dev, s)));
+        } else {
+            VY_TRY(launch_quantize(c->x, c->act_dtype, c->x_row_stride, c->n_tokens, c->hidden, L.x_codes, L.x_scales,
+                                   dev->sm_count, s));
+            g.row_scale = L.x_scales;
+            const StreamCall gate{c->w_gate, c->w_up, L.x_codes, c->hidden, t, 1, c->inter, c->hidden, true, L.maxima, ctas};
+            VY_TRY((stream_launch<EPI_I8GATE, VY_BF16>(gate, g, c->flags, dev, s)));
+        }
+        const StreamCall down{c->w_down, nullptr, L.h, c->inter, t, 1, c->hidden, c->inter, true, L.maxima, ctas};
+        VY_TRY((stream_launch<EPI_I8, VY_BF16, SRC_HIDDEN>(down, d, c->flags, dev, s)));
+        return check_launch("vy_int8_gated_ffn");
+    }
     VY_TRY(launch_quantize(c->x, c->act_dtype, c->x_row_stride, c->n_tokens, c->hidden, L.x_codes, L.x_scales, dev->sm_count, s));
     Product gu{L.x_codes, c->hidden, L.x_scales, {c->w_gate, c->w_up}, {c->gate_scales, c->up_scales}, c->n_tokens,
-               c->hidden, c->inter, L.h, c->inter, VY_F32, c->activation, nullptr, 0, c->flags};
+               c->hidden, c->inter, L.h, c->inter, VY_F32, c->activation, nullptr, 0, c->flags, nullptr, 0};
     VY_TRY(launch_product<true>(gu, false, dev, s));
     VY_TRY(launch_quantize(L.h, VY_F32, c->inter, c->n_tokens, c->inter, L.h_codes, L.h_scales, dev->sm_count, s));
     Product down{L.h_codes, c->inter, L.h_scales, {c->w_down, nullptr}, {c->down_scales, nullptr}, c->n_tokens, c->inter,
-                 c->hidden, c->out, c->out_row_stride, c->act_dtype, 0, nullptr, 0, c->flags};
+                 c->hidden, c->out, c->out_row_stride, c->act_dtype, 0, nullptr, 0, c->flags, nullptr, 0};
     VY_TRY(launch_product<false>(down, false, dev, s));
     return check_launch("vy_int8_gated_ffn");
 }

@@ -10,11 +10,18 @@
 // barrier each CTA adds its slice over all shares, in rank order.  No workspace, no atomics, one
 // order of summation, and no remote read to wait for.
 //
+// With up to 16 tokens the int8 block needs no quantisation kernels (Source): the four warps that read
+// the sums at the end are idle until then and write the token tile's codes themselves, a 16-value
+// piece of a token each per K block, from rows that are still floats.  The rows' largest magnitudes
+// come from the kernel in front, whose every CTA leaves the maximum of the columns it wrote (no
+// atomics, nothing to clear), or, for one or two tokens, are taken over the whole row in place.
+//
 // A kernel that is not the first of its call starts loading weights before the kernel in front of it
 // has finished (they do not depend on it); its token tiles wait for it.
 #pragma once
 
 #include "vy_dense.cuh"
+#include "vy_quant.cuh"
 
 namespace vy {
 
@@ -22,7 +29,15 @@ constexpr int kStreamRows = 128;        // weight rows of a unit (of each matrix
 constexpr int kStreamMaxTokens = 128;
 constexpr int kStreamThreads = 192;     // warps 0-3 read the sums, 4 loads, 5 issues the MMAs
 constexpr int kStreamMaxStages = 12;
-constexpr int kSmemMost = 226 * 1024, kSmemHalf = 112 * 1024;   // dynamic bytes of one CTA, of two on an SM
+constexpr int kSmemMost = 225 * 1024, kSmemHalf = 111 * 1024;   // dynamic bytes of one CTA, of two on an SM
+
+// Where the token tile comes from.
+enum Source {
+    SRC_TMA = 0,      // [tokens, K] in the weights' type
+    SRC_ROWS = 1,     // int8 codes made here from 16-bit rows, whose maxima are taken here
+    SRC_HIDDEN = 2    // int8 codes made here from fp32 rows, whose maxima the previous kernel left
+};
+constexpr int kSourceTokens = 16;      // 8 pieces of a K block each, one per thread of four warps
 
 struct StreamParams {
     CUtensorMap w[2], x;
@@ -34,11 +49,17 @@ struct StreamParams {
     int parts;              // 2: x holds high parts, then low parts; an output is the sum of both
     EpiParams epi;
     int32_t* flags;
+    const void* rows;       // SRC_ROWS, SRC_HIDDEN: [tokens, k], row stride, K in elements
+    int64_t rows_ld;
+    int k;
+    uint32_t* maxima;       // EPI_I8GATE: this kernel's, [CTA][token]; SRC_HIDDEN: the previous one's
+    int n_maxima;           // CTAs in it (0: none wanted)
 };
 
 struct StreamBars {
     uint64_t full[kStreamMaxStages], empty[kStreamMaxStages], done;
     float token_scale[kStreamMaxTokens];
+    uint32_t token_top[kSourceTokens], part_top[4][kSourceTokens];
     uint32_t tmem_base;
     int abort_flag;
 };
@@ -65,7 +86,7 @@ __device__ __forceinline__ ColumnScale column_scale(const StreamParams& p, int r
 }
 template <int EPI, int ACT>
 __device__ __forceinline__ void stream_put(const StreamParams& p, int row, int t, uint32_t s0, uint32_t s1,
-                                           const ColumnScale& cs, const float* token_scale) {
+                                           const ColumnScale& cs, const float* token_scale, uint32_t* token_top) {
     const EpiParams& e = p.epi;
     const int64_t at = int64_t(t) * e.ldo + row;
     if constexpr (EPI == EPI_GATE) {
@@ -83,7 +104,9 @@ __device__ __forceinline__ void stream_put(const StreamParams& p, int row, int t
     } else if constexpr (EPI == EPI_I8GATE) {
         const float g = __fmul_rn(__fmul_rn(float(int(s0)), token_scale[t]), cs.a);
         const float u = __fmul_rn(__fmul_rn(float(int(s1)), token_scale[t]), cs.b);
-        reinterpret_cast<float*>(e.out)[at] = gate_act(g, e.act) * u;
+        const float h = gate_act(g, e.act) * u;
+        reinterpret_cast<float*>(e.out)[at] = h;
+        if (p.n_maxima) atomicMax(token_top + t, __float_as_uint(h) & 0x7FFFFFFFu);
     } else {
         float v = __fmul_rn(__fmul_rn(float(int(s0)), token_scale[t]), cs.a);
         if (e.bias) v = __fadd_rn(v, cs.b);
@@ -95,7 +118,34 @@ __device__ __forceinline__ void st_cluster(uint32_t addr, uint32_t v) {
     asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
 }
 
-template <int EPI, int ACT>
+// A piece of 16 values of a row that starts on a 16-byte boundary.
+template <int SRC, int ACT>
+struct RowPiece {
+    static constexpr int DT = SRC == SRC_HIDDEN ? VY_F32 : ACT;
+    static constexpr int V = DT == VY_F32 ? 4 : 2;      // 16-byte loads
+    uint4 u[V];
+    __device__ __forceinline__ void load(const void* rows, int64_t at, bool in) {
+        const uint4* p = reinterpret_cast<const uint4*>(static_cast<const unsigned char*>(rows) + at * (DT == VY_F32 ? 4 : 2));
+#pragma unroll
+        for (int i = 0; i < V; ++i) u[i] = in ? ld_piece(p + i) : make_uint4(0, 0, 0, 0);
+    }
+    __device__ __forceinline__ uint4 codes(const RowScale& r) const {
+        using P = Piece<DT>;
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            float v[P::N];
+            uint32_t o[P::N / 4];
+            P::values(u[i], v);
+            quant_words<P::N>(v, r, o);
+#pragma unroll
+            for (int j = 0; j < P::N / 4; ++j) w[i * (P::N / 4) + j] = o[j];
+        }
+        return make_uint4(w[0], w[1], w[2], w[3]);
+    }
+};
+
+template <int EPI, int ACT, int SRC>
 __global__ void __launch_bounds__(kStreamThreads) stream_kernel(const __grid_constant__ StreamParams p) {
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     __shared__ StreamBars S;
@@ -111,12 +161,13 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(const __grid_con
     const int row0 = unit * kStreamRows;
     const uint32_t x_bytes = uint32_t(p.cols) * 128u;
     const uint32_t stage_bytes = NW * 16384u + x_bytes;
+    constexpr bool kOwnCodes = SRC != SRC_TMA;
     const int k_first = int(int64_t(p.nk) * rank / splits), k_last = int(int64_t(p.nk) * (rank + 1) / splits);
     const int nk = k_last - k_first;
 
     if (tid == 0) {
         for (int i = 0; i < p.stages; ++i) {
-            mbar_init(&S.full[i], 1);
+            mbar_init(&S.full[i], kOwnCodes ? 5 : 1);      // the loads, and the four code-writing warps
             mbar_init(&S.empty[i], 1);
         }
         mbar_init(&S.done, 1);
@@ -126,7 +177,7 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(const __grid_con
     if (warp == 4 && lane == 0) {
         prefetch_map(&p.w[0]);
         if (NW == 2) prefetch_map(&p.w[1]);
-        prefetch_map(&p.x);
+        if (!kOwnCodes) prefetch_map(&p.x);
     }
     if (warp == 0) tmem_alloc_n<0>(&S.tmem_base, p.tmem_cols);
     tc_fence_before();
@@ -141,16 +192,60 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(const __grid_con
         grid_dependents_launch();
     }
 
+    if (kOwnCodes && warp < 4) {
+        // thread: token tid / 8, piece tid % 8 of each K block
+        const int t = tid >> 3, c = tid & 7;
+        uint32_t top = 0;
+        if constexpr (SRC == SRC_HIDDEN) {
+            if (t < p.tokens)
+                for (int i = c; i < p.n_maxima; i += 8) top = max(top, p.maxima[i * p.tokens + t]);
+#pragma unroll
+            for (int d = 1; d < 8; d *= 2) top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
+        } else if constexpr (SRC == SRC_ROWS) {
+            using P = Piece<ACT>;
+            for (int r = 0; r < p.tokens; ++r) {
+                const uint4* row = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.rows) + r * p.rows_ld);
+                uint32_t m = 0;
+#pragma unroll 4
+                for (int i = tid; i < p.k / 8; i += 128) m = P::top(m, ld_piece(row + i));
+                m = __reduce_max_sync(0xffffffffu, P::wide(m));
+                if (lane == 0) S.part_top[warp][r] = m;
+            }
+            asm volatile("bar.sync 1, 128;" ::: "memory");
+            if (t < p.tokens)
+                for (int w = 0; w < 4; ++w) top = max(top, S.part_top[w][t]);
+        }
+        const RowScale scale = row_scale(top);
+        if (c == 0 && t < p.tokens) S.token_scale[t] = scale.s;
+        RowPiece<SRC, ACT> piece;
+        const int64_t at = t * p.rows_ld + int64_t(k_first) * kBlockK + c * 16;
+        const int left = p.k - k_first * kBlockK - c * 16;      // values from my first piece to the row's end
+        piece.load(p.rows, at, t < p.tokens && left > 0);
+        int stage = 0;
+        uint32_t phase = 1;
+        for (int i = 0; i < nk; ++i) {
+            const uint4 codes = piece.codes(scale);
+            if (i + 1 < nk) piece.load(p.rows, at + (i + 1) * kBlockK, t < p.tokens && left > (i + 1) * kBlockK);
+            if (!mbar_wait_warp(&S.empty[stage], phase, abort_flag, p.flags)) break;
+            // rows of padding tokens keep what the ring holds: their sums are not used
+            if (t < p.tokens)
+                *reinterpret_cast<uint4*>(ring + stage * stage_bytes + NW * 16384 + t * 128 + ((c ^ (t & 7)) << 4)) = codes;
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&S.full[stage]);
+            if (++stage == p.stages) stage = 0, phase ^= 1;
+        }
+    }
     if (warp == 4) {
         auto load_w = [&](int i, uint32_t s) {
             const int k = (k_first + i) * kBlockK;
             unsigned char* at = ring + s * stage_bytes;
-            mbar_expect_tx(&S.full[s], stage_bytes);
+            mbar_expect_tx(&S.full[s], kOwnCodes ? NW * 16384u : stage_bytes);
             tma_load_2d(at, &p.w[0], k, row0, &S.full[s]);
             if (NW == 2) tma_load_2d(at + 16384, &p.w[1], k, row0, &S.full[s]);
         };
         auto load_x = [&](int i, uint32_t s) {
-            tma_load_2d(ring + s * stage_bytes + NW * 16384, &p.x, (k_first + i) * kBlockK, 0, &S.full[s]);
+            if (!kOwnCodes) tma_load_2d(ring + s * stage_bytes + NW * 16384, &p.x, (k_first + i) * kBlockK, 0, &S.full[s]);
         };
         const int ahead = p.early ? min(p.stages, nk) : 0;
         if (elect_one())
@@ -199,16 +294,18 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(const __grid_con
     __syncwarp();
 
     // received sums [share][matrix][token][row of my slice], rows fastest
-    const int rows = kStreamRows / splits;      // 1, 2, 4 or 8 shares
+    const int row_bits = 7 - (31 - __clz(splits)), rows = 1 << row_bits;      // 1, 2, 4 or 8 shares of 128 rows
     uint32_t* sums = reinterpret_cast<uint32_t*>(ring + p.sums_at);
     // the weight row of this thread: its lane's when it reads all sums itself, else of my slice
     // (whole multiples of a slice's rows take part, so every output a thread adds has the same row)
-    const int step = kStreamThreads / rows * rows;
+    const int step = rows == kStreamRows ? kStreamRows : kStreamThreads;
     const bool direct = splits == 1 && p.parts == 1;      // nothing to join: outputs straight from TMEM
-    const int my_row = row0 + (direct ? tid & (kStreamRows - 1) : int(rank) * rows + tid % rows);
+    const int my_row = row0 + (direct ? tid & (kStreamRows - 1) : int(rank) * rows + (tid & (rows - 1)));
     const ColumnScale cs = column_scale<EPI>(p, my_row);
     if constexpr (epi_is_i8(EPI)) {
-        for (int t = tid; t < p.tokens; t += kStreamThreads) S.token_scale[t] = p.epi.row_scale[t];
+        if (!kOwnCodes)
+            for (int t = tid; t < p.tokens; t += kStreamThreads) S.token_scale[t] = p.epi.row_scale[t];
+        if (tid < kSourceTokens) S.token_top[tid] = 0;
         __syncthreads();
     }
     if (splits > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
@@ -217,8 +314,8 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(const __grid_con
         tc_fence_after();
         const uint32_t lanes = uint32_t(warp * 32) << 16;
         const int row = warp * 32 + lane;
-        const uint32_t owner = map_to_rank(smem_u32(sums), row / rows) +
-                               4u * (rank * NW * p.tokens * rows + row % rows);
+        const uint32_t owner = map_to_rank(smem_u32(sums), row >> row_bits) +
+                               4u * (rank * NW * p.tokens * rows + (row & (rows - 1)));
         if (ready) {
             for (int c = 0; c < p.cols; c += 16) {
                 uint32_t v[NW][16];
@@ -231,7 +328,7 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(const __grid_con
 #pragma unroll
                         for (int j = 0; j < 16; ++j)
                             if (c + j < p.tokens) stream_put<EPI, ACT>(p, row0 + row, c + j, v[0][j], v[NW - 1][j], cs,
-                                                     S.token_scale);
+                                                     S.token_scale, S.token_top);
                     }
                 } else {
 #pragma unroll
@@ -247,31 +344,38 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(const __grid_con
     __syncwarp();
     if (!direct) {
         cluster_sync();
-        const int share = NW * p.tokens * rows;
-        for (int q = tid < step ? tid : rows * p.tokens; q < rows * (p.tokens / p.parts); q += step) {
-            const int t = q / rows;
-            if (my_row >= p.n) continue;
-            uint32_t sum[NW];
+        const int share = NW * p.tokens * rows, count = p.parts == 2 ? p.tokens / 2 * rows : p.tokens * rows;
+        // all shares of a sum are fetched before the first is added
+        auto joined = [&](const uint32_t* at) {
+            uint32_t v[8];
 #pragma unroll
-            for (int m = 0; m < NW; ++m) {
-                const uint32_t* at = sums + (m * p.tokens + t) * rows + q % rows;
-                uint32_t acc = at[0];
-                for (uint32_t r = 1; r < splits; ++r) {
-                    const uint32_t v = at[r * share];
-                    acc = I8 ? acc + v : __float_as_uint(__fadd_rn(__uint_as_float(acc), __uint_as_float(v)));
-                }
-                if (EPI == EPI_STORE && p.parts == 2) {
-                    at += p.tokens / 2 * rows;
-                    float low = __uint_as_float(at[0]);
-                    for (uint32_t r = 1; r < splits; ++r) low = __fadd_rn(low, __uint_as_float(at[r * share]));
-                    acc = __float_as_uint(__fadd_rn(__uint_as_float(acc), low));
-                }
-                sum[m] = acc;
-            }
-            stream_put<EPI, ACT>(p, my_row, t, sum[0], sum[NW - 1], cs, S.token_scale);
+            for (uint32_t r = 0; r < 8; ++r)
+                if (r < splits) v[r] = at[r * share];
+            uint32_t acc = v[0];
+#pragma unroll
+            for (uint32_t r = 1; r < 8; ++r)
+                if (r < splits)
+                    acc = I8 ? acc + v[r] : __float_as_uint(__fadd_rn(__uint_as_float(acc), __uint_as_float(v[r])));
+            return acc;
+        };
+        for (int q = tid; q < count && tid < step && my_row < p.n; q += step) {
+            const int t = q >> row_bits;
+            const uint32_t* at = sums + q;
+            uint32_t sum[NW];
+            sum[0] = joined(at);
+            if (NW == 2) sum[NW - 1] = joined(at + p.tokens * rows);
+            if (EPI == EPI_STORE && p.parts == 2)
+                sum[0] = __float_as_uint(__fadd_rn(__uint_as_float(sum[0]), __uint_as_float(joined(at + count))));
+            stream_put<EPI, ACT>(p, my_row, t, sum[0], sum[NW - 1], cs, S.token_scale, S.token_top);
         }
     } else {
         __syncthreads();
+    }
+    if constexpr (EPI == EPI_I8GATE) {
+        if (p.n_maxima) {
+            __syncthreads();
+            if (tid < p.tokens) p.maxima[int64_t(blockIdx.x) * p.tokens + tid] = S.token_top[tid];
+        }
     }
     tc_fence_after();
     if (warp == 0) tmem_free_n<0>(tmem, p.tmem_cols);
@@ -305,41 +409,63 @@ inline StreamPlan stream_plan(int nw, int tokens, int parts, int n, int nk, int 
     return p;
 }
 
-// w: NW weight matrices [n, k], contiguous; x: [tokens, k] (parts == 2: high parts, then low parts).
-template <int EPI, int ACT>
-int stream_launch(const void* w0, const void* w1, const void* x, int64_t x_ld, int tokens, int parts, int n, int k,
-                  bool early, const EpiParams& epi, int32_t* flags, const DeviceInfo* dev, cudaStream_t s) {
+// One product: its weight matrices [n, k] (contiguous) and its token rows.
+struct StreamCall {
+    const void *w0, *w1;      // w1: the up matrix of a gated product
+    const void* x;            // [tokens, k]; parts == 2: high parts, then low parts of tokens / 2 rows
+    int64_t x_ld;
+    int tokens, parts, n, k;
+    bool early;               // a kernel of the same call runs in front of this one
+    uint32_t* maxima;         // see StreamParams
+    int n_maxima;
+};
+
+// CTAs of a product's launch.
+inline int stream_ctas(int nw, int tokens, int parts, int n, int nk, int sm_count) {
+    return (n + kStreamRows - 1) / kStreamRows * stream_plan(nw, tokens, parts, n, nk, sm_count).splits;
+}
+
+template <int EPI, int ACT, int SRC = SRC_TMA>
+int stream_launch(const StreamCall& a, const EpiParams& epi, int32_t* flags, const DeviceInfo* dev, cudaStream_t s) {
     constexpr bool I8 = epi_is_i8(EPI);
     constexpr int NW = epi_is_gate(EPI) ? 2 : 1;
     constexpr int block = I8 ? 128 : 64;
     const int dtype = I8 ? VY_E4M3 : ACT;
     StreamParams p{};
-    p.tokens = tokens;
-    p.n = n;
-    p.nk = (k + block - 1) / block;
-    p.cols = (tokens + 15) / 16 * 16;
-    p.early = early;
-    p.parts = parts;
+    p.tokens = a.tokens;
+    p.n = a.n;
+    p.nk = (a.k + block - 1) / block;
+    p.cols = (a.tokens + 15) / 16 * 16;
+    p.early = a.early;
+    p.parts = a.parts;
     p.epi = epi;
     p.flags = flags;
+    p.maxima = a.maxima;
+    p.n_maxima = a.n_maxima;
     p.tmem_cols = 32;
     while (p.tmem_cols < NW * p.cols) p.tmem_cols *= 2;
     int st;
-    if ((st = make_map_2d(&p.w[0], dtype, w0, n, k, k, block, kStreamRows)) != VY_OK) return st;
-    if (NW == 2 && (st = make_map_2d(&p.w[1], dtype, w1, n, k, k, block, kStreamRows)) != VY_OK) return st;
-    if ((st = make_map_2d(&p.x, dtype, x, tokens, k, x_ld, block, p.cols)) != VY_OK) return st;
-    const StreamPlan plan = stream_plan(NW, tokens, parts, n, p.nk, dev->sm_count);
-    if (plan.stages < 2) return fail(VY_ERR_UNSUPPORTED, "dense stream: %d tokens", tokens);
+    if ((st = make_map_2d(&p.w[0], dtype, a.w0, a.n, a.k, a.k, block, kStreamRows)) != VY_OK) return st;
+    if (NW == 2 && (st = make_map_2d(&p.w[1], dtype, a.w1, a.n, a.k, a.k, block, kStreamRows)) != VY_OK) return st;
+    if (SRC == SRC_TMA) {
+        if ((st = make_map_2d(&p.x, dtype, a.x, a.tokens, a.k, a.x_ld, block, p.cols)) != VY_OK) return st;
+    } else {
+        p.rows = a.x;
+        p.rows_ld = a.x_ld;
+        p.k = a.k;
+    }
+    const StreamPlan plan = stream_plan(NW, a.tokens, a.parts, a.n, p.nk, dev->sm_count);
+    if (plan.stages < 2) return fail(VY_ERR_UNSUPPORTED, "dense stream: %d tokens", a.tokens);
     p.stages = plan.stages;
     p.sums_at = plan.stages * plan.stage;
     const int bytes = p.sums_at + plan.sums + 1024;
-    auto kern = stream_kernel<EPI, ACT>;
+    auto kern = stream_kernel<EPI, ACT, SRC>;
     st = once_per_device(reinterpret_cast<const void*>(kern), [](int, void* f) {
         const cudaError_t e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMost);
         return e == cudaSuccess ? VY_OK : fail(VY_ERR_CUDA, "dense stream shared memory: %s", cudaGetErrorString(e));
     }, reinterpret_cast<void*>(kern));
     if (st != VY_OK) return st;
-    const unsigned units = (n + kStreamRows - 1) / kStreamRows;
+    const unsigned units = (a.n + kStreamRows - 1) / kStreamRows;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(units * plan.splits);
     cfg.blockDim = dim3(kStreamThreads);
