@@ -133,4 +133,45 @@ struct EpiParams {
     int bias_dtype;
 };
 
+// ── host: clusters the device runs at once ──────────────────────────────────────────────────
+
+constexpr int kSmemMost = 225 * 1024, kSmemHalf = 111 * 1024;   // dynamic bytes of one CTA, of two on an SM
+
+// How many clusters of 1, 2, 4 and 8 CTAs are resident together with one or two CTAs an SM.  A cluster
+// sits in one GPC, so the larger ones leave SMs over: 148, 74, 33 and 15 at one CTA an SM.
+struct ClusterCaps {
+    int one[4], two[4];
+};
+static __global__ void __launch_bounds__(384, 1) cluster_probe_kernel() {}
+inline const ClusterCaps* cluster_caps(int* status) {
+    static ClusterCaps caps[kMaxDevices];
+    *status = once_per_device(reinterpret_cast<const void*>(caps), [](int device, void* c) {
+        cudaError_t e = cudaFuncSetAttribute(cluster_probe_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMost);
+        for (int i = 0; i < 8 && e == cudaSuccess; ++i) {
+            cudaLaunchConfig_t cfg = {};
+            cfg.gridDim = dim3(1024);
+            cfg.blockDim = dim3(384);
+            cfg.dynamicSmemBytes = i < 4 ? kSmemMost : kSmemHalf;
+            cudaLaunchAttribute attr[1];
+            attr[0].id = cudaLaunchAttributeClusterDimension;
+            attr[0].val.clusterDim.x = 1u << (i & 3);
+            attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+            cfg.attrs = attr;
+            cfg.numAttrs = 1;
+            int n = 0;
+            e = cudaOccupancyMaxActiveClusters(&n, cluster_probe_kernel, &cfg);
+            ClusterCaps& to = static_cast<ClusterCaps*>(c)[device];
+            (i < 4 ? to.one : to.two)[i & 3] = n > 0 ? n : 1;
+        }
+        return e == cudaSuccess ? VY_OK : fail(VY_ERR_CUDA, "cluster occupancy: %s", cudaGetErrorString(e));
+    }, caps);
+    if (*status != VY_OK) return nullptr;
+    const int dev = current_device();
+    if (dev < 0) {
+        *status = VY_ERR_CUDA;
+        return nullptr;
+    }
+    return &caps[dev];
+}
+
 }  // namespace vy

@@ -71,7 +71,7 @@ void epi_store(TileProblem* q, void* out, int64_t ldo) {
 int k_blocks(int64_t k) { return static_cast<int>((k + 63) / 64); }
 
 template <int ACT>
-int forward(const vy_ffn_call* c, const DeviceInfo* dev, cudaStream_t s) {
+int forward(const vy_ffn_call* c, const ClusterCaps& caps, cudaStream_t s) {
     const int64_t T = c->n_tokens, H = c->hidden, I = c->inter;
     uint16_t* h = reinterpret_cast<uint16_t*>((reinterpret_cast<uintptr_t>(c->workspace) + 255) & ~uintptr_t(255));
     EpiParams e{};
@@ -87,36 +87,34 @@ int forward(const vy_ffn_call* c, const DeviceInfo* dev, cudaStream_t s) {
     if (T <= kStreamMaxTokens) {
         const int t = static_cast<int>(T), parts = h_parts(c);
         const StreamCall gate{c->w_gate, c->w_up, c->x, c->x_row_stride, t, 1, c->inter, c->hidden, false, nullptr, 0};
-        VY_TRY((stream_launch<EPI_GATE, ACT>(gate, e, c->flags, dev, s)));
+        VY_TRY((stream_launch<EPI_GATE, ACT>(gate, e, c->flags, caps, s)));
         const StreamCall down{c->w_down, nullptr, h, I, t * parts, parts, c->hidden, c->inter, true, nullptr, 0};
-        return stream_launch<EPI_STORE, ACT>(down, d, c->flags, dev, s);
+        return stream_launch<EPI_STORE, ACT>(down, d, c->flags, caps, s);
     }
-    const int pairs = dev->sm_count / 2;
     {
         TileParams p{};
         TileProblem& q = tile_add(&p, T, I, k_blocks(H));
-        tile_layout(&p, true, pairs);
+        tile_layout(&p, true, caps);
         VY_TRY(tile_operand(&q.a[0], ACT, c->x, T, H, c->x_row_stride, false, 128));
         VY_TRY(tile_operand(&q.b[0], ACT, c->w_gate, I, H, H, false, q.bn / 2));
         VY_TRY(tile_operand(&q.b[1], ACT, c->w_up, I, H, H, false, q.bn / 2));
         q.epi = e;
         p.flags = c->flags;
-        VY_TRY((tile_launch<EPI_GATE, ACT>(p, pairs, s)));
+        VY_TRY((tile_launch<EPI_GATE, ACT>(p, caps, s)));
     }
     TileParams p{};
     TileProblem& q = tile_add(&p, T, H, k_blocks(I));
-    tile_layout(&p, false, pairs);
+    tile_layout(&p, false, caps);
     VY_TRY(tile_operand(&q.a[0], ACT, h, T, I, I, false, 128));
     VY_TRY(tile_operand(&q.b[0], ACT, c->w_down, H, I, I, false, q.bn / 2));
     q.epi = d;
     p.flags = c->flags;
-    return tile_launch<EPI_STORE, ACT>(p, pairs, s);
+    return tile_launch<EPI_STORE, ACT>(p, caps, s);
 }
 
 template <int ACT>
-int backward(const vy_ffn_call* c, const DeviceInfo* dev, cudaStream_t s) {
+int backward(const vy_ffn_call* c, const ClusterCaps& caps, cudaStream_t s) {
     const int64_t T = c->n_tokens, H = c->hidden, I = c->inter;
-    const int pairs = dev->sm_count / 2;
     char* base = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(c->workspace) + 255) & ~uintptr_t(255));
     const size_t each = h_bytes(c);
     const int parts = h_parts(c);
@@ -127,7 +125,7 @@ int backward(const vy_ffn_call* c, const DeviceInfo* dev, cudaStream_t s) {
     {
         TileParams p{};
         TileProblem& q = tile_add(&p, T, I, k_blocks(H));
-        tile_layout(&p, false, pairs);
+        tile_layout(&p, false, caps);
         q.b_mn = 1;
         VY_TRY(tile_operand(&q.a[0], ACT, c->d_out, T, H, c->d_out_row_stride, false, 128));
         VY_TRY(tile_operand(&q.b[0], ACT, c->w_down, I, H, I, true, 0));
@@ -140,7 +138,7 @@ int backward(const vy_ffn_call* c, const DeviceInfo* dev, cudaStream_t s) {
         q.epi.du = du;
         q.epi.h = h;
         p.flags = c->flags;
-        VY_TRY((tile_launch<EPI_DGATE, ACT>(p, pairs, s)));
+        VY_TRY((tile_launch<EPI_DGATE, ACT>(p, caps, s)));
     }
     TileParams p{};
     p.flags = c->flags;
@@ -181,8 +179,8 @@ int backward(const vy_ffn_call* c, const DeviceInfo* dev, cudaStream_t s) {
         epi_store(&q, g.out, g.n);
     }
     if (p.n_problems == 0) return VY_OK;
-    tile_layout(&p, false, pairs);
-    return tile_launch<EPI_STORE, ACT>(p, pairs, s);
+    tile_layout(&p, false, caps);
+    return tile_launch<EPI_STORE, ACT>(p, caps, s);
 }
 
 }  // namespace
@@ -202,18 +200,20 @@ extern "C" size_t vy_gated_ffn_workspace_size(const vy_ffn_call* c, int32_t back
 extern "C" int vy_gated_ffn_forward(const vy_ffn_call* c, void* stream) {
     int st;
     if ((st = check_ffn(c, false)) != VY_OK) return st;
-    const DeviceInfo* dev = device_info(&st);
-    if (!dev) return st;
+    if (!device_info(&st)) return st;
+    const ClusterCaps* caps = cluster_caps(&st);
+    if (!caps) return st;
     if (c->n_tokens == 0) return ok();
-    st = c->act_dtype == VY_BF16 ? forward<VY_BF16>(c, dev, as_stream(stream)) : forward<VY_F16>(c, dev, as_stream(stream));
+    st = c->act_dtype == VY_BF16 ? forward<VY_BF16>(c, *caps, as_stream(stream)) : forward<VY_F16>(c, *caps, as_stream(stream));
     return st != VY_OK ? st : check_launch("vy_gated_ffn_forward");
 }
 
 extern "C" int vy_gated_ffn_backward(const vy_ffn_call* c, void* stream) {
     int st;
     if ((st = check_ffn(c, true)) != VY_OK) return st;
-    const DeviceInfo* dev = device_info(&st);
-    if (!dev) return st;
+    if (!device_info(&st)) return st;
+    const ClusterCaps* caps = cluster_caps(&st);
+    if (!caps) return st;
     if (c->n_tokens == 0) {      // no token, no contribution: the weight gradients are zero
         const size_t bytes = size_t(c->hidden) * size_t(c->inter) * 2;
         for (void* w : {c->d_w_gate, c->d_w_up, c->d_w_down})
@@ -221,6 +221,6 @@ extern "C" int vy_gated_ffn_backward(const vy_ffn_call* c, void* stream) {
                 return check_launch("vy_gated_ffn_backward");
         return ok();
     }
-    st = c->act_dtype == VY_BF16 ? backward<VY_BF16>(c, dev, as_stream(stream)) : backward<VY_F16>(c, dev, as_stream(stream));
+    st = c->act_dtype == VY_BF16 ? backward<VY_BF16>(c, *caps, as_stream(stream)) : backward<VY_F16>(c, *caps, as_stream(stream));
     return st != VY_OK ? st : check_launch("vy_gated_ffn_backward");
 }

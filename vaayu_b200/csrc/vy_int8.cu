@@ -138,7 +138,7 @@ struct Product {
 };
 
 template <bool GATE>
-int launch_product(const Product& a, bool first, const DeviceInfo* dev, cudaStream_t s) {
+int launch_product(const Product& a, bool first, const ClusterCaps& caps, cudaStream_t s) {
     EpiParams e{};
     e.out = a.out;
     e.ldo = a.ldo;
@@ -154,18 +154,17 @@ int launch_product(const Product& a, bool first, const DeviceInfo* dev, cudaStre
     if (a.tokens <= kStreamMaxTokens) {
         const StreamCall c{a.w[0], a.w[1], a.codes, a.codes_ld, static_cast<int>(a.tokens), 1, a.n, a.k, !first,
                            a.maxima, a.n_maxima};
-        return stream_launch<EPI, VY_BF16>(c, e, a.flags, dev, s);
+        return stream_launch<EPI, VY_BF16>(c, e, a.flags, caps, s);
     }
-    const int pairs = dev->sm_count / 2;
     TileParams p{};
     TileProblem& q = tile_add(&p, a.tokens, a.n, (a.k + 127) / 128);
-    tile_layout(&p, GATE, pairs);
+    tile_layout(&p, GATE, caps);
     VY_TRY(tile_operand(&q.a[0], VY_E4M3, a.codes, a.tokens, a.k, a.codes_ld, false, 128));
     VY_TRY(tile_operand(&q.b[0], VY_E4M3, a.w[0], a.n, a.k, a.k, false, q.bn / 2));
     if (GATE) VY_TRY(tile_operand(&q.b[1], VY_E4M3, a.w[1], a.n, a.k, a.k, false, q.bn / 2));
     q.epi = e;
     p.flags = a.flags;
-    return tile_launch<EPI, VY_BF16>(p, pairs, s);
+    return tile_launch<EPI, VY_BF16>(p, caps, s);
 }
 
 bool float_dtype(int d) { return d == VY_BF16 || d == VY_F16 || d == VY_F32; }
@@ -265,12 +264,13 @@ extern "C" size_t vy_int8_linear_workspace_size(const vy_int8_linear_call*) { re
 extern "C" int vy_int8_linear(const vy_int8_linear_call* c, void* stream) {
     int st;
     if ((st = check_linear(c)) != VY_OK) return st;
-    const DeviceInfo* dev = device_info(&st);
-    if (!dev) return st;
+    if (!device_info(&st)) return st;
+    const ClusterCaps* caps = cluster_caps(&st);
+    if (!caps) return st;
     if (c->n_tokens == 0) return ok();
     Product a{c->codes, c->codes_row_stride, c->scales, {c->weight, nullptr}, {c->weight_scales, nullptr}, c->n_tokens,
               c->k, c->n, c->out, c->out_row_stride, c->out_dtype, 0, c->bias, c->bias_dtype, c->flags, nullptr, 0};
-    st = launch_product<false>(a, true, dev, as_stream(stream));
+    st = launch_product<false>(a, true, *caps, as_stream(stream));
     return st != VY_OK ? st : check_launch("vy_int8_linear");
 }
 
@@ -284,6 +284,8 @@ extern "C" int vy_int8_gated_ffn(const vy_int8_ffn_call* c, void* stream) {
     if ((st = check_ffn(c)) != VY_OK) return st;
     const DeviceInfo* dev = device_info(&st);
     if (!dev) return st;
+    const ClusterCaps* caps = cluster_caps(&st);
+    if (!caps) return st;
     if (c->n_tokens == 0) return ok();
     cudaStream_t s = as_stream(stream);
     const FfnLayout L = ffn_layout(
@@ -296,7 +298,7 @@ extern "C" int vy_int8_gated_ffn(const vy_int8_ffn_call* c, void* stream) {
     d.col_scale[0] = c->down_scales;
     if (c->n_tokens <= kSourceTokens) {
         const int nk = (c->hidden + 127) / 128;
-        const int ctas = stream_ctas(2, t, 1, c->inter, nk, dev->sm_count);
+        const int ctas = stream_ctas(2, t, 1, c->inter, nk, *caps);
         EpiParams g{};
         g.out = L.h;
         g.ldo = c->inter;
@@ -307,26 +309,26 @@ extern "C" int vy_int8_gated_ffn(const vy_int8_ffn_call* c, void* stream) {
         const bool rows = c->n_tokens * c->hidden <= 16384 && aligned16(c->x) && (t == 1 || c->x_row_stride % 8 == 0);
         if (rows) {
             const StreamCall gate{c->w_gate, c->w_up, c->x, c->x_row_stride, t, 1, c->inter, c->hidden, false, L.maxima, ctas};
-            VY_TRY(c->act_dtype == VY_BF16 ? (stream_launch<EPI_I8GATE, VY_BF16, SRC_ROWS>(gate, g, c->flags, dev, s))
-                                           : (stream_launch<EPI_I8GATE, VY_F16, SRC_ROWS>(gate, g, c->flags, dev, s)));
+            VY_TRY(c->act_dtype == VY_BF16 ? (stream_launch<EPI_I8GATE, VY_BF16, SRC_ROWS>(gate, g, c->flags, *caps, s))
+                                           : (stream_launch<EPI_I8GATE, VY_F16, SRC_ROWS>(gate, g, c->flags, *caps, s)));
         } else {
             VY_TRY(launch_quantize(c->x, c->act_dtype, c->x_row_stride, c->n_tokens, c->hidden, L.x_codes, L.x_scales,
                                    dev->sm_count, s));
             g.row_scale = L.x_scales;
             const StreamCall gate{c->w_gate, c->w_up, L.x_codes, c->hidden, t, 1, c->inter, c->hidden, true, L.maxima, ctas};
-            VY_TRY((stream_launch<EPI_I8GATE, VY_BF16>(gate, g, c->flags, dev, s)));
+            VY_TRY((stream_launch<EPI_I8GATE, VY_BF16>(gate, g, c->flags, *caps, s)));
         }
         const StreamCall down{c->w_down, nullptr, L.h, c->inter, t, 1, c->hidden, c->inter, true, L.maxima, ctas};
-        VY_TRY((stream_launch<EPI_I8, VY_BF16, SRC_HIDDEN>(down, d, c->flags, dev, s)));
+        VY_TRY((stream_launch<EPI_I8, VY_BF16, SRC_HIDDEN>(down, d, c->flags, *caps, s)));
         return check_launch("vy_int8_gated_ffn");
     }
     VY_TRY(launch_quantize(c->x, c->act_dtype, c->x_row_stride, c->n_tokens, c->hidden, L.x_codes, L.x_scales, dev->sm_count, s));
     Product gu{L.x_codes, c->hidden, L.x_scales, {c->w_gate, c->w_up}, {c->gate_scales, c->up_scales}, c->n_tokens,
                c->hidden, c->inter, L.h, c->inter, VY_F32, c->activation, nullptr, 0, c->flags, nullptr, 0};
-    VY_TRY(launch_product<true>(gu, false, dev, s));
+    VY_TRY(launch_product<true>(gu, false, *caps, s));
     VY_TRY(launch_quantize(L.h, VY_F32, c->inter, c->n_tokens, c->inter, L.h_codes, L.h_scales, dev->sm_count, s));
     Product down{L.h_codes, c->inter, L.h_scales, {c->w_down, nullptr}, {c->down_scales, nullptr}, c->n_tokens, c->inter,
                  c->hidden, c->out, c->out_row_stride, c->act_dtype, 0, nullptr, 0, c->flags, nullptr, 0};
-    VY_TRY(launch_product<false>(down, false, dev, s));
+    VY_TRY(launch_product<false>(down, false, *caps, s));
     return check_launch("vy_int8_gated_ffn");
 }

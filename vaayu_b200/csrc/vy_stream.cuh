@@ -29,7 +29,9 @@ constexpr int kStreamRows = 128;        // weight rows of a unit (of each matrix
 constexpr int kStreamMaxTokens = 128;
 constexpr int kStreamThreads = 192;     // warps 0-3 read the sums, 4 loads, 5 issues the MMAs
 constexpr int kStreamMaxStages = 12;
-constexpr int kSmemMost = 225 * 1024, kSmemHalf = 111 * 1024;   // dynamic bytes of one CTA, of two on an SM
+// Weight bytes a CTA asks for in L2 before it waits for the kernel in front, behind what its ring holds
+// (37 x 7168 -> 2048, int8: 7.4 -> 6.9 us; more of it takes bandwidth from the kernel in front).
+constexpr int kStreamFetch = 64 * 1024;
 
 // Where the token tile comes from.
 enum Source {
@@ -248,8 +250,12 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(const __grid_con
             if (!kOwnCodes) tma_load_2d(ring + s * stage_bytes + NW * 16384, &p.x, (k_first + i) * kBlockK, 0, &S.full[s]);
         };
         const int ahead = p.early ? min(p.stages, nk) : 0;
-        if (elect_one())
+        if (elect_one()) {
             for (int i = 0; i < ahead; ++i) load_w(i, i);
+            const int fetch = min(nk, ahead + kStreamFetch / (NW * 16384));
+            for (int i = ahead; i < fetch; ++i)
+                for (int m = 0; m < NW; ++m) tma_prefetch_2d(&p.w[m], (k_first + i) * kBlockK, row0);
+        }
         __syncwarp();
         grid_dependency_wait();
         grid_dependents_launch();
@@ -393,17 +399,18 @@ struct StreamPlan {
 // memory.  Up to 32 tokens two stages a CTA are enough for that (16 x 7168 x 2048, bf16: 27.5 us
 // against 32.3 with one deep ring an SM); with more, the token tiles crowd the ring, and one CTA with
 // five stages is faster than two with two (64 x 4096 x 14336: 82 us against 99).
-inline StreamPlan stream_plan(int nw, int tokens, int parts, int n, int nk, int sm_count) {
+inline StreamPlan stream_plan(int nw, int tokens, int parts, int n, int nk, const ClusterCaps& caps) {
     const int units = (n + kStreamRows - 1) / kStreamRows;
     StreamPlan p{};
     p.stage = nw * 16384 + (tokens + 15) / 16 * 16 * 128;
-    for (p.splits = 8; p.splits >= 1; p.splits /= 2) {
+    for (int i = 3; i >= 0; --i) {
+        p.splits = 1 << i;
         p.sums = p.splits > 1 || parts > 1 ? (nw * tokens * kStreamRows * 4 + 1023) / 1024 * 1024 : 0;
         const int half = (kSmemHalf - 1024 - p.sums) / p.stage, whole = (kSmemMost - 1024 - p.sums) / p.stage;
         const bool two = half >= (tokens <= 32 ? 2 : 3);
         p.stages = two ? half : whole;
         if (p.splits == 1) break;
-        if (p.stages >= 2 && nk >= 2 * p.splits && units * p.splits <= (two ? 2 : 1) * sm_count) break;
+        if (p.stages >= 2 && nk >= 2 * p.splits && units <= (two ? caps.two : caps.one)[i]) break;
     }
     if (p.stages > kStreamMaxStages) p.stages = kStreamMaxStages;
     return p;
@@ -421,12 +428,12 @@ struct StreamCall {
 };
 
 // CTAs of a product's launch.
-inline int stream_ctas(int nw, int tokens, int parts, int n, int nk, int sm_count) {
-    return (n + kStreamRows - 1) / kStreamRows * stream_plan(nw, tokens, parts, n, nk, sm_count).splits;
+inline int stream_ctas(int nw, int tokens, int parts, int n, int nk, const ClusterCaps& caps) {
+    return (n + kStreamRows - 1) / kStreamRows * stream_plan(nw, tokens, parts, n, nk, caps).splits;
 }
 
 template <int EPI, int ACT, int SRC = SRC_TMA>
-int stream_launch(const StreamCall& a, const EpiParams& epi, int32_t* flags, const DeviceInfo* dev, cudaStream_t s) {
+int stream_launch(const StreamCall& a, const EpiParams& epi, int32_t* flags, const ClusterCaps& caps, cudaStream_t s) {
     constexpr bool I8 = epi_is_i8(EPI);
     constexpr int NW = epi_is_gate(EPI) ? 2 : 1;
     constexpr int block = I8 ? 128 : 64;
@@ -454,7 +461,7 @@ int stream_launch(const StreamCall& a, const EpiParams& epi, int32_t* flags, con
         p.rows_ld = a.x_ld;
         p.k = a.k;
     }
-    const StreamPlan plan = stream_plan(NW, a.tokens, a.parts, a.n, p.nk, dev->sm_count);
+    const StreamPlan plan = stream_plan(NW, a.tokens, a.parts, a.n, p.nk, caps);
     if (plan.stages < 2) return fail(VY_ERR_UNSUPPORTED, "dense stream: %d tokens", a.tokens);
     p.stages = plan.stages;
     p.sums_at = plan.stages * plan.stage;

@@ -478,9 +478,10 @@ inline int tile_operand(CUtensorMap* map, int dtype, const void* base, int64_t r
 }
 
 // Lays a launch's problems out (sizes and K blocks set): tile columns, tiles, K shares.  A gated
-// product's tile has bn / 2 output columns.  `pairs`: CTA pairs the device runs at once.
+// product's tile has bn / 2 output columns.
 constexpr int kShareLeast = 16;      // K blocks a pair's share is worth joining for
-inline void tile_layout(TileParams* p, bool gate, int pairs) {
+inline void tile_layout(TileParams* p, bool gate, const ClusterCaps& caps) {
+    const int pairs = caps.one[1];
     int least = 1 << 30, wide = 0;
     for (int i = 0; i < p->n_problems; ++i) {
         const TileProblem& q = p->prob[i];
@@ -489,7 +490,8 @@ inline void tile_layout(TileParams* p, bool gate, int pairs) {
         wide += (q.m + 255) / 256 * ((n + 255) / 256);
     }
     p->splits = 1;
-    while (p->splits < 4 && wide * p->splits * 2 <= pairs && least >= kShareLeast * p->splits * 2) p->splits *= 2;
+    // every tile's cluster is resident at once, and every share long enough
+    for (int i = 2; i < 4 && wide <= caps.one[i] && least >= kShareLeast << (i - 1); ++i) p->splits = 1 << (i - 1);
     const bool narrow = p->splits == 1 && wide * 2 <= pairs;
     p->n_tiles = 0;
     for (int i = 0; i < p->n_problems; ++i) {
@@ -521,7 +523,8 @@ inline TileProblem& tile_add(TileParams* p, int64_t m, int64_t n, int nk, int se
 }
 
 template <int EPI, int ACT>
-int tile_launch(const TileParams& p, int pairs, cudaStream_t s) {
+int tile_launch(const TileParams& p, const ClusterCaps& caps, cudaStream_t s) {
+    const int pairs = caps.one[1];
     auto kern = tile_kernel<EPI, ACT>;
     constexpr int smem = sizeof(TileSmem) + 1024;
     int st = once_per_device(reinterpret_cast<const void*>(kern), [](int, void* k) {

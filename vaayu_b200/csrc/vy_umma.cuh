@@ -115,6 +115,12 @@ __device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, v
     return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, err));
 }
 
+// Asks for a tile in L2.  L2 is where the writes of a kernel still running arrive too, so this is safe
+// before the wait on the kernel in front, whatever that one writes.
+__device__ __forceinline__ void tma_prefetch_2d(const CUtensorMap* map, int x, int y) {
+    asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(map), "r"(x), "r"(y) : "memory");
+}
+
 // ── tcgen05 on a CTA pair ───────────────────────────────────────────────────────────────────
 
 __device__ __forceinline__ uint32_t cluster_rank() {
