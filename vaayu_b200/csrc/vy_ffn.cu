@@ -86,9 +86,9 @@ int forward(const vy_ffn_call* c, const ClusterCaps& caps, cudaStream_t s) {
     d.ldo = c->out_row_stride;
     if (T <= kStreamMaxTokens) {
         const int t = static_cast<int>(T), parts = h_parts(c);
-        const StreamCall gate{c->w_gate, c->w_up, c->x, c->x_row_stride, t, 1, c->inter, c->hidden, false, nullptr, 0};
+        const StreamCall gate{c->w_gate, c->w_up, c->x, c->x_row_stride, t, 1, c->inter, c->hidden, false, nullptr, 0, nullptr};
         VY_TRY((stream_launch<EPI_GATE, ACT>(gate, e, c->flags, caps, s)));
-        const StreamCall down{c->w_down, nullptr, h, I, t * parts, parts, c->hidden, c->inter, true, nullptr, 0};
+        const StreamCall down{c->w_down, nullptr, h, I, t * parts, parts, c->hidden, c->inter, true, nullptr, 0, nullptr};
         return stream_launch<EPI_STORE, ACT>(down, d, c->flags, caps, s);
     }
     {
@@ -122,36 +122,49 @@ int backward(const vy_ffn_call* c, const ClusterCaps& caps, cudaStream_t s) {
     uint16_t* dg = reinterpret_cast<uint16_t*>(base);
     uint16_t* du = reinterpret_cast<uint16_t*>(base + each);
     uint16_t* h = reinterpret_cast<uint16_t*>(base + 2 * each);
-    {
+    const int t = static_cast<int>(T);
+    EpiParams e{};
+    e.act = c->activation;
+    e.saved = c->saved;
+    e.saved_bands = saved_bands(T);
+    e.part = part;
+    e.ldo = I;
+    e.dg = dg;
+    e.du = du;
+    e.h = h;
+    // dh streams Wd while its epilogue, a value at a time there, is short; d_x streams Wg and Wu as long
+    // as the forward call would
+    if (T <= kPartTokens) {
+        const StreamCall dh{c->w_down, nullptr, c->d_out, c->d_out_row_stride, t, 1, c->inter, c->hidden, false,
+                            nullptr, 0, nullptr};
+        VY_TRY((stream_launch<EPI_DGATE, ACT, SRC_TMA, true>(dh, e, c->flags, caps, s)));
+    } else {
         TileParams p{};
         TileProblem& q = tile_add(&p, T, I, k_blocks(H));
         tile_layout(&p, false, caps);
         q.b_mn = 1;
         VY_TRY(tile_operand(&q.a[0], ACT, c->d_out, T, H, c->d_out_row_stride, false, 128));
         VY_TRY(tile_operand(&q.b[0], ACT, c->w_down, I, H, I, true, 0));
-        q.epi.act = c->activation;
-        q.epi.saved = c->saved;
-        q.epi.saved_bands = saved_bands(T);
-        q.epi.part = part;
-        q.epi.ldo = I;
-        q.epi.dg = dg;
-        q.epi.du = du;
-        q.epi.h = h;
+        q.epi = e;
         p.flags = c->flags;
         VY_TRY((tile_launch<EPI_DGATE, ACT>(p, caps, s)));
     }
     TileParams p{};
     p.flags = c->flags;
-    if (c->d_x) {      // K segments: the parts of dg with Wg, those of du with Wu
-        TileProblem& q = tile_add(&p, T, H, k_blocks(I), 2 * parts);
+    if (c->d_x && T <= kStreamMaxTokens) {
+        EpiParams d{};
+        d.out = c->d_x;
+        d.ldo = c->d_x_row_stride;
+        const StreamCall dx{c->w_gate, c->w_up, dg, I, t * parts, parts, c->hidden, c->inter, true, nullptr, 0, du};
+        VY_TRY((stream_launch<EPI_STORE, ACT, SRC_TMA, true>(dx, d, c->flags, caps, s)));
+    } else if (c->d_x) {      // K segments: dg with Wg, du with Wu
+        TileProblem& q = tile_add(&p, T, H, k_blocks(I), 2);
         q.b_mn = 1;
-        for (int i = 0; i < 2 * parts; ++i) {
-            q.a_of[i] = static_cast<uint8_t>(i);
-            q.b_of[i] = static_cast<uint8_t>(i / parts);
-            VY_TRY(tile_operand(&q.a[i], ACT, (i / parts ? du : dg) + i % parts * part, T, I, I, false, 128));
+        for (int i = 0; i < 2; ++i) {
+            q.a_of[i] = q.b_of[i] = static_cast<uint8_t>(i);
+            VY_TRY(tile_operand(&q.a[i], ACT, i ? du : dg, T, I, I, false, 128));
+            VY_TRY(tile_operand(&q.b[i], ACT, i ? c->w_up : c->w_gate, H, I, H, true, 0));
         }
-        VY_TRY(tile_operand(&q.b[0], ACT, c->w_gate, H, I, H, true, 0));
-        VY_TRY(tile_operand(&q.b[1], ACT, c->w_up, H, I, H, true, 0));
         epi_store(&q, c->d_x, c->d_x_row_stride);
     }
     struct Grad {

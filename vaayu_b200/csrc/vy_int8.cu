@@ -153,7 +153,7 @@ int launch_product(const Product& a, bool first, const ClusterCaps& caps, cudaSt
     constexpr int EPI = GATE ? EPI_I8GATE : EPI_I8;
     if (a.tokens <= kStreamMaxTokens) {
         const StreamCall c{a.w[0], a.w[1], a.codes, a.codes_ld, static_cast<int>(a.tokens), 1, a.n, a.k, !first,
-                           a.maxima, a.n_maxima};
+                           a.maxima, a.n_maxima, nullptr};
         return stream_launch<EPI, VY_BF16>(c, e, a.flags, caps, s);
     }
     TileParams p{};
@@ -308,17 +308,17 @@ extern "C" int vy_int8_gated_ffn(const vy_int8_ffn_call* c, void* stream) {
         // the rows' maxima taken in every CTA: worth a launch while a row set is small (32 KB)
         const bool rows = c->n_tokens * c->hidden <= 16384 && aligned16(c->x) && (t == 1 || c->x_row_stride % 8 == 0);
         if (rows) {
-            const StreamCall gate{c->w_gate, c->w_up, c->x, c->x_row_stride, t, 1, c->inter, c->hidden, false, L.maxima, ctas};
+            const StreamCall gate{c->w_gate, c->w_up, c->x, c->x_row_stride, t, 1, c->inter, c->hidden, false, L.maxima, ctas, nullptr};
             VY_TRY(c->act_dtype == VY_BF16 ? (stream_launch<EPI_I8GATE, VY_BF16, SRC_ROWS>(gate, g, c->flags, *caps, s))
                                            : (stream_launch<EPI_I8GATE, VY_F16, SRC_ROWS>(gate, g, c->flags, *caps, s)));
         } else {
             VY_TRY(launch_quantize(c->x, c->act_dtype, c->x_row_stride, c->n_tokens, c->hidden, L.x_codes, L.x_scales,
                                    dev->sm_count, s));
             g.row_scale = L.x_scales;
-            const StreamCall gate{c->w_gate, c->w_up, L.x_codes, c->hidden, t, 1, c->inter, c->hidden, true, L.maxima, ctas};
+            const StreamCall gate{c->w_gate, c->w_up, L.x_codes, c->hidden, t, 1, c->inter, c->hidden, true, L.maxima, ctas, nullptr};
             VY_TRY((stream_launch<EPI_I8GATE, VY_BF16>(gate, g, c->flags, *caps, s)));
         }
-        const StreamCall down{c->w_down, nullptr, L.h, c->inter, t, 1, c->hidden, c->inter, true, L.maxima, ctas};
+        const StreamCall down{c->w_down, nullptr, L.h, c->inter, t, 1, c->hidden, c->inter, true, L.maxima, ctas, nullptr};
         VY_TRY((stream_launch<EPI_I8, VY_BF16, SRC_HIDDEN>(down, d, c->flags, *caps, s)));
         return check_launch("vy_int8_gated_ffn");
     }

@@ -10,6 +10,9 @@
 // barrier each CTA adds its slice over all shares, in rank order.  No workspace, no atomics, one
 // order of summation, and no remote read to wait for.
 //
+// The backward products read the same weights across their rows: there the weight tile is MN-major
+// ([K, N] in memory), and d_x takes its K from two tensor pairs (dg with Wg, du with Wu).
+//
 // With up to 16 tokens the int8 block needs no quantisation kernels (Source): the four warps that read
 // the sums at the end are idle until then and write the token tile's codes themselves, a 16-value
 // piece of a token each per K block, from rows that are still floats.  The rows' largest magnitudes
@@ -42,8 +45,9 @@ enum Source {
 constexpr int kSourceTokens = 16;      // 8 pieces of a K block each, one per thread of four warps
 
 struct StreamParams {
-    CUtensorMap w[2], x;
+    CUtensorMap w[2], x[2]; // of a gated product gate and up, else of the K segments
     int tokens, n, nk;      // rows of x; nk: K blocks of 128 bytes
+    int segment;            // K blocks of the first segment (nk when there is one)
     int cols;               // MMA N: tokens rounded up to 16
     int stages, tmem_cols;
     int sums_at;            // offset of the received sums in dynamic shared memory
@@ -91,7 +95,19 @@ __device__ __forceinline__ void stream_put(const StreamParams& p, int row, int t
                                            const ColumnScale& cs, const float* token_scale, uint32_t* token_top) {
     const EpiParams& e = p.epi;
     const int64_t at = int64_t(t) * e.ldo + row;
-    if constexpr (EPI == EPI_GATE) {
+    if constexpr (EPI == EPI_DGATE) {
+        const float dh = __uint_as_float(s0);
+        const float* s = e.saved + saved_at(e.saved_bands, t, row);
+        const float g = s[0], u = s[kSavedBlock / 2];
+        const float2 a = gate_act_grad(g, e.act);
+        const float v[3] = {dh * u * a.y, dh * a.x, a.x * u};
+        uint16_t* const to[3] = {e.dg, e.du, e.h};
+#pragma unroll
+        for (int i = 0; i < 3; ++i) {
+            to[i][at] = static_cast<uint16_t>(act_bits<ACT>(v[i]));
+            if (e.part) to[i][at + e.part] = static_cast<uint16_t>(act_bits<ACT>(low_part<ACT>(v[i])));
+        }
+    } else if constexpr (EPI == EPI_GATE) {
         const float g = __uint_as_float(s0), u = __uint_as_float(s1);
         const float h = gate_act(g, e.act) * u;
         reinterpret_cast<uint16_t*>(e.out)[at] = static_cast<uint16_t>(act_bits<ACT>(h));
@@ -147,7 +163,7 @@ struct RowPiece {
     }
 };
 
-template <int EPI, int ACT, int SRC>
+template <int EPI, int ACT, int SRC, bool MN>
 __global__ void __launch_bounds__(kStreamThreads) stream_kernel(const __grid_constant__ StreamParams p) {
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     __shared__ StreamBars S;
@@ -178,8 +194,8 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(const __grid_con
     }
     if (warp == 4 && lane == 0) {
         prefetch_map(&p.w[0]);
-        if (NW == 2) prefetch_map(&p.w[1]);
-        if (!kOwnCodes) prefetch_map(&p.x);
+        if (NW == 2 || MN) prefetch_map(&p.w[1]);
+        if (!kOwnCodes) prefetch_map(&p.x[0]);
     }
     if (warp == 0) tmem_alloc_n<0>(&S.tmem_base, p.tmem_cols);
     tc_fence_before();
@@ -240,20 +256,29 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(const __grid_con
     }
     if (warp == 4) {
         auto load_w = [&](int i, uint32_t s) {
-            const int k = (k_first + i) * kBlockK;
             unsigned char* at = ring + s * stage_bytes;
             mbar_expect_tx(&S.full[s], kOwnCodes ? NW * 16384u : stage_bytes);
-            tma_load_2d(at, &p.w[0], k, row0, &S.full[s]);
-            if (NW == 2) tma_load_2d(at + 16384, &p.w[1], k, row0, &S.full[s]);
+            if constexpr (MN) {
+                const int kb = k_first + i, seg = kb >= p.segment, k = (kb - (seg ? p.segment : 0)) * kBlockK;
+                tma_load_2d(at, &p.w[seg], row0, k, &S.full[s]);
+                tma_load_2d(at + 8192, &p.w[seg], row0 + 64, k, &S.full[s]);
+            } else {
+                const int k = (k_first + i) * kBlockK;
+                tma_load_2d(at, &p.w[0], k, row0, &S.full[s]);
+                if (NW == 2) tma_load_2d(at + 16384, &p.w[1], k, row0, &S.full[s]);
+            }
         };
         auto load_x = [&](int i, uint32_t s) {
-            if (!kOwnCodes) tma_load_2d(ring + s * stage_bytes + NW * 16384, &p.x, (k_first + i) * kBlockK, 0, &S.full[s]);
+            const int kb = k_first + i, seg = MN && kb >= p.segment;
+            if (!kOwnCodes)
+                tma_load_2d(ring + s * stage_bytes + NW * 16384, &p.x[seg], (kb - (seg ? p.segment : 0)) * kBlockK, 0,
+                            &S.full[s]);
         };
         const int ahead = p.early ? min(p.stages, nk) : 0;
         if (elect_one()) {
             for (int i = 0; i < ahead; ++i) load_w(i, i);
             const int fetch = min(nk, ahead + kStreamFetch / (NW * 16384));
-            for (int i = ahead; i < fetch; ++i)
+            for (int i = ahead; i < fetch && !MN; ++i)
                 for (int m = 0; m < NW; ++m) tma_prefetch_2d(&p.w[m], (k_first + i) * kBlockK, row0);
         }
         __syncwarp();
@@ -277,19 +302,21 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(const __grid_con
         if (lane == 0)
             for (int j = max(0, i - p.stages); j < i; ++j) mbar_drain(&S.empty[j % p.stages], (j / p.stages) & 1, p.flags);
     } else if (warp == 5) {
-        const uint32_t idesc = umma_idesc(I8, ACT == VY_BF16, 0, 0, kStreamRows, p.cols);
-        const uint64_t first = umma_desc(smem_u32(ring), 16, 1024);
+        const uint32_t idesc = umma_idesc(I8, ACT == VY_BF16, MN, 0, kStreamRows, p.cols);
+        const uint64_t first = umma_desc(smem_u32(ring), MN ? 8192 : 16, 1024);
+        const uint64_t first_x = umma_desc(smem_u32(ring), 16, 1024) + NW * 1024;
+        constexpr uint32_t w_step = MN ? 128 : 2;      // one MMA's K: 16 rows of 128 bytes, or 32 bytes of a row
         uint32_t stage = 0, phase = 0;
         for (int i = 0; i < nk; ++i) {
             if (!mbar_wait_warp(&S.full[stage], phase, abort_flag, p.flags)) break;
             tc_fence_after();
             if (elect_one()) {
-                const uint64_t dw = first + (stage * stage_bytes >> 4), dx = dw + NW * 1024;
+                const uint64_t dw = first + (stage * stage_bytes >> 4), dx = first_x + (stage * stage_bytes >> 4);
 #pragma unroll
                 for (int m = 0; m < NW; ++m)
 #pragma unroll
                     for (int k = 0; k < 4; ++k)
-                        mma_ss<I8, 0>(tmem + m * p.cols, dw + m * 1024 + 2 * k, dx + 2 * k, idesc, i != 0 || k != 0);
+                        mma_ss<I8, 0>(tmem + m * p.cols, dw + m * 1024 + w_step * k, dx + 2 * k, idesc, i != 0 || k != 0);
                 mma_commit_one(&S.empty[stage]);
                 if (i == nk - 1) mma_commit_one(&S.done);
             }
@@ -418,13 +445,14 @@ inline StreamPlan stream_plan(int nw, int tokens, int parts, int n, int nk, cons
 
 // One product: its weight matrices [n, k] (contiguous) and its token rows.
 struct StreamCall {
-    const void *w0, *w1;      // w1: the up matrix of a gated product
+    const void *w0, *w1;      // w1: the up matrix of a gated product, or (MN) the second K segment's, or null
     const void* x;            // [tokens, k]; parts == 2: high parts, then low parts of tokens / 2 rows
     int64_t x_ld;
     int tokens, parts, n, k;
     bool early;               // a kernel of the same call runs in front of this one
     uint32_t* maxima;         // see StreamParams
     int n_maxima;
+    const void* x1;           // (MN) the second K segment's tokens
 };
 
 // CTAs of a product's launch.
@@ -432,7 +460,8 @@ inline int stream_ctas(int nw, int tokens, int parts, int n, int nk, const Clust
     return (n + kStreamRows - 1) / kStreamRows * stream_plan(nw, tokens, parts, n, nk, caps).splits;
 }
 
-template <int EPI, int ACT, int SRC = SRC_TMA>
+// MN: the weights are [k, n] in memory; k is that of one segment.
+template <int EPI, int ACT, int SRC = SRC_TMA, bool MN = false>
 int stream_launch(const StreamCall& a, const EpiParams& epi, int32_t* flags, const ClusterCaps& caps, cudaStream_t s) {
     constexpr bool I8 = epi_is_i8(EPI);
     constexpr int NW = epi_is_gate(EPI) ? 2 : 1;
@@ -441,7 +470,8 @@ int stream_launch(const StreamCall& a, const EpiParams& epi, int32_t* flags, con
     StreamParams p{};
     p.tokens = a.tokens;
     p.n = a.n;
-    p.nk = (a.k + block - 1) / block;
+    p.segment = (a.k + block - 1) / block;
+    p.nk = MN && a.w1 ? 2 * p.segment : p.segment;
     p.cols = (a.tokens + 15) / 16 * 16;
     p.early = a.early;
     p.parts = a.parts;
@@ -452,10 +482,15 @@ int stream_launch(const StreamCall& a, const EpiParams& epi, int32_t* flags, con
     p.tmem_cols = 32;
     while (p.tmem_cols < NW * p.cols) p.tmem_cols *= 2;
     int st;
-    if ((st = make_map_2d(&p.w[0], dtype, a.w0, a.n, a.k, a.k, block, kStreamRows)) != VY_OK) return st;
-    if (NW == 2 && (st = make_map_2d(&p.w[1], dtype, a.w1, a.n, a.k, a.k, block, kStreamRows)) != VY_OK) return st;
+    const void* const w[2] = {a.w0, a.w1};
+    for (int i = 0; i < 2 && w[i]; ++i) {
+        st = MN ? make_map_2d(&p.w[i], dtype, w[i], a.k, a.n, a.n, 64, 64)
+                : make_map_2d(&p.w[i], dtype, w[i], a.n, a.k, a.k, block, kStreamRows);
+        if (st != VY_OK) return st;
+    }
     if (SRC == SRC_TMA) {
-        if ((st = make_map_2d(&p.x, dtype, a.x, a.tokens, a.k, a.x_ld, block, p.cols)) != VY_OK) return st;
+        if ((st = make_map_2d(&p.x[0], dtype, a.x, a.tokens, a.k, a.x_ld, block, p.cols)) != VY_OK) return st;
+        if (a.x1 && (st = make_map_2d(&p.x[1], dtype, a.x1, a.tokens, a.k, a.x_ld, block, p.cols)) != VY_OK) return st;
     } else {
         p.rows = a.x;
         p.rows_ld = a.x_ld;
@@ -466,7 +501,7 @@ int stream_launch(const StreamCall& a, const EpiParams& epi, int32_t* flags, con
     p.stages = plan.stages;
     p.sums_at = plan.stages * plan.stage;
     const int bytes = p.sums_at + plan.sums + 1024;
-    auto kern = stream_kernel<EPI, ACT, SRC>;
+    auto kern = stream_kernel<EPI, ACT, SRC, MN>;
     st = once_per_device(reinterpret_cast<const void*>(kern), [](int, void* f) {
         const cudaError_t e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMost);
         return e == cudaSuccess ? VY_OK : fail(VY_ERR_CUDA, "dense stream shared memory: %s", cudaGetErrorString(e));
