@@ -57,9 +57,10 @@ int check_ffn(const vy_ffn_call* c, bool backward) {
     return VY_OK;
 }
 
-void epi_store(TileProblem* q, void* out, int64_t ldo) {
+int epi_store(TileProblem* q, int act_dtype, void* out, int64_t ldo) {
     q->epi.out = out;
     q->epi.ldo = ldo;
+    return make_map_2d(&q->out, act_dtype, out, q->m, q->n, ldo, 64, 32);
 }
 
 #define VY_TRY(expr)                         \
@@ -107,7 +108,7 @@ int forward(const vy_ffn_call* c, const ClusterCaps& caps, cudaStream_t s) {
     tile_layout(&p, false, caps);
     VY_TRY(tile_operand(&q.a[0], ACT, h, T, I, I, false, 128));
     VY_TRY(tile_operand(&q.b[0], ACT, c->w_down, H, I, I, false, q.bn / 2));
-    q.epi = d;
+    VY_TRY(epi_store(&q, ACT, c->out, c->out_row_stride));
     p.flags = c->flags;
     return tile_launch<EPI_STORE, ACT>(p, caps, s);
 }
@@ -165,7 +166,7 @@ int backward(const vy_ffn_call* c, const ClusterCaps& caps, cudaStream_t s) {
             VY_TRY(tile_operand(&q.a[i], ACT, i ? du : dg, T, I, I, false, 128));
             VY_TRY(tile_operand(&q.b[i], ACT, i ? c->w_up : c->w_gate, H, I, H, true, 0));
         }
-        epi_store(&q, c->d_x, c->d_x_row_stride);
+        VY_TRY(epi_store(&q, ACT, c->d_x, c->d_x_row_stride));
     }
     struct Grad {
         void* out;
@@ -189,7 +190,7 @@ int backward(const vy_ffn_call* c, const ClusterCaps& caps, cudaStream_t s) {
             if (i == 0 || g.b_parts)
                 VY_TRY(tile_operand(&q.b[i], ACT, static_cast<const uint16_t*>(g.b) + at, g.n, T, g.ldb, true, 0));
         }
-        epi_store(&q, g.out, g.n);
+        VY_TRY(epi_store(&q, ACT, g.out, g.n));
     }
     if (p.n_problems == 0) return VY_OK;
     tile_layout(&p, false, caps);

@@ -26,12 +26,12 @@
 namespace vy {
 
 constexpr int kTileThreads = 384;
-constexpr int kTileStages = 6;
 constexpr int kTileProblems = 4;
 constexpr int kHalfBytes = 128 * 128;          // one operand's share of a stage: 128 rows x 128 bytes
 constexpr uint32_t kTileTmemCols = 512;
 
 struct TileProblem {
+    CUtensorMap out;             // EPI_STORE: the output in 32 x 64 tiles
     CUtensorMap a[4], b[2];      // operands of the K segments (a gated product: b is gate, up)
     int m, n;                    // rows, output columns
     int nk[4];                   // K blocks of each segment
@@ -50,9 +50,13 @@ struct TileParams {
     int32_t* flags;
 };
 
+// A plain product's epilogue needs 32 KB to lay its rows out for TMA stores; the others store directly.
+template <int EPI>
 struct __align__(1024) TileSmem {
+    static constexpr int kTileStages = EPI == EPI_STORE ? 5 : 6;
     unsigned char a[kTileStages][kHalfBytes];
     unsigned char b[kTileStages][kHalfBytes];
+    unsigned char rows[EPI == EPI_STORE ? 8 : 1][EPI == EPI_STORE ? 4096 : 16];
     uint64_t full[kTileStages], empty[kTileStages];
     uint64_t acc_full[2], acc_empty[2];
     float cols[8][2][128];       // int8: an epilogue warp's column scales (gate, up) or scale and bias
@@ -283,10 +287,47 @@ __device__ __forceinline__ void dgate_epilogue(const TileProblem& q, GateChunk& 
     }
 }
 
+// A warp's 32 rows x columns [c0, c1) of a tile, 64 columns at a time: packed into shared memory in the
+// 128-byte swizzle and written by TMA, whole 128-byte lines.  (Storing 32 bytes of each row directly
+// takes the load/store unit 32 lines an instruction, 5 us a tile, which the MMAs of a weight gradient
+// over few tokens do not hide: 190 us for three of 4096 x 14336 over 16 tokens, 103 this way.)
+template <int ACT>
+__device__ __forceinline__ void store_rows(const TileProblem& q, unsigned char* rows, int row0, int col0, uint32_t tmem,
+                                           int c0, int c1) {
+    const int lane = threadIdx.x & 31;
+    for (int c = c0; c < c1; c += 64) {
+        if (lane == 0) tma_store_wait_read();
+        __syncwarp();
+#pragma unroll
+        for (int k = 0; k < 4; k += 2) {
+            uint32_t r[2][16];
+            tmem_ld16(tmem + c + 16 * k, r[0]);
+            tmem_ld16(tmem + c + 16 * k + 16, r[1]);
+            tmem_wait16(r[0]);
+            tmem_wait16(r[1]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t* v = &r[i / 2][8 * (i & 1)];
+                uint4 o;
+                o.x = pack_act<ACT>(__uint_as_float(v[0]), __uint_as_float(v[1]));
+                o.y = pack_act<ACT>(__uint_as_float(v[2]), __uint_as_float(v[3]));
+                o.z = pack_act<ACT>(__uint_as_float(v[4]), __uint_as_float(v[5]));
+                o.w = pack_act<ACT>(__uint_as_float(v[6]), __uint_as_float(v[7]));
+                *reinterpret_cast<uint4*>(rows + lane * 128 + (((2 * k + i) ^ (lane & 7)) << 4)) = o;
+            }
+        }
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0 && row0 < q.m && col0 + c < q.n) tma_store_2d(&q.out, col0 + c, row0, rows);
+    }
+}
+
 template <int EPI, int ACT>
 __global__ void __launch_bounds__(kTileThreads, 1) tile_kernel(const __grid_constant__ TileParams p) {
     extern __shared__ __align__(1024) unsigned char smem_raw[];
-    TileSmem& S = *reinterpret_cast<TileSmem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    using Smem = TileSmem<EPI>;
+    constexpr int kTileStages = Smem::kTileStages;
+    Smem& S = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     constexpr bool I8 = epi_is_i8(EPI);
     constexpr int kBlockK = I8 ? 128 : 64;      // elements of a 128-byte K block
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -420,12 +461,15 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_kernel(const __grid_cons
             tc_fence_after();
             if constexpr (EPI == EPI_DGATE)
                 dgate_epilogue<ACT>(q, first, row, t.n, sums, c0, c1);
+            else if constexpr (EPI == EPI_STORE)
+                store_rows<ACT>(q, S.rows[warp & 7], row - lane, t.n * q.bn, sums.tmem, c0, c1);
             else
                 tile_epilogue<EPI, ACT>(q, row, t.n, sums, c0, c1, rs, S.cols[warp & 7]);
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive_remote(map_to_rank(smem_u32(&S.acc_empty[buf]), leader));
         }
+        if (EPI == EPI_STORE && lane == 0) tma_store_wait();
     }
     if (splits > 1) {
         // one tile a cluster: send, meet, add my columns
@@ -526,7 +570,7 @@ template <int EPI, int ACT>
 int tile_launch(const TileParams& p, const ClusterCaps& caps, cudaStream_t s) {
     const int pairs = caps.one[1];
     auto kern = tile_kernel<EPI, ACT>;
-    constexpr int smem = sizeof(TileSmem) + 1024;
+    constexpr int smem = sizeof(TileSmem<EPI>) + 1024;
     int st = once_per_device(reinterpret_cast<const void*>(kern), [](int, void* k) {
         const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
         return e == cudaSuccess ? VY_OK : fail(VY_ERR_CUDA, "dense GEMM shared memory: %s", cudaGetErrorString(e));

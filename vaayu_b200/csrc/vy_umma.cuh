@@ -121,6 +121,17 @@ __device__ __forceinline__ void tma_prefetch_2d(const CUtensorMap* map, int x, i
     asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(map), "r"(x), "r"(y) : "memory");
 }
 
+// A 2D tile from shared memory (what lies outside the matrix is not written), the calling thread's
+// bulk group, and its waits: until shared memory has been read, or until all is written.
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, int x, int y, const void* src) {
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(map), "r"(x), "r"(y),
+                 "r"(smem_u32(src))
+                 : "memory");
+    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+__device__ __forceinline__ void tma_store_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+__device__ __forceinline__ void tma_store_wait() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+
 // ── tcgen05 on a CTA pair ───────────────────────────────────────────────────────────────────
 
 __device__ __forceinline__ uint32_t cluster_rank() {
