@@ -460,12 +460,8 @@ typedef struct vy_int8_linear_call {
     int32_t out_dtype;         /* VY_BF16 / VY_F16 / VY_F32 */
     void* out;                 /* [n_tokens, n] */
     int64_t out_row_stride;
-    void* workspace;           /* vy_int8_linear_workspace_size() */
-    size_t workspace_bytes;
     int32_t* flags;
 } vy_int8_linear_call;
-
-size_t vy_int8_linear_workspace_size(const vy_int8_linear_call* call);
 
 /*
  * out[t, n] = (sum_k codes[t, k] * weight[n, k]) * scales[t] * weight_scales[n] (+ bias[n]): the

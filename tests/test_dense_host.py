@@ -148,7 +148,6 @@ def test_int8_linear_entry_point_refuses(field, value, status):
     c.n_tokens, c.k, c.n = 3, 64, 5
     c.codes, c.codes_row_stride, c.scales, c.weight, c.weight_scales = A, 64, A, A, A
     c.out_dtype, c.out, c.out_row_stride = _lib.BF16, A, 5
-    c.workspace, c.workspace_bytes = A, 1 << 30
     setattr(c, field, value)
     assert lib.vy_int8_linear(ctypes.byref(c), None) == status
 

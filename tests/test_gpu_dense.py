@@ -385,16 +385,18 @@ def test_int8_gated_ffn(tokens, hidden, inter, dtype, act):
     R.assert_within(y, want, bound, "y")
 
 
-def test_int8_gated_ffn_layouts_and_capture():
-    ops, _ = make(24, 272, 144, BF16)
+@pytest.mark.parametrize("tokens", [1, 12, 24, 300])
+def test_int8_gated_ffn_layouts_and_capture(tokens):
+    ops, _ = make(tokens, 272, 144, BF16)
     x = ops[0]
     q = [t for w in ops[1:] for t in vb.quantize_int8(w)]
     want = vb.int8_gated_ffn(x, *q)
-    wide = torch.zeros(24, 301, dtype=BF16, device="cuda")
-    wide[:, 5:277] = x
-    assert torch.equal(vb.int8_gated_ffn(wide[:, 5:277], *q), want)
-    out = torch.full((24, 275), 2.0, dtype=BF16, device="cuda")
-    vb.int8_gated_ffn(x.view(24, 272), *q, out=out[:, :272])
+    wide = torch.zeros(tokens, 301, dtype=BF16, device="cuda")
+    for at in (5, 8):
+        wide[:, at:at + 272] = x
+        assert torch.equal(vb.int8_gated_ffn(wide[:, at:at + 272], *q), want)
+    out = torch.full((tokens, 275), 2.0, dtype=BF16, device="cuda")
+    vb.int8_gated_ffn(x.view(tokens, 272), *q, out=out[:, :272])
     assert torch.equal(out[:, :272], want) and (out[:, 272:] == 2).all()
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
@@ -405,11 +407,60 @@ def test_int8_gated_ffn_layouts_and_capture():
     for g in graphs:
         with torch.cuda.graph(g):
             outs.append(vb.int8_gated_ffn(x, *q))
-    x.copy_(make(24, 272, 144, BF16, seed=5)[0][0])
+    x.copy_(make(tokens, 272, 144, BF16, seed=5)[0][0])
     for g in graphs:
         g.replay()
     want = vb.int8_gated_ffn(x, *q)
     assert all(torch.equal(o, want) for o in outs)
+
+
+@pytest.mark.parametrize("tokens", [2, 9, 40, 300])
+def test_int8_gated_ffn_odd_rows_stay_alone(tokens):
+    """A zero row gives zeros, a row with a NaN or an infinity NaN, and no other row changes."""
+    ops, _ = make(tokens, 272, 144, BF16)
+    q = [t for w in ops[1:] for t in vb.quantize_int8(w)]
+    want = vb.int8_gated_ffn(ops[0], *q)
+    for bad in (0.0, float("nan"), -float("inf")):
+        x = ops[0].clone()
+        x[1] = 0.0
+        x[1, 7] = bad
+        y = vb.int8_gated_ffn(x, *q)
+        keep = torch.arange(tokens, device="cuda") != 1
+        assert torch.equal(y[keep], want[keep])
+        assert (y[1] == 0).all() if bad == 0.0 else torch.isnan(y[1]).all()
+
+
+@pytest.mark.parametrize("tokens", [3, 100, 400])
+def test_two_streams_at_once(tokens):
+    ops, _ = make(tokens, 1040, 528, BF16)
+    q = [t for w in ops[1:] for t in vb.quantize_int8(w)]
+    codes, scale = vb.quantize_int8(ops[0])
+
+    def calls():
+        return vb.gated_ffn(*ops), vb.int8_gated_ffn(ops[0], *q), vb.int8_linear(codes, scale, q[0], q[1])
+
+    want = calls()
+    torch.cuda.synchronize()
+    streams, results = [torch.cuda.Stream() for _ in range(2)], []
+    for _ in range(5):
+        for s in streams:
+            with torch.cuda.stream(s):
+                results.append(calls())
+    torch.cuda.synchronize()
+    for got in results:
+        assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
+@pytest.mark.skipif("torch.cuda.device_count() < 2")
+def test_a_device_that_is_not_current():
+    ops, dy = make(40, 256, 136, BF16, grad=True)
+    there = [t.detach().to("cuda:1").requires_grad_(True) for t in ops]
+    y, z = vb.gated_ffn(*ops), vb.gated_ffn(*there)
+    assert torch.equal(y.cpu(), z.cpu())
+    for a, b in zip(torch.autograd.grad(y, ops, dy), torch.autograd.grad(z, there, dy.to("cuda:1"))):
+        assert torch.equal(a.cpu(), b.cpu())
+    with pytest.raises(RuntimeError, match="tensors on"):
+        vb.gated_ffn(ops[0], *there[1:])
 
 
 # ── together ─────────────────────────────────────────────────────────────────────────────────

@@ -56,8 +56,7 @@ class Int8LinearCall(ctypes.Structure):
     """vy_int8_linear_call."""
     _fields_ = [("n_tokens", I64T), ("k", I32T), ("n", I32T), ("codes", P), ("codes_row_stride", I64T),
                 ("scales", P), ("weight", P), ("weight_scales", P), ("bias", P), ("bias_dtype", I32T),
-                ("out_dtype", I32T), ("out", P), ("out_row_stride", I64T), ("workspace", P),
-                ("workspace_bytes", SZ), ("flags", P)]
+                ("out_dtype", I32T), ("out", P), ("out_row_stride", I64T), ("flags", P)]
 
 
 class Int8FfnCall(ctypes.Structure):
@@ -98,7 +97,6 @@ SIGNATURES = {
     "vy_gated_ffn_forward": (ctypes.c_int, [P, P]),
     "vy_gated_ffn_backward": (ctypes.c_int, [P, P]),
     "vy_int8_quantize": (ctypes.c_int, [P, I32T, I64T, I64T, I64T, P, P, P]),
-    "vy_int8_linear_workspace_size": (SZ, [P]),
     "vy_int8_linear": (ctypes.c_int, [P, P]),
     "vy_int8_gated_ffn_workspace_size": (SZ, [P]),
     "vy_int8_gated_ffn": (ctypes.c_int, [P, P]),

@@ -183,9 +183,6 @@ int check_linear(const vy_int8_linear_call* c) {
         return fail(VY_ERR_ALIGNMENT, "codes and weight must have 16-byte aligned rows (row stride %lld)",
                     (long long)c->codes_row_stride);
     if (c->out_row_stride < c->n) return fail(VY_ERR_INVALID, "out row stride %lld", (long long)c->out_row_stride);
-    const size_t bytes = vy_int8_linear_workspace_size(c);
-    if (bytes && (!c->workspace || c->workspace_bytes < bytes))
-        return fail(VY_ERR_WORKSPACE, "workspace %zu bytes, %zu needed", c->workspace_bytes, bytes);
     return VY_OK;
 }
 
@@ -258,8 +255,6 @@ extern "C" int vy_int8_quantize(const void* x, int32_t x_dtype, int64_t x_row_st
     st = launch_quantize(x, x_dtype, x_row_stride, rows, cols, codes, scales, dev->sm_count, as_stream(stream));
     return st != VY_OK ? st : check_launch("vy_int8_quantize");
 }
-
-extern "C" size_t vy_int8_linear_workspace_size(const vy_int8_linear_call*) { return 0; }
 
 extern "C" int vy_int8_linear(const vy_int8_linear_call* c, void* stream) {
     int st;

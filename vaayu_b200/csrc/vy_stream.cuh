@@ -194,7 +194,7 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(const __grid_con
     }
     if (warp == 4 && lane == 0) {
         prefetch_map(&p.w[0]);
-        if (NW == 2 || MN) prefetch_map(&p.w[1]);
+        if (NW == 2 || p.segment < p.nk) prefetch_map(&p.w[1]);
         if (!kOwnCodes) prefetch_map(&p.x[0]);
     }
     if (warp == 0) tmem_alloc_n<0>(&S.tmem_base, p.tmem_cols);

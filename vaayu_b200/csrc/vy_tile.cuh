@@ -32,10 +32,10 @@ constexpr uint32_t kTileTmemCols = 512;
 
 struct TileProblem {
     CUtensorMap out;             // EPI_STORE: the output in 32 x 64 tiles
-    CUtensorMap a[4], b[2];      // operands of the K segments (a gated product: b is gate, up)
+    CUtensorMap a[2], b[2];      // operands of the K segments (a gated product: b is gate, up)
     int m, n;                    // rows, output columns
-    int nk[4];                   // K blocks of each segment
-    uint8_t a_of[4], b_of[4];    // each segment's operands
+    int nk[2];                   // K blocks of each segment
+    uint8_t a_of[2], b_of[2];    // each segment's operands
     int a_mn, b_mn;              // 1: that operand is MN-major (memory [K, M] / [K, N])
     int bn;                      // tile columns, 256 or 128
     int m_tiles, n_tiles, first; // tiles [first, first + m_tiles * n_tiles)
@@ -64,7 +64,7 @@ struct __align__(1024) TileSmem {
     int abort_flag;
 };
 
-__host__ __device__ __forceinline__ int k_total(const TileProblem& q) { return q.nk[0] + q.nk[1] + q.nk[2] + q.nk[3]; }
+__host__ __device__ __forceinline__ int k_total(const TileProblem& q) { return q.nk[0] + q.nk[1]; }
 
 // A pair's tiles: first, first + pairs, ...  When the first problem's tiles are long ones (dx: its K is
 // both halves' channels), they come first, n_long of them, and the pairs that get one fewer of them
@@ -273,17 +273,6 @@ __device__ __forceinline__ void dgate_epilogue(const TileProblem& q, GateChunk& 
         store16<ACT>(e.dg + at, dg, valid);
         store16<ACT>(e.du + at, du, valid);
         store16<ACT>(e.h + at, h, valid);
-        if (e.part) {
-#pragma unroll
-            for (int j = 0; j < 16; ++j) {
-                dg[j] = low_part<ACT>(dg[j]);
-                du[j] = low_part<ACT>(du[j]);
-                h[j] = low_part<ACT>(h[j]);
-            }
-            store16<ACT>(e.dg + at + e.part, dg, valid);
-            store16<ACT>(e.du + at + e.part, du, valid);
-            store16<ACT>(e.h + at + e.part, h, valid);
-        }
     }
 }
 
@@ -368,7 +357,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_kernel(const __grid_cons
             const int n0 = epi_is_gate(EPI) ? t.n * (q.bn / 2) : t.n * q.bn + int(rank) * (q.bn / 2);
             const uint32_t bytes = 2u * (kHalfBytes + uint32_t(q.bn) * 64u);
             const int nk = k_total(q), k_first = nk * share / splits, k_last = nk * (share + 1) / splits;
-            for (int seg = 0, before = 0; go && seg < 4; before += q.nk[seg++]) {
+            for (int seg = 0, before = 0; go && seg < 2; before += q.nk[seg++]) {
                 const CUtensorMap* ma = &q.a[q.a_of[seg]];
                 const CUtensorMap* mb = &q.b[epi_is_gate(EPI) ? rank : q.b_of[seg]];
                 const int last = min(q.nk[seg], k_last - before);

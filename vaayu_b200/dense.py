@@ -32,7 +32,7 @@ _MAX_K = 131072      # an int32 sum of fewer int8 products cannot overflow
 # The call structures of include/vaayu_b200.h, packed in one go: a ctypes structure filled field by
 # field costs more host time than the launch of a small call.
 _FFN = struct.Struct("@iiqiiPqPPPPqPPNPPqPqPPP")
-_LINEAR = struct.Struct("@qiiPqPPPPiiPqPNP")
+_LINEAR = struct.Struct("@qiiPqPPPPiiPqP")
 _INT8_FFN = struct.Struct("@iiqiiPqPPPPPPPqPNP")
 
 _current_device = torch._C._cuda_getDevice
@@ -325,7 +325,7 @@ def int8_linear(codes: torch.Tensor, scale: torch.Tensor, weight: torch.Tensor, 
         flat, out_stride = _given(out, (*shape[:-1], n), dtype, what)
     flags = _flags(codes, check)
     call = _LINEAR.pack(tokens, k, n, rows.data_ptr(), stride, sx.data_ptr(), w.data_ptr(), sw.data_ptr(),
-                        _ptr(bias), bias_code, out_code, flat.data_ptr(), out_stride, 0, 0, _ptr(flags))
+                        _ptr(bias), bias_code, out_code, flat.data_ptr(), out_stride, _ptr(flags))
     _enqueue(_lib.lib().vy_int8_linear, what, index, call)
     if check:
         _raise_on(flags, what)
