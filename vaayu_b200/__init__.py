@@ -4,6 +4,9 @@ The operator surface the engine's MoE patch calls, with the same names and seman
 reference (vaayu/packed_expert_kernels.py, vaayu/moe_patch.py's packed-expert helpers and the
 DeepSeek-V4 block-scaled dequant), running on libvaayu_b200's CUDA kernels.  There is no CPU,
 torch or Triton fallback: calls on CPU tensors or geometry the kernels do not take raise.
+
+Beside the packed experts, the layers a checkpoint leaves unpacked: `gated_ffn` (16-bit gated
+feed-forward blocks, with gradients), `quantize_int8`, `int8_linear` and `int8_gated_ffn`.
 """
 from .arena import ExpertArena
 from .block_scaled import (dequantize_block_scaled, dequantize_fp4_block_scaled, fp4_gemv,
