@@ -90,6 +90,17 @@ def test_a_thread_that_has_made_no_cuda_call():
     assert torch.equal(got[0], want)
 
 
+def test_gradients_are_not_differentiable_again():
+    """Under create_graph the gradients come as ever; differentiating them raises instead of giving zeros."""
+    ops, dy = make(6, 64, 40, BF16, grad=True)
+    want = torch.autograd.grad(vb.gated_ffn(*ops), ops, dy)
+    dy.requires_grad_(True)
+    got = torch.autograd.grad(vb.gated_ffn(*ops), ops, dy, create_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        got[0].sum().backward()
+
+
 def test_only_wanted_gradients():
     for wanted in ((0,), (1,), (2,), (3,), (1, 3), (0, 2)):
         ops, dy = make(40, 128, 72, BF16)

@@ -168,6 +168,11 @@ def _ffn_workspace(tokens: int, hidden: int, inter: int, backward: int) -> int:
     return size
 
 
+def _ffn_saved(tokens: int, inter: int) -> int:
+    key = (tokens, inter)
+    return _SIZES.get(key) or _remember(key, _lib.lib().vy_gated_ffn_saved_floats(tokens, inter))
+
+
 def _ffn_forward(x, w_gate, w_up, w_down, hidden: int, inter: int, act: int, flat, out_stride: int, index: int,
                  save: bool, check: bool):
     """The forward call into `flat`; returns what the backward pass needs when `save`."""
@@ -177,7 +182,7 @@ def _ffn_forward(x, w_gate, w_up, w_down, hidden: int, inter: int, act: int, fla
     lib = _lib.lib()
     size = _ffn_workspace(tokens, hidden, inter, 0)
     ws = rows.new_empty((size + 1) // 2)
-    saved = rows.new_empty(lib.vy_gated_ffn_saved_floats(tokens, inter), dtype=_F32) if save else None
+    saved = rows.new_empty(_ffn_saved(tokens, inter), dtype=_F32) if save else None
     flags = _flags(rows, check)
     call = _FFN.pack(_CODE[rows.dtype], act, tokens, hidden, inter, rows.data_ptr(), x_stride, wg.data_ptr(),
                      wu.data_ptr(), wd.data_ptr(), flat.data_ptr(), out_stride, _ptr(saved), ws.data_ptr(), size,
@@ -186,6 +191,27 @@ def _ffn_forward(x, w_gate, w_up, w_down, hidden: int, inter: int, act: int, fla
     if check:
         _raise_on(flags, "gated_ffn")
     return saved
+
+
+def _ffn_backward(ctx, d_out):
+    x, w_gate, w_up, w_down, saved = ctx.saved_tensors
+    (rows, x_stride), (dy, dy_stride) = _rows(x, 8), _rows(d_out, 8)
+    wg, wu, wd = _aligned(w_gate), _aligned(w_up), _aligned(w_down)
+    tokens, (inter, hidden) = rows.shape[0], wg.shape
+    need = ctx.needs_input_grad
+    grads = [_like(t) if n else None for t, n in zip((x, w_gate, w_up, w_down), need)]
+    size = _ffn_workspace(tokens, hidden, inter, 1)
+    ws, flags = rows.new_empty((size + 1) // 2), _flags(rows, ctx.check)
+    call = _FFN.pack(_CODE[rows.dtype], ctx.act, tokens, hidden, inter, rows.data_ptr(), x_stride,
+                     wg.data_ptr(), wu.data_ptr(), wd.data_ptr(), 0, 0, saved.data_ptr(), ws.data_ptr(), size,
+                     _ptr(flags), dy.data_ptr(), dy_stride, _ptr(grads[0]), hidden, *map(_ptr, grads[1:]))
+    _enqueue(_lib.lib().vy_gated_ffn_backward, "gated_ffn backward", x.get_device(), call)
+    if ctx.check:
+        _raise_on(flags, "gated_ffn backward")
+    return (*grads, None, None)
+
+
+_ffn_backward_once = torch.autograd.function.once_differentiable(_ffn_backward)
 
 
 class _GatedFfn(torch.autograd.Function):
@@ -199,23 +225,10 @@ class _GatedFfn(torch.autograd.Function):
         return out
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, d_out):
-        x, w_gate, w_up, w_down, saved = ctx.saved_tensors
-        (rows, x_stride), (dy, dy_stride) = _rows(x, 8), _rows(d_out, 8)
-        wg, wu, wd = _aligned(w_gate), _aligned(w_up), _aligned(w_down)
-        tokens, (inter, hidden) = rows.shape[0], wg.shape
-        need = ctx.needs_input_grad
-        grads = [_like(t) if n else None for t, n in zip((x, w_gate, w_up, w_down), need)]
-        size = _ffn_workspace(tokens, hidden, inter, 1)
-        ws, flags = rows.new_empty((size + 1) // 2), _flags(rows, ctx.check)
-        call = _FFN.pack(_CODE[rows.dtype], ctx.act, tokens, hidden, inter, rows.data_ptr(), x_stride,
-                         wg.data_ptr(), wu.data_ptr(), wd.data_ptr(), 0, 0, saved.data_ptr(), ws.data_ptr(), size,
-                         _ptr(flags), dy.data_ptr(), dy_stride, _ptr(grads[0]), hidden, *map(_ptr, grads[1:]))
-        _enqueue(_lib.lib().vy_gated_ffn_backward, "gated_ffn backward", x.get_device(), call)
-        if ctx.check:
-            _raise_on(flags, "gated_ffn backward")
-        return (*grads, None, None)
+        # grad mode is on here only under create_graph; the wrapper that marks the gradients as not
+        # differentiable again costs 10 us of host time
+        return _ffn_backward_once(ctx, d_out) if torch.is_grad_enabled() else _ffn_backward(ctx, d_out)
 
 
 def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor,
