@@ -27,7 +27,7 @@ def make(tokens, hidden, inter, dtype, seed=0, grad=False):
 
 SIZES = [(1, 8, 8), (1, 1024, 512), (2, 72, 40), (3, 1024, 512), (7, 136, 1000), (8, 8, 8), (15, 2048, 768), (16, 64, 64),
          (17, 200, 72), (31, 512, 264), (33, 1032, 520), (64, 256, 128), (65, 256, 136), (127, 128, 256), (128, 264, 1032),
-         (129, 520, 72), (192, 64, 2048), (255, 392, 120), (256, 256, 256), (257, 24, 1032), (700, 1024, 512),
+         (129, 520, 72), (160, 520, 1032), (161, 136, 72), (192, 64, 2048), (255, 392, 120), (256, 256, 256), (257, 24, 1032), (700, 1024, 512),
          (1003, 2048, 768)]
 
 
@@ -324,7 +324,7 @@ def test_quantize_layouts():
 
 LINEAR = [(1, 16, 1), (1, 4096, 300), (2, 32, 7), (3, 272, 97), (8, 128, 128), (15, 1040, 129), (16, 4096, 1000),
           (17, 48, 255), (33, 7168, 256), (64, 528, 513), (65, 256, 1024), (100, 14336, 64), (128, 144, 384),
-          (129, 128, 2048), (256, 512, 256), (300, 272, 97), (777, 1040, 1001), (1003, 2048, 768)]
+          (129, 128, 2048), (160, 1040, 300), (161, 528, 97), (256, 512, 256), (300, 272, 97), (777, 1040, 1001), (1003, 2048, 768)]
 
 
 def int8_operands(tokens, k, n, seed=0):

@@ -82,17 +82,11 @@ int forward(const vy_ffn_call* c, const ClusterCaps& caps, cudaStream_t s) {
     e.saved = c->saved;
     e.saved_bands = saved_bands(T);
     e.part = h_parts(c) == 2 ? h_elems(c) : 0;
-    EpiParams d{};
-    d.out = c->out;
-    d.ldo = c->out_row_stride;
-    if (T <= kStreamMaxTokens) {
-        const int t = static_cast<int>(T), parts = h_parts(c);
+    const int t = static_cast<int>(T), parts = h_parts(c);
+    if (T <= kStreamMaxGate) {
         const StreamCall gate{c->w_gate, c->w_up, c->x, c->x_row_stride, t, 1, c->inter, c->hidden, false, nullptr, 0, nullptr};
         VY_TRY((stream_launch<EPI_GATE, ACT>(gate, e, c->flags, caps, s)));
-        const StreamCall down{c->w_down, nullptr, h, I, t * parts, parts, c->hidden, c->inter, true, nullptr, 0, nullptr};
-        return stream_launch<EPI_STORE, ACT>(down, d, c->flags, caps, s);
-    }
-    {
+    } else {
         TileParams p{};
         TileProblem& q = tile_add(&p, T, I, k_blocks(H));
         tile_layout(&p, true, caps);
@@ -102,6 +96,13 @@ int forward(const vy_ffn_call* c, const ClusterCaps& caps, cudaStream_t s) {
         q.epi = e;
         p.flags = c->flags;
         VY_TRY((tile_launch<EPI_GATE, ACT>(p, caps, s)));
+    }
+    if (T <= kStreamMaxPlain) {
+        EpiParams d{};
+        d.out = c->out;
+        d.ldo = c->out_row_stride;
+        const StreamCall down{c->w_down, nullptr, h, I, t * parts, parts, c->hidden, c->inter, true, nullptr, 0, nullptr};
+        return stream_launch<EPI_STORE, ACT>(down, d, c->flags, caps, s);
     }
     TileParams p{};
     TileProblem& q = tile_add(&p, T, H, k_blocks(I));
@@ -152,7 +153,7 @@ int backward(const vy_ffn_call* c, const ClusterCaps& caps, cudaStream_t s) {
     }
     TileParams p{};
     p.flags = c->flags;
-    if (c->d_x && T <= kStreamMaxTokens) {
+    if (c->d_x && T <= kStreamMaxPlain) {
         EpiParams d{};
         d.out = c->d_x;
         d.ldo = c->d_x_row_stride;

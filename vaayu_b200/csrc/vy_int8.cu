@@ -151,7 +151,7 @@ int launch_product(const Product& a, bool first, const ClusterCaps& caps, cudaSt
     e.bias = a.bias;
     e.bias_dtype = a.bias_dtype;
     constexpr int EPI = GATE ? EPI_I8GATE : EPI_I8;
-    if (a.tokens <= kStreamMaxTokens) {
+    if (a.tokens <= (GATE ? kStreamMaxGate : kStreamMaxPlain)) {
         const StreamCall c{a.w[0], a.w[1], a.codes, a.codes_ld, static_cast<int>(a.tokens), 1, a.n, a.k, !first,
                            a.maxima, a.n_maxima, nullptr};
         return stream_launch<EPI, VY_BF16>(c, e, a.flags, caps, s);

@@ -1,4 +1,4 @@
-// vy_stream.cuh -- dense GEMM for few rows: out[T, N] = x[T, K] W[N, K]^T with T <= 128.
+// vy_stream.cuh -- dense GEMM for few rows: out[T, N] = x[T, K] W[N, K]^T.
 //
 // The weights' bytes are the cost, so the kernel is a weight stream that happens to use the tensor
 // core: 128 weight rows are the MMA's M (a gated product holds 128 gate and 128 up rows), the tokens
@@ -29,7 +29,11 @@
 namespace vy {
 
 constexpr int kStreamRows = 128;        // weight rows of a unit (of each matrix)
-constexpr int kStreamMaxTokens = 128;
+// Up to here a product streams its weights; above, the pairs of vy_tile.cuh are faster.  Measured on
+// both (us, stream against pairs): plain products, int8 4096 -> 4096, 128 tokens 11 : 15, 160 tokens
+// 13 : 15, 192 tokens 15 : 15; the gated product (with the same down product behind it), 128 tokens
+// 2048 x 2048 27 : 25, 7168 x 2048 51 : 46, 4096 x 1024 24 : 27, level at 96 tokens.
+constexpr int kStreamMaxGate = 96, kStreamMaxPlain = 160;
 constexpr int kStreamThreads = 192;     // warps 0-3 read the sums, 4 loads, 5 issues the MMAs
 constexpr int kStreamMaxStages = 12;
 // Weight bytes a CTA asks for in L2 before it waits for the kernel in front, behind what its ring holds
@@ -64,7 +68,7 @@ struct StreamParams {
 
 struct StreamBars {
     uint64_t full[kStreamMaxStages], empty[kStreamMaxStages], done;
-    float token_scale[kStreamMaxTokens];
+    float token_scale[kStreamMaxPlain];
     uint32_t token_top[kSourceTokens], part_top[4][kSourceTokens];
     uint32_t tmem_base;
     int abort_flag;
