@@ -90,23 +90,25 @@ def test_a_thread_that_has_made_no_cuda_call():
     assert torch.equal(got[0], want)
 
 
-def test_gradients_are_not_differentiable_again():
+@pytest.mark.parametrize("check", [False, True])
+def test_gradients_are_not_differentiable_again(check):
     """Under create_graph the gradients come as ever; differentiating them raises instead of giving zeros."""
     ops, dy = make(6, 64, 40, BF16, grad=True)
     want = torch.autograd.grad(vb.gated_ffn(*ops), ops, dy)
     dy.requires_grad_(True)
-    got = torch.autograd.grad(vb.gated_ffn(*ops), ops, dy, create_graph=True)
+    got = torch.autograd.grad(vb.gated_ffn(*ops, check=check), ops, dy, create_graph=True)
     assert all(torch.equal(a, b) for a, b in zip(want, got))
     with pytest.raises(RuntimeError, match="once_differentiable"):
         got[0].sum().backward()
 
 
-def test_only_wanted_gradients():
+@pytest.mark.parametrize("check", [False, True])
+def test_only_wanted_gradients(check):
     for wanted in ((0,), (1,), (2,), (3,), (1, 3), (0, 2)):
         ops, dy = make(40, 128, 72, BF16)
         for i in wanted:
             ops[i].requires_grad_(True)
-        y = vb.gated_ffn(*ops)
+        y = vb.gated_ffn(*ops, check=check)
         parts = R.ffn(*ops, "silu", BF16)[2]
         ref = R.ffn_gradients(parts, dy, BF16)
         got = torch.autograd.grad(y, [ops[i] for i in wanted], dy)
@@ -472,6 +474,32 @@ def test_a_device_that_is_not_current():
         assert torch.equal(a.cpu(), b.cpu())
     with pytest.raises(RuntimeError, match="tensors on"):
         vb.gated_ffn(ops[0], *there[1:])
+
+
+@pytest.mark.parametrize("tokens", [1, 20, 200])
+def test_both_host_paths_make_the_same_calls(tokens):
+    """The extension (ordinary calls) and the Python path (here: check=True, or a row stride) run the
+    same kernels: equal bits, gradients among them."""
+    ops, dy = make(tokens, 272, 144, F16, grad=True)
+    a, b = vb.gated_ffn(*ops), vb.gated_ffn(*ops, check=True)
+    assert type(a.grad_fn).__name__ != type(b.grad_fn).__name__
+    assert torch.equal(a, b)
+    for g, h in zip(torch.autograd.grad(a, ops, dy), torch.autograd.grad(b, ops, dy)):
+        assert torch.equal(g, h)
+    x, (wg, wu, wd) = ops[0].detach(), (w.detach() for w in ops[1:])
+    with torch.no_grad():
+        assert torch.equal(vb.gated_ffn(*ops), a) and not vb.gated_ffn(*ops).requires_grad
+    wide = torch.zeros(tokens, 288, dtype=F16, device="cuda")
+    wide[:, :272] = x
+    for p, q in zip(vb.quantize_int8(x), vb.quantize_int8(wide[:, :272])):
+        assert torch.equal(p, q)
+    codes, scale = vb.quantize_int8(x)
+    q = [t for w in (wg, wu, wd) for t in vb.quantize_int8(w)]
+    assert torch.equal(vb.int8_linear(codes, scale, q[0], q[1], dtype=F32),
+                       vb.int8_linear(codes, scale, q[0], q[1], dtype=F32, check=True))
+    assert torch.equal(vb.int8_gated_ffn(x, *q), vb.int8_gated_ffn(x, *q, check=True))
+    x3 = x.view(1, tokens, 272)
+    assert vb.int8_gated_ffn(x3, *q).shape == x3.shape and vb.quantize_int8(x3)[1].shape == (1, tokens, 1)
 
 
 # ── together ─────────────────────────────────────────────────────────────────────────────────

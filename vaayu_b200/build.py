@@ -1,4 +1,5 @@
-"""Build libvaayu_b200.so from vaayu_b200/csrc/*.cu with nvcc for sm_100a, in-tree.
+"""Build libvaayu_b200.so from vaayu_b200/csrc/*.cu with nvcc for sm_100a, in-tree, and the dense
+layers' host extension (_dense_host.so, csrc/dense_host.cpp) with g++ against torch.
 
     python -m vaayu_b200.build [--force] [--verbose]
 
@@ -19,6 +20,8 @@ SRC = PKG / "csrc"
 OBJ = PKG / "_build"
 LIB = PKG / "libvaayu_b200.so"
 INCLUDE = PKG.parent / "include"
+HOST_SRC = SRC / "dense_host.cpp"
+HOST_LIB = PKG / "_dense_host.so"
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "-Xcompiler", "-O3",
@@ -50,6 +53,30 @@ def _compile(src: Path, verbose: bool, ptxas_v: bool) -> Path:
     return obj
 
 
+def build_host(force: bool = False) -> Path:
+    """The extension module that makes the dense layers' ordinary calls without Python in between."""
+    import sysconfig
+
+    import torch
+
+    newest = max(HOST_SRC.stat().st_mtime, *(h.stat().st_mtime for h in INCLUDE.glob("*.h")))
+    if not force and HOST_LIB.exists() and HOST_LIB.stat().st_mtime >= newest:
+        return HOST_LIB
+    root = Path(torch.__file__).resolve().parent
+    cuda = Path(nvcc()).resolve().parent.parent
+    tmp = HOST_LIB.with_suffix(".so.tmp%d" % os.getpid())
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f"-I{root / 'include'}",
+           f"-I{root / 'include/torch/csrc/api/include'}", f"-I{cuda / 'include'}",
+           f"-I{sysconfig.get_paths()['include']}", str(HOST_SRC), "-o", str(tmp), f"-L{root / 'lib'}",
+           "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_python"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"{HOST_SRC.name} failed to build:\n{res.stderr}")
+    os.replace(tmp, HOST_LIB)
+    return HOST_LIB
+
+
 def build(force: bool = False, verbose: bool = False, ptxas_v: bool = False) -> Path:
     """Compile every stale .cu (in parallel) and link the shared library; returns its path."""
     OBJ.mkdir(exist_ok=True)
@@ -69,6 +96,7 @@ def build(force: bool = False, verbose: bool = False, ptxas_v: bool = False) -> 
         if res.returncode != 0:
             raise RuntimeError(f"link failed:\n{res.stderr}")
         os.replace(tmp, LIB)
+    build_host(force)
     return LIB
 
 

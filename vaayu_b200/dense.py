@@ -18,7 +18,9 @@ when a device-side wait ran out.  They may be captured in a CUDA graph.
 """
 from __future__ import annotations
 
+import ctypes
 import struct
+import threading
 
 import torch
 
@@ -34,6 +36,30 @@ _MAX_K = 131072      # an int32 sum of fewer int8 products cannot overflow
 _FFN = struct.Struct("@iiqiiPqPPPPqPPNPPqPqPPP")
 _LINEAR = struct.Struct("@qiiPqPPPPiiPqP")
 _INT8_FFN = struct.Struct("@iiqiiPqPPPPPPPqPNP")
+
+_HOST = None
+_HOST_LOCK = threading.Lock()
+_HOST_ENTRIES = ("vy_last_error", "vy_gated_ffn_saved_floats", "vy_gated_ffn_workspace_size", "vy_gated_ffn_forward",
+                 "vy_gated_ffn_backward", "vy_int8_quantize", "vy_int8_linear", "vy_int8_gated_ffn_workspace_size",
+                 "vy_int8_gated_ffn")
+
+
+def _host():
+    """The extension that makes ordinary calls (contiguous and aligned operands on the current device)
+    without Python in between; it returns None for any other, which the code below takes."""
+    global _HOST
+    if _HOST is None:
+        with _HOST_LOCK:
+            if _HOST is None:
+                try:
+                    from . import _dense_host as host
+                except ImportError as e:
+                    raise RuntimeError("_dense_host is not built; run `python -m vaayu_b200.build`") from e
+                lib = _lib.lib()
+                host.bind([ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in _HOST_ENTRIES])
+                _HOST = host
+    return _HOST
+
 
 _current_device = torch._C._cuda_getDevice
 _raw_stream = torch._C._cuda_getCurrentRawStream
@@ -243,6 +269,8 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
     Rows of x may be strided; rows or weights that do not start on 16-byte boundaries are copied."""
     what = "gated_ffn"
     code = _activation(act, what)
+    if out is None and not check and (y := (_HOST or _host()).gated_ffn(x, w_gate, w_up, w_down, code)) is not None:
+        return y
     hidden, inter = _check_ffn(x, w_gate, w_up, w_down, what)
     dtype = x.dtype
     if (dtype is not _BF16 and dtype is not _F16) or not (w_gate.dtype is w_up.dtype is w_down.dtype is dtype):
@@ -276,6 +304,9 @@ def quantize_int8(x: torch.Tensor) -> tuple:
     scale = amax(|x|) / 127 rounded to fp32; code = the nearest integer of the exact quotient
     x / scale (ties to even), so the codes do not depend on how the division is carried out.  A zero
     row has codes 0 and scale 0; a row with an infinity or NaN has codes 0 and scale NaN."""
+    pair = (_HOST or _host()).quantize_int8(x)
+    if pair is not None:
+        return pair
     what = "quantize_int8"
     code = _CODE.get(x.dtype)
     if code is None:
@@ -311,6 +342,10 @@ def int8_linear(codes: torch.Tensor, scale: torch.Tensor, weight: torch.Tensor, 
     exact (int32); the scales and the bias are applied in fp32, in that order, and the result is
     rounded once to `dtype` (bf16, fp16 or fp32)."""
     what = "int8_linear"
+    if out is None and not check:
+        y = (_HOST or _host()).int8_linear(codes, scale, weight, weight_scale, bias, _CODE.get(dtype, -1))
+        if y is not None:
+            return y
     if codes.dtype is not _INT8 or weight.dtype is not _INT8:
         raise NotImplementedError(f"{what}: codes {codes.dtype}, weight {weight.dtype} (int8)")
     shape = codes.shape
@@ -365,6 +400,10 @@ def int8_gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, gate_scale: torch.Tens
     No gradients."""
     what = "int8_gated_ffn"
     code = _activation(act, what)
+    if out is None and not check:
+        y = (_HOST or _host()).int8_gated_ffn(x, w_gate, gate_scale, w_up, up_scale, w_down, down_scale, code)
+        if y is not None:
+            return y
     if not (w_gate.dtype is w_up.dtype is w_down.dtype is _INT8):
         raise NotImplementedError(f"{what}: weights {w_gate.dtype}, {w_up.dtype}, {w_down.dtype} (int8)")
     hidden, inter = _check_ffn(x, w_gate, w_up, w_down, what)
