@@ -1,0 +1,68 @@
+"""Dense operators on the GPU at their edges: derivatives finer than a 16-bit rounding, what autograd
+may ask for beyond one backward pass, unusual views and operands, the two-part hidden rows."""
+import pytest
+import torch
+
+import vaayu_b200 as vb
+from tests import dense_reference as R
+
+pytestmark = pytest.mark.gpu
+BF16, F16, F32, F64 = torch.bfloat16, torch.float16, torch.float32, torch.float64
+
+
+def randn(*shape, seed=0):
+    return torch.randn(*shape, generator=torch.Generator(device="cuda").manual_seed(seed), device="cuda")
+
+
+def block(tokens, hidden, inter, dtype, grad=False):
+    """x, w_gate, w_up, w_down of a block with unit-variance sums."""
+    x = randn(tokens, hidden).to(dtype)
+    ws = [(randn(a, b, seed=i + 1) / b ** 0.5).to(dtype)
+          for i, (a, b) in enumerate(((inter, hidden), (inter, hidden), (hidden, inter)))]
+    return [t.requires_grad_(grad) for t in (x, *ws)]
+
+
+# ── derivatives ──────────────────────────────────────────────────────────────────────────────
+
+
+@pytest.mark.parametrize("act,check", [("gelu_tanh", False), ("gelu_tanh", True), ("silu", False)])
+def test_the_gates_derivative_in_32_bits(act, check):
+    """act'(g) to fp32 accuracy, through a d_x whose leading bits cancel: column 7 of d_x is
+    16 (256 act'(g) + hi + lo), where two more channels, whose act' is exactly 1 (g = 40), carry
+    256 act'(g) rounded to hi + lo in fp16.  Up to 32 tokens dg keeps 22 bits.
+
+    Bound, u = 2^-24: the sigmoid's argument z is off by 7 u |z| (seven roundings, constants among
+    them), exp by 4 u more, the sum and the approximate quotient by 5 u; a' = s + g s (1 - s) z' follows
+    s, with 9 u on the second term, its 1 - s, and a rounding each of the sum and of s; dg's two parts
+    are off by 2^-22, the sums of d_x by R.sum_error(16) of their terms; then the result's rounding."""
+    u = 2.0 ** -24
+    tokens = 20
+    g = (-4.5 + 0.125 * torch.arange(tokens, device="cuda", dtype=F64))
+    want = R.act_and_slope(g, act)[1]
+    k, c = 1.5957691216057308, 0.044715
+    z = g if act == "silu" else k * (g + c * g ** 3)
+    dz = torch.ones_like(g) if act == "silu" else k * (1 + 3 * c * g * g)
+    s = torch.sigmoid(z)
+    rel_s = (1 - s) * (7 * u * z.abs() + 4 * u) + 5 * u
+    term = (g * s * (1 - s) * dz).abs()
+    off = want.abs() * rel_s + term * (9 * u + s / (1 - s) * rel_s + u) + (s + want.abs()) * u
+    off = off + want.abs() * (2.0 ** -22 + 2 * R.sum_error(16))
+
+    hi = (-256 * want).to(F16)
+    lo = (-256 * want - hi.double()).to(F16)
+    x = torch.zeros(tokens, 8, device="cuda", dtype=F16)
+    x[:, 0], x[:, 1], x[:, 2], x[:, 3], x[:, 4] = g.to(F16), 40, hi, lo, 256
+    assert torch.equal(x[:, 0].double(), g)
+    wg, wu, wd = (torch.zeros(8, 8, device="cuda", dtype=F16) for _ in range(3))
+    wg[0, 0] = wg[1, 1] = wg[2, 1] = 1
+    wg[:3, 7] = 1
+    wu[0, 4] = wu[1, 2] = wu[2, 3] = 1
+    wd[0, :3] = 1
+    dy = torch.zeros_like(x)
+    dy[:, 0] = 16
+    x.requires_grad_(True)
+    y = vb.gated_ffn(x, wg, wu, wd, act=act, check=check)
+    dx, = torch.autograd.grad(y, x, dy)
+    exact = 16 * (256 * want + hi.double() + lo.double())
+    bound = (4096 * off) * (1 + R.unit(F16)) + R.unit(F16) * exact.abs() + R.tiny(F16)
+    R.assert_within(dx[:, 7], exact, bound, "the cancelled column")

@@ -11,9 +11,10 @@ namespace vy {
 // Both are g times a sigmoid: silu(g) = g s(g), and since (1 + tanh v) / 2 = s(2v), gelu_tanh(g) =
 // g s(2 sqrt(2/pi) (g + 0.044715 g^3)).  One exponential and one approximate division (2 ulp): no
 // branch, so the loads of a tile's other columns are not held up behind it.
+constexpr double kGeluCubic = 0.044715, kGeluScale = 1.5957691216057308;      // 2 sqrt(2/pi)
 __device__ __forceinline__ float sigmoid(float z) { return __fdividef(1.f, 1.f + expf(-z)); }
 __device__ __forceinline__ float gate_arg(float g, int act) {
-    return act == VY_ACT_SILU ? g : 1.5957691216057308f * (g + 0.044715f * g * g * g);
+    return act == VY_ACT_SILU ? g : float(kGeluScale) * (g + float(kGeluCubic) * g * g * g);
 }
 __device__ __forceinline__ float gate_act(float g, int act) { return g * sigmoid(gate_arg(g, act)); }
 // (value, derivative): d(g s(z)) = s + g s (1 - s) z'
@@ -21,7 +22,7 @@ __device__ __forceinline__ float2 gate_act_grad(float g, int act) {
     const float s = sigmoid(gate_arg(g, act));
     // beyond +-16 gelu's s (1 - s) is zero; the clamp keeps z' finite there
     const float c = fminf(fmaxf(g, -16.f), 16.f);
-    const float dz = act == VY_ACT_SILU ? 1.f : 1.5957691216057308f + 0.21406859462151464f * c * c;
+    const float dz = act == VY_ACT_SILU ? 1.f : float(kGeluScale) + float(3 * kGeluScale * kGeluCubic) * c * c;
     const float gs = g * s;
     return make_float2(gs, s + gs * (1.f - s) * dz);
 }
