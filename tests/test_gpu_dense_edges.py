@@ -66,3 +66,26 @@ def test_the_gates_derivative_in_32_bits(act, check):
     exact = 16 * (256 * want + hi.double() + lo.double())
     bound = (4096 * off) * (1 + R.unit(F16)) + R.unit(F16) * exact.abs() + R.tiny(F16)
     R.assert_within(dx[:, 7], exact, bound, "the cancelled column")
+
+
+@pytest.mark.parametrize("how", ["ordinary", "check", "strided"])
+def test_no_second_derivative_without_a_differentiable_incoming_gradient(how):
+    """y.sum()'s gradient is a constant, and the gradients that come of it under create_graph still
+    depend on x and the weights: a second backward pass raises, whichever host path made the call."""
+    x, wg, wu, wd = block(6, 64, 40, BF16, grad=True)
+    want = torch.autograd.grad(vb.gated_ffn(x, wg, wu, wd).sum(), (x, wg, wu, wd))
+    z = x
+    if how == "strided":
+        wide = torch.zeros(6, 72, dtype=BF16, device="cuda")
+        wide[:, :64] = x.detach()
+        z = wide[:, :64].requires_grad_(True)
+    y = vb.gated_ffn(z, wg, wu, wd, check=how == "check")
+    got = torch.autograd.grad(y.sum(), (z, wg, wu, wd), create_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+    for g in got:
+        assert g.requires_grad
+        with pytest.raises(RuntimeError, match="once_differentiable"):
+            (y.sum() + g.float().pow(2).sum()).backward(retain_graph=True)
+    only, = torch.autograd.grad(vb.gated_ffn(z, wg, wu, wd, check=how == "check").sum(), wu, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        only.sum().backward()

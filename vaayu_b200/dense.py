@@ -182,6 +182,16 @@ def _raise_on(flags: torch.Tensor, what: str) -> None:
         raise RuntimeError(f"{what}: device error flags {v:#x} (a device-side wait ran out); the output is not valid")
 
 
+def _undifferentiable(results: tuple, message: bytes) -> tuple:
+    """The results (None among them), with a node behind them that raises `message` in a backward pass."""
+    given = [t.detach().requires_grad_(True) for t in results if t is not None]
+    if not given:
+        return results
+    marked = torch._C._functions.DelayedError(message, len(given))(*given)
+    marked = iter(marked if isinstance(marked, tuple) else (marked,))
+    return tuple(t if t is None else next(marked) for t in results)
+
+
 # ── gated feed-forward, 16-bit ───────────────────────────────────────────────────────────────
 
 
@@ -237,9 +247,6 @@ def _ffn_backward(ctx, d_out):
     return (*grads, None, None)
 
 
-_ffn_backward_once = torch.autograd.function.once_differentiable(_ffn_backward)
-
-
 class _GatedFfn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w_gate, w_up, w_down, act, check):
@@ -252,9 +259,14 @@ class _GatedFfn(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, d_out):
-        # grad mode is on here only under create_graph; the wrapper that marks the gradients as not
-        # differentiable again costs 10 us of host time
-        return _ffn_backward_once(ctx, d_out) if torch.is_grad_enabled() else _ffn_backward(ctx, d_out)
+        if not torch.is_grad_enabled():
+            return _ffn_backward(ctx, d_out)
+        # create_graph: the gradients depend on x and the weights even where d_out does not require
+        # gradients (a sum's does not), so they are marked whatever d_out is
+        with torch.no_grad():
+            grads = _ffn_backward(ctx, d_out)
+        return _undifferentiable(grads, b"trying to differentiate twice a function that was marked with "
+                                        b"@once_differentiable")
 
 
 def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor,
