@@ -403,8 +403,8 @@ typedef struct vy_ffn_call {
     const void* w_down;         /* [hidden, inter], contiguous */
     void* out;                  /* forward: [n_tokens, hidden] */
     int64_t out_row_stride;     /* a multiple of 8 */
-    float* saved;               /* g and u in fp32, vy_gated_ffn_saved_floats() of them: written by
-                                   the forward call when not NULL, read by the backward call */
+    float* saved;               /* g and u in fp32, vy_gated_ffn_saved_floats() of them, 16-byte aligned:
+                                   written by the forward call when not NULL, read by the backward call */
     void* workspace;
     size_t workspace_bytes;
     int32_t* flags;

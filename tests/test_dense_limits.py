@@ -1,0 +1,29 @@
+"""Refusals of the dense operators' C entry points that keep a kernel from a bad access or an unfinished
+wait (no GPU: every call fails in its argument checks)."""
+import ctypes
+
+import pytest
+
+from vaayu_b200 import _lib
+
+A = 1 << 20      # an aligned address that is never read
+
+
+def ffn_call(backward):
+    lib, c = _lib.lib(), _lib.FfnCall()
+    c.act_dtype, c.activation, c.n_tokens, c.hidden, c.inter = _lib.BF16, 0, 4, 64, 32
+    c.x, c.x_row_stride, c.w_gate, c.w_up, c.w_down = A, 64, A, A, A
+    c.out, c.out_row_stride, c.saved = A, 64, A
+    c.d_out, c.d_out_row_stride, c.d_x, c.d_x_row_stride = A, 64, A, 64
+    c.workspace, c.workspace_bytes = A, 1 << 62
+    return c, lib.vy_gated_ffn_backward if backward else lib.vy_gated_ffn_forward
+
+
+@pytest.mark.parametrize("backward", [False, True])
+@pytest.mark.parametrize("off", [2, 4, 8, 12])
+def test_saved_must_be_aligned(backward, off):
+    """g and u move as 16-byte vectors; a float array inside a larger buffer may start anywhere."""
+    c, fn = ffn_call(backward)
+    c.saved = A + off
+    assert fn(ctypes.byref(c), None) == -3
+    assert b"saved" in _lib.lib().vy_last_error()

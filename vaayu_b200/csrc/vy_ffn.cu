@@ -36,6 +36,7 @@ int check_ffn(const vy_ffn_call* c, bool backward) {
         if (!q) return fail(VY_ERR_INVALID, "null operand");
         if (!aligned16(q)) return fail(VY_ERR_ALIGNMENT, "operands must be 16-byte aligned");
     }
+    if (!aligned16(c->saved)) return fail(VY_ERR_ALIGNMENT, "saved must be 16-byte aligned");      // moved as float4
     if (c->x_row_stride < c->hidden || c->x_row_stride % 8)
         return fail(VY_ERR_ALIGNMENT, "x row stride %lld", (long long)c->x_row_stride);
     if (!backward) {
