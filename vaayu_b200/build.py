@@ -22,6 +22,7 @@ LIB = PKG / "libvaayu_b200.so"
 INCLUDE = PKG.parent / "include"
 HOST_SRC = SRC / "dense_host.cpp"
 HOST_LIB = PKG / "_dense_host.so"
+HOST_MADE = OBJ / "_dense_host.txt"      # what it was built with
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "-Xcompiler", "-O3",
@@ -55,25 +56,33 @@ def _compile(src: Path, verbose: bool, ptxas_v: bool) -> Path:
 
 def build_host(force: bool = False) -> Path:
     """The extension module that makes the dense layers' ordinary calls without Python in between."""
+    import platform
     import sysconfig
 
     import torch
 
-    newest = max(HOST_SRC.stat().st_mtime, *(h.stat().st_mtime for h in INCLUDE.glob("*.h")))
-    if not force and HOST_LIB.exists() and HOST_LIB.stat().st_mtime >= newest:
-        return HOST_LIB
     root = Path(torch.__file__).resolve().parent
     cuda = Path(nvcc()).resolve().parent.parent
+    flags = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared",
+             f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f"-I{root / 'include'}",
+             f"-I{root / 'include/torch/csrc/api/include'}", f"-I{cuda / 'include'}",
+             f"-I{sysconfig.get_paths()['include']}", f"-L{root / 'lib'}",
+             "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_python"]
+    # it links against one torch and one Python: another of either, or other flags, makes it stale
+    made_with = "\n".join([f"torch {torch.__version__}", f"python {platform.python_version()}", *flags])
+    newest = max(HOST_SRC.stat().st_mtime, *(h.stat().st_mtime for h in INCLUDE.glob("*.h")))
+    if (not force and HOST_LIB.exists() and HOST_LIB.stat().st_mtime >= newest and HOST_MADE.exists()
+            and HOST_MADE.read_text() == made_with):
+        return HOST_LIB
     tmp = HOST_LIB.with_suffix(".so.tmp%d" % os.getpid())
-    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared",
-           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f"-I{root / 'include'}",
-           f"-I{root / 'include/torch/csrc/api/include'}", f"-I{cuda / 'include'}",
-           f"-I{sysconfig.get_paths()['include']}", str(HOST_SRC), "-o", str(tmp), f"-L{root / 'lib'}",
-           "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_python"]
+    libs = [f for f in flags if f.startswith("-l")]      # behind the source, which needs them
+    cmd = [*(f for f in flags if f not in libs), str(HOST_SRC), "-o", str(tmp), *libs]
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         raise RuntimeError(f"{HOST_SRC.name} failed to build:\n{res.stderr}")
     os.replace(tmp, HOST_LIB)
+    OBJ.mkdir(exist_ok=True)
+    HOST_MADE.write_text(made_with)
     return HOST_LIB
 
 

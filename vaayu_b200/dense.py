@@ -54,7 +54,7 @@ def _host():
                 try:
                     from . import _dense_host as host
                 except ImportError as e:
-                    raise RuntimeError("_dense_host is not built; run `python -m vaayu_b200.build`") from e
+                    raise RuntimeError(f"_dense_host does not load ({e}); run `python -m vaayu_b200.build`") from e
                 lib = _lib.lib()
                 host.bind([ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in _HOST_ENTRIES])
                 _HOST = host
