@@ -1,5 +1,7 @@
 """How the dense layers' host extension is built and found (no GPU)."""
 import os
+import shutil
+import subprocess
 
 import pytest
 
@@ -46,3 +48,14 @@ def test_an_extension_that_does_not_load_names_the_cause(monkeypatch):
     monkeypatch.delattr("vaayu_b200._dense_host", raising=False)
     with pytest.raises(RuntimeError, match="does not load .*vaayu_b200._dense_host"):
         dense._host()
+
+
+@pytest.mark.skipif(not shutil.which("readelf"), reason="binutils not available")
+def test_the_extension_uses_the_process_s_c_plus_plus_library():
+    """A second C++ library inside the extension has streams of its own that nobody initialised: an error
+    message with a number in it (every refused C call has one) ended the process."""
+    out = subprocess.run(["readelf", "-d", str(build.HOST_LIB)], capture_output=True, text=True, check=True).stdout
+    assert "libstdc++.so.6" in out
+    symbols = subprocess.run(["readelf", "-W", "--dyn-syms", str(build.HOST_LIB)], capture_output=True, text=True,
+                             check=True).stdout
+    assert not [s for s in symbols.splitlines() if "_ZNSo9_M_insert" in s and " UND " not in s]

@@ -89,3 +89,28 @@ def test_no_second_derivative_without_a_differentiable_incoming_gradient(how):
     only, = torch.autograd.grad(vb.gated_ffn(z, wg, wu, wd, check=how == "check").sum(), wu, create_graph=True)
     with pytest.raises(RuntimeError, match="once_differentiable"):
         only.sum().backward()
+
+
+# ── errors ───────────────────────────────────────────────────────────────────────────────────
+
+
+def test_a_refused_call_of_the_extension_raises():
+    """A C entry that answers with an error (here a stand-in for the quantisation's) raises, with its
+    status, and the next call works."""
+    import ctypes
+    from vaayu_b200 import _lib, dense
+    x = randn(3, 64)
+    want = vb.quantize_int8(x)
+    host, lib = dense._host(), _lib.lib()
+    real = [ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in dense._HOST_ENTRIES]
+    restype, argtypes = _lib.SIGNATURES["vy_int8_quantize"]
+    stand_in = ctypes.CFUNCTYPE(restype, *argtypes)(lambda *a: -5)
+    fake = list(real)
+    fake[dense._HOST_ENTRIES.index("vy_int8_quantize")] = ctypes.cast(stand_in, ctypes.c_void_p).value
+    host.bind(fake)
+    try:
+        with pytest.raises(RuntimeError, match=r"quantize_int8 failed \(status -5\)"):
+            vb.quantize_int8(x)
+    finally:
+        host.bind(real)
+    assert all(torch.equal(a, b) for a, b in zip(vb.quantize_int8(x), want))

@@ -67,7 +67,9 @@ def build_host(force: bool = False) -> Path:
              f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f"-I{root / 'include'}",
              f"-I{root / 'include/torch/csrc/api/include'}", f"-I{cuda / 'include'}",
              f"-I{sysconfig.get_paths()['include']}", f"-L{root / 'lib'}",
-             "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_python"]
+             # the C++ library of the process, by its file: a toolchain that has only the archive would put a
+             # second one into the extension, whose streams crash on the first error message with a number
+             "-l:libstdc++.so.6", "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_python"]
     # it links against one torch and one Python: another of either, or other flags, makes it stale
     made_with = "\n".join([f"torch {torch.__version__}", f"python {platform.python_version()}", *flags])
     newest = max(HOST_SRC.stat().st_mtime, *(h.stat().st_mtime for h in INCLUDE.glob("*.h")))
