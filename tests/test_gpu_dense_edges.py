@@ -114,3 +114,52 @@ def test_a_refused_call_of_the_extension_raises():
     finally:
         host.bind(real)
     assert all(torch.equal(a, b) for a, b in zip(vb.quantize_int8(x), want))
+
+
+@pytest.mark.parametrize("check", [False, True])
+def test_saved_tensors_that_hooks_give_back(check):
+    """Hooks on saved tensors may hand the backward pass equal tensors of another layout: the same
+    gradients.  Tensors elsewhere, of another type or size are refused before any address is taken."""
+    ops = block(40, 128, 72, BF16, grad=True)
+    dy = randn(40, 128, seed=4).to(BF16)
+    want = torch.autograd.grad(vb.gated_ffn(*ops), ops, dy)
+
+    def grads(pack, unpack):
+        with torch.autograd.graph.saved_tensors_hooks(pack, unpack):
+            y = vb.gated_ffn(*ops, check=check)
+        return torch.autograd.grad(y, ops, dy)
+
+    def off_a_boundary(t):
+        return torch.empty(t.numel() + 1, dtype=t.dtype, device=t.device)[1:].view(t.shape).copy_(t)
+
+    def across(t):
+        return t.t().contiguous().t() if t.dim() == 2 else torch.stack((t, t), 1)[:, 0]
+
+    same = [lambda t: t, lambda t: t.clone(), across, off_a_boundary]
+    for unpack in same:
+        for a, b in zip(grads(lambda t: t, unpack), want):
+            assert torch.equal(a, b)
+    for a, b in zip(grads(lambda t: t.cpu(), lambda t: t.cuda()), want):
+        assert torch.equal(a, b)
+    with torch.autograd.graph.save_on_cpu():
+        y = vb.gated_ffn(*ops, check=check)
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(y, ops, dy), want))
+    for wrong in (lambda t: t.cpu(), lambda t: t.double(), lambda t: t[:-1], lambda t: t.reshape(1, -1),
+                  lambda t: t.cpu() if t.dtype == F32 else t, lambda t: t[:-4] if t.dtype == F32 else t,
+                  lambda t: t[:33] if t.shape[0] == 40 else t, lambda t: t.half() if t.dtype == BF16 else t):
+        with pytest.raises((RuntimeError, ValueError, NotImplementedError)):
+            grads(lambda t: t, wrong)
+
+
+@pytest.mark.parametrize("check", [False, True])
+def test_a_node_called_by_hand(check):
+    ops = block(9, 64, 40, BF16, grad=True)
+    dy = randn(9, 64, seed=4).to(BF16)
+    y = vb.gated_ffn(*ops, check=check)
+    node = y.grad_fn.apply if check else y.grad_fn
+    want = torch.autograd.grad(y, ops, dy, retain_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(node(dy), want))
+    assert all(torch.equal(a, b) for a, b in zip(node(dy.t().contiguous().t()), want))
+    for wrong in (dy.cpu(), dy.float(), dy[:8], dy[:, :32], dy.view(-1)):
+        with pytest.raises((RuntimeError, ValueError, NotImplementedError)):
+            node(wrong)

@@ -9,6 +9,7 @@
 #include <ATen/ATen.h>
 #include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/cuda/CUDAFunctions.h>
+#include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
@@ -120,6 +121,15 @@ std::tuple<Tensor, Tensor> ffn_forward(const Tensor& x, const Tensor& wg, const 
     return {out, saved};
 }
 
+// A tensor of the backward pass as the kernels take it.  What a hook on saved tensors gives back, or a
+// node called by hand is given, may be anything: it is checked before its address is used.
+Tensor backward_operand(const Tensor& t, at::ScalarType type, int device, const char* what) {
+    TORCH_CHECK(t.is_cuda() && t.get_device() == device && t.scalar_type() == type, "gated_ffn backward: ", what,
+                " is not on cuda:", device, " in ", type);
+    const Tensor c = t.contiguous();
+    return aligned(c) ? c : c.clone();
+}
+
 struct GatedFfn : torch::autograd::Function<GatedFfn> {
     static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const Tensor& wg, const Tensor& wu,
                           const Tensor& wd, int64_t act) {
@@ -131,13 +141,21 @@ struct GatedFfn : torch::autograd::Function<GatedFfn> {
     }
     static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
                                                    torch::autograd::variable_list grads) {
-        const auto v = ctx->get_saved_variables();
+        auto v = ctx->get_saved_variables();
         const bool again = at::GradMode::is_enabled();      // create_graph
         torch::autograd::variable_list out(5);
         {
             at::AutoDispatchBelowADInplaceOrView below;
-            Tensor dy = grads[0].contiguous();
-            if (!aligned(dy)) dy = dy.clone();
+            TORCH_CHECK(v[0].is_cuda() && is16(v[0]), "gated_ffn backward: x is not a 16-bit CUDA tensor");
+            const at::ScalarType type = v[0].scalar_type();
+            const int device = v[0].get_device();
+            const c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(device));
+            const char* const names[5] = {"x", "w_gate", "w_up", "w_down", "what the forward call saved"};
+            for (int i = 0; i < 5; ++i) v[i] = backward_operand(v[i], i < 4 ? type : at::kFloat, device, names[i]);
+            const Tensor dy = backward_operand(grads[0], type, device, "the incoming gradient");
+            TORCH_CHECK(ffn_shapes(v[0], v[1], v[2], v[3], 8) && dy.sizes() == v[0].sizes() &&
+                            v[4].numel() == g.ffn_saved(v[0].numel() / v[0].size(-1), static_cast<int32_t>(v[1].size(0))),
+                        "gated_ffn backward: tensors of other sizes than the forward call's");
             vy_ffn_call c = ffn_call(v[0], v[1], v[2], v[3], ctx->saved_data["act"].toInt());
             for (int i = 0; i < 4; ++i)
                 if (ctx->needs_input_grad(i)) out[i] = at::empty_like(v[i]);

@@ -231,9 +231,20 @@ def _ffn_forward(x, w_gate, w_up, w_down, hidden: int, inter: int, act: int, fla
 
 def _ffn_backward(ctx, d_out):
     x, w_gate, w_up, w_down, saved = ctx.saved_tensors
+    # what a hook on saved tensors gives back, or a node called by hand is given, may be anything
+    what, dtype = "gated_ffn backward", x.dtype
+    hidden, inter = _check_ffn(x, w_gate, w_up, w_down, what)
+    _device(what, x, w_gate, w_up, w_down, saved, d_out)
+    if (dtype not in (_BF16, _F16) or not (w_gate.dtype is w_up.dtype is w_down.dtype is d_out.dtype is dtype)
+            or saved.dtype is not _F32):
+        raise NotImplementedError(f"{what}: {x.dtype}, {w_gate.dtype}, {w_up.dtype}, {w_down.dtype}, {saved.dtype}, "
+                                  f"{d_out.dtype}")
+    if d_out.shape != x.shape or saved.numel() != _ffn_saved(x.numel() // hidden, inter):
+        raise ValueError(f"{what}: tensors of other sizes than the forward call's")
+    saved = _aligned(saved)
     (rows, x_stride), (dy, dy_stride) = _rows(x, 8), _rows(d_out, 8)
     wg, wu, wd = _aligned(w_gate), _aligned(w_up), _aligned(w_down)
-    tokens, (inter, hidden) = rows.shape[0], wg.shape
+    tokens = rows.shape[0]
     need = ctx.needs_input_grad
     grads = [_like(t) if n else None for t, n in zip((x, w_gate, w_up, w_down), need)]
     size = _ffn_workspace(tokens, hidden, inter, 1)
@@ -241,9 +252,9 @@ def _ffn_backward(ctx, d_out):
     call = _FFN.pack(_CODE[rows.dtype], ctx.act, tokens, hidden, inter, rows.data_ptr(), x_stride,
                      wg.data_ptr(), wu.data_ptr(), wd.data_ptr(), 0, 0, saved.data_ptr(), ws.data_ptr(), size,
                      _ptr(flags), dy.data_ptr(), dy_stride, _ptr(grads[0]), hidden, *map(_ptr, grads[1:]))
-    _enqueue(_lib.lib().vy_gated_ffn_backward, "gated_ffn backward", x.get_device(), call)
+    _enqueue(_lib.lib().vy_gated_ffn_backward, what, x.get_device(), call)
     if ctx.check:
-        _raise_on(flags, "gated_ffn backward")
+        _raise_on(flags, what)
     return (*grads, None, None)
 
 
