@@ -395,8 +395,8 @@ enum vy_activation {
 typedef struct vy_ffn_call {
     int32_t act_dtype;  /* VY_BF16 or VY_F16: x, the weights, out and all gradients */
     int32_t activation; /* vy_activation */
-    int64_t n_tokens;
-    int32_t hidden, inter;      /* multiples of 8 */
+    int64_t n_tokens;           /* up to 2^30; up to 2^27 for weight gradients (sums over the tokens) */
+    int32_t hidden, inter;      /* multiples of 8, up to 2^27 and 2^26 */
     const void* x;              /* [n_tokens, hidden], 16-byte aligned rows */
     int64_t x_row_stride;       /* elements, a multiple of 8 */
     const void *w_gate, *w_up;  /* [inter, hidden], contiguous */

@@ -27,3 +27,21 @@ def test_saved_must_be_aligned(backward, off):
     c.saved = A + off
     assert fn(ctypes.byref(c), None) == -3
     assert b"saved" in _lib.lib().vy_last_error()
+
+
+def test_sums_that_could_outlast_a_bounded_wait_are_refused():
+    """A tile's sum of more than 2^27 products may take longer than its epilogue waits (2 s), and would
+    leave the tile unwritten."""
+    for backward, field, value in ((False, "hidden", (1 << 27) + 8), (False, "inter", (1 << 26) + 8),
+                                   (True, "hidden", (1 << 27) + 8), (True, "inter", (1 << 26) + 8)):
+        c, fn = ffn_call(backward)
+        setattr(c, field, value)
+        c.x_row_stride = c.out_row_stride = c.d_out_row_stride = c.d_x_row_stride = 1 << 28
+        assert fn(ctypes.byref(c), None) == -1
+        assert b"2^27" in _lib.lib().vy_last_error()
+    for name in ("d_w_gate", "d_w_up", "d_w_down"):
+        c, fn = ffn_call(True)
+        c.n_tokens = (1 << 27) + 1
+        setattr(c, name, A)
+        assert fn(ctypes.byref(c), None) == -1
+        assert b"2^27" in _lib.lib().vy_last_error()

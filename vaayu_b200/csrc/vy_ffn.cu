@@ -14,6 +14,11 @@ namespace {
 
 size_t align256(size_t v) { return (v + 255) & ~size_t(255); }
 
+// The longest sum of one output tile, in values of K: 2^21 blocks of 64, each 0.24 us at the tensor cores'
+// rate and 0.75 us where every block comes from HBM.  Beyond it a tile could take longer than the 2 s after
+// which a wait for its sums gives up.
+constexpr int64_t kMaxFfnK = int64_t(1) << 27;
+
 // Elements of one part of a hidden row's matrix, and bytes of the matrix.
 int64_t h_elems(const vy_ffn_call* c) { return c->n_tokens * int64_t(c->inter); }
 int h_parts(const vy_ffn_call* c) { return c->n_tokens <= kPartTokens ? 2 : 1; }
@@ -30,6 +35,10 @@ int check_ffn(const vy_ffn_call* c, bool backward) {
     if (c->n_tokens > (int64_t(1) << 30)) return fail(VY_ERR_UNSUPPORTED, "n_tokens %lld", (long long)c->n_tokens);
     if (c->hidden % 8 || c->inter % 8)
         return fail(VY_ERR_UNSUPPORTED, "hidden %d and inter %d must be multiples of 8", c->hidden, c->inter);
+    const bool by_token = backward && (c->d_w_gate || c->d_w_up || c->d_w_down);      // sums over the tokens
+    if (c->hidden > kMaxFfnK || 2 * int64_t(c->inter) > kMaxFfnK || (by_token && c->n_tokens > kMaxFfnK))
+        return fail(VY_ERR_UNSUPPORTED, "n_tokens %lld, hidden %d, inter %d: a sum of more than 2^27 products",
+                    (long long)c->n_tokens, c->hidden, c->inter);
     const bool empty = c->n_tokens == 0;
     const void* need[] = {empty ? c->w_gate : c->x, c->w_gate, c->w_up, c->w_down};
     for (const void* q : need) {
