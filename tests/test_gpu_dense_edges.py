@@ -91,6 +91,42 @@ def test_no_second_derivative_without_a_differentiable_incoming_gradient(how):
         only.sum().backward()
 
 
+@pytest.mark.parametrize("check", [False, True])
+def test_forward_mode_derivatives_are_refused(check):
+    """A dual tensor would come out without its tangent, a derivative of zero; it is refused."""
+    fwd = torch.autograd.forward_ad
+    ops = block(5, 64, 48, BF16)
+    q = [t for w in ops[1:] for t in vb.quantize_int8(w)]
+    codes, scale = vb.quantize_int8(ops[0])
+    bias = randn(48)
+    want = vb.gated_ffn(*ops)
+    with fwd.dual_level():
+        def dual(ts, i):
+            return [fwd.make_dual(t, torch.ones_like(t)) if j == i else t for j, t in enumerate(ts)]
+
+        for i in range(4):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                vb.gated_ffn(*dual(ops, i), check=check)
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            vb.quantize_int8(dual(ops, 0)[0])
+        linear = (codes, scale, q[0], q[1], bias)
+        for i in (1, 3, 4):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                vb.int8_linear(*dual(linear, i), check=check)
+        block_ops = (ops[0], *q)
+        for i in (0, 2, 4, 6):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                vb.int8_gated_ffn(*dual(block_ops, i), check=check)
+        assert torch.equal(vb.gated_ffn(*ops, check=check), want)      # no dual operand: as ever
+        leaf = ops[0].clone().requires_grad_(True)
+        y = vb.gated_ffn(leaf, *ops[1:], check=check)
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            torch.autograd.grad(y, leaf, dual(ops, 0)[0])
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            vb.gated_ffn(*ops, out=fwd.make_dual(torch.ones_like(want), torch.ones_like(want)))
+    assert torch.equal(vb.gated_ffn(*ops, check=check), want)
+
+
 # ── errors ───────────────────────────────────────────────────────────────────────────────────
 
 

@@ -65,9 +65,11 @@ int code_of(at::ScalarType t) {
     }
 }
 
+// A tensor with a forward-mode tangent, which the kernels would drop.
+bool dual(const Tensor& t) { return t._fw_grad(0).defined(); }
 // A plain CUDA tensor whose memory the kernels can take as it is.
 bool plain(const Tensor& t, int device) {
-    if (!t.is_cuda() || t.get_device() != device || !t.is_contiguous() || t.is_neg()) return false;
+    if (!t.is_cuda() || t.get_device() != device || !t.is_contiguous() || t.is_neg() || dual(t)) return false;
     const auto keys = t.unsafeGetTensorImpl()->key_set();
     return !keys.has(c10::DispatchKey::Python) && !keys.has(c10::DispatchKey::FuncTorchBatched) &&
            !keys.has(c10::DispatchKey::FuncTorchGradWrapper) && !keys.has(c10::DispatchKey::Functionalize);
@@ -126,6 +128,7 @@ std::tuple<Tensor, Tensor> ffn_forward(const Tensor& x, const Tensor& wg, const 
 Tensor backward_operand(const Tensor& t, at::ScalarType type, int device, const char* what) {
     TORCH_CHECK(t.is_cuda() && t.get_device() == device && t.scalar_type() == type, "gated_ffn backward: ", what,
                 " is not on cuda:", device, " in ", type);
+    TORCH_CHECK_NOT_IMPLEMENTED(!dual(t), "gated_ffn backward: no forward-mode derivatives (", what, " is a dual tensor)");
     const Tensor c = t.contiguous();
     return aligned(c) ? c : c.clone();
 }

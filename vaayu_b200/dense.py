@@ -182,6 +182,13 @@ def _raise_on(flags: torch.Tensor, what: str) -> None:
         raise RuntimeError(f"{what}: device error flags {v:#x} (a device-side wait ran out); the output is not valid")
 
 
+def _no_tangents(what: str, *tensors) -> None:
+    """Refuses dual tensors: the kernels would drop their tangents, a derivative of zero."""
+    for t in tensors:
+        if t is not None and t.is_floating_point() and torch.autograd.forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError(f"{what}: no forward-mode derivatives (an operand is a dual tensor)")
+
+
 def _undifferentiable(results: tuple, message: bytes) -> tuple:
     """The results (None among them), with a node behind them that raises `message` in a backward pass."""
     given = [t.detach().requires_grad_(True) for t in results if t is not None]
@@ -235,6 +242,7 @@ def _ffn_backward(ctx, d_out):
     what, dtype = "gated_ffn backward", x.dtype
     hidden, inter = _check_ffn(x, w_gate, w_up, w_down, what)
     _device(what, x, w_gate, w_up, w_down, saved, d_out)
+    _no_tangents(what, x, w_gate, w_up, w_down, saved, d_out)
     if (dtype not in (_BF16, _F16) or not (w_gate.dtype is w_up.dtype is w_down.dtype is d_out.dtype is dtype)
             or saved.dtype is not _F32):
         raise NotImplementedError(f"{what}: {x.dtype}, {w_gate.dtype}, {w_up.dtype}, {w_down.dtype}, {saved.dtype}, "
@@ -302,6 +310,7 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
     if hidden % 8 or inter % 8 or not hidden or not inter:
         raise NotImplementedError(f"{what}: hidden {hidden} and inter {inter} must be multiples of 8")
     index = _device(what, x, w_gate, w_up, w_down, out)
+    _no_tangents(what, x, w_gate, w_up, w_down, out)
     if torch.is_grad_enabled() and (x.requires_grad or w_gate.requires_grad or w_up.requires_grad
                                     or w_down.requires_grad):
         if out is not None:
@@ -338,6 +347,7 @@ def quantize_int8(x: torch.Tensor) -> tuple:
     if not shape or shape[-1] == 0:
         raise ValueError(f"{what}: x {tuple(shape)} has no values in a row")
     index = _device(what, x)
+    _no_tangents(what, x)
     rows, stride = _unit_rows(x)
     tokens, width = rows.shape
     codes = torch.empty_like(x, dtype=_INT8) if x.is_contiguous() else x.new_empty(shape, dtype=_INT8)
@@ -386,6 +396,7 @@ def int8_linear(codes: torch.Tensor, scale: torch.Tensor, weight: torch.Tensor, 
             raise ValueError(f"{what}: bias {tuple(bias.shape)} for {n} output channels")
         bias, bias_code = bias.contiguous(), _CODE[bias.dtype]
     index = _device(what, codes, scale, weight, weight_scale, bias, out)
+    _no_tangents(what, scale, weight_scale, bias, out)
     (rows, stride), w = _rows(codes, 16), _aligned(weight)
     tokens = rows.shape[0]
     sx, sw = _scales(scale, tokens, what), _scales(weight_scale, n, what)
@@ -436,6 +447,7 @@ def int8_gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, gate_scale: torch.Tens
     if hidden % 16 or inter % 16 or not 0 < hidden < _MAX_K or not 0 < inter < _MAX_K:
         raise NotImplementedError(f"{what}: hidden {hidden} and inter {inter} must be multiples of 16 below {_MAX_K}")
     index = _device(what, x, w_gate, gate_scale, w_up, up_scale, w_down, down_scale, out)
+    _no_tangents(what, x, gate_scale, up_scale, down_scale, out)
     (rows, stride), wg, wu, wd = _unit_rows(x), _aligned(w_gate), _aligned(w_up), _aligned(w_down)
     sg, su, sd = _scales(gate_scale, inter, what), _scales(up_scale, inter, what), _scales(down_scale, hidden, what)
     if out is None:
