@@ -127,6 +127,45 @@ def test_forward_mode_derivatives_are_refused(check):
     assert torch.equal(vb.gated_ffn(*ops, check=check), want)
 
 
+@pytest.mark.parametrize("check", [False, True])
+def test_int8_calls_say_that_they_have_no_gradients(check):
+    """The int8 calls run on operands that require gradients, with the same bits, and a backward pass
+    through their results raises: it would silently leave the operands without their share."""
+    ops = block(5, 64, 48, BF16)
+    q = [t for w in ops[1:] for t in vb.quantize_int8(w)]
+    codes, scale = vb.quantize_int8(ops[0])
+    linear = (codes, scale, q[0], q[1], randn(48))
+    whole = (ops[0], *q)
+
+    def grad_of(ts, i):
+        return [t.clone().requires_grad_(True) if j == i else t for j, t in enumerate(ts)]
+
+    calls = [(vb.int8_linear, linear, (1, 3, 4)), (vb.int8_gated_ffn, whole, (0, 2, 4, 6))]
+    for fn, operands, places in calls:
+        want = fn(*operands, check=check)
+        assert not want.requires_grad
+        for i in places:
+            with_grad = grad_of(operands, i)
+            y = fn(*with_grad, check=check)
+            assert torch.equal(y, want) and y.requires_grad
+            with pytest.raises(RuntimeError, match="no gradients"):
+                y.float().sum().backward()
+            assert with_grad[i].grad is None
+            with torch.no_grad():
+                assert not fn(*with_grad, check=check).requires_grad
+            with pytest.raises(RuntimeError, match="out="):
+                fn(*with_grad, out=torch.empty_like(want))
+    x = ops[0].clone().requires_grad_(True)
+    c, s = vb.quantize_int8(x)
+    assert torch.equal(c, codes) and torch.equal(s, scale) and not c.requires_grad
+    y = vb.int8_linear(c, s, q[0], q[1], check=check)
+    for result in (s, y):
+        with pytest.raises(RuntimeError, match="no gradients"):
+            result.float().sum().backward()
+    empty = vb.quantize_int8(torch.empty(0, 48, device="cuda", requires_grad=True))
+    assert empty[1].requires_grad and empty[1].shape == (0, 1)
+
+
 # ── errors ───────────────────────────────────────────────────────────────────────────────────
 
 

@@ -67,6 +67,8 @@ int code_of(at::ScalarType t) {
 
 // A tensor with a forward-mode tangent, which the kernels would drop.
 bool dual(const Tensor& t) { return t._fw_grad(0).defined(); }
+// Gradients are wanted for an operand of a call that has none: dense.py marks its result.
+bool cut_off(const Tensor& t) { return t.requires_grad() && at::GradMode::is_enabled(); }
 // A plain CUDA tensor whose memory the kernels can take as it is.
 bool plain(const Tensor& t, int device) {
     if (!t.is_cuda() || t.get_device() != device || !t.is_contiguous() || t.is_neg() || dual(t)) return false;
@@ -209,7 +211,7 @@ std::optional<std::tuple<Tensor, Tensor>> quantize(const Tensor& x) {
     const int code = code_of(x.scalar_type());
     if (!x.is_cuda() || code < 0 || x.dim() < 1 || x.numel() == 0) return std::nullopt;
     const int device = c10::cuda::current_device();
-    if (!plain(x, device)) return std::nullopt;
+    if (!plain(x, device) || cut_off(x)) return std::nullopt;
     at::AutoDispatchBelowADInplaceOrView below;
     const int64_t cols = x.size(-1), rows = x.numel() / cols;
     if (rows > 0x7FFFFFFF) return std::nullopt;
@@ -225,7 +227,7 @@ std::optional<std::tuple<Tensor, Tensor>> quantize(const Tensor& x) {
 
 // fp32 scales of `n` rows.
 bool plain_scales(const Tensor& s, int64_t n, int device) {
-    return s.scalar_type() == at::kFloat && s.numel() == n && plain(s, device);
+    return s.scalar_type() == at::kFloat && s.numel() == n && plain(s, device) && !cut_off(s);
 }
 
 std::optional<Tensor> int8_linear(const Tensor& codes, const Tensor& scale, const Tensor& w, const Tensor& ws,
@@ -240,7 +242,8 @@ std::optional<Tensor> int8_linear(const Tensor& codes, const Tensor& scale, cons
         !aligned(w) || !plain_scales(scale, rows, device) || !plain_scales(ws, n, device))
         return std::nullopt;
     if (bias.has_value()) {
-        if (bias->dim() != 1 || bias->size(0) != n || code_of(bias->scalar_type()) < 0 || !plain(*bias, device))
+        if (bias->dim() != 1 || bias->size(0) != n || code_of(bias->scalar_type()) < 0 || !plain(*bias, device) ||
+            cut_off(*bias))
             return std::nullopt;
         c.bias = bias->const_data_ptr();
         c.bias_dtype = code_of(bias->scalar_type());
@@ -269,7 +272,7 @@ std::optional<Tensor> int8_gated_ffn(const Tensor& x, const Tensor& wg, const Te
                                      const Tensor& wd, const Tensor& sd, int64_t act) {
     if (!x.is_cuda() || !ffn_shapes(x, wg, wu, wd, 16) || !is16(x)) return std::nullopt;
     const int device = c10::cuda::current_device();
-    if (!plain(x, device)) return std::nullopt;
+    if (!plain(x, device) || cut_off(x)) return std::nullopt;
     for (const Tensor* t : {&wg, &wu, &wd})
         if (t->scalar_type() != at::kChar || !plain(*t, device) || !aligned(*t)) return std::nullopt;
     vy_int8_ffn_call c{};

@@ -330,12 +330,23 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
 # ── int8 ─────────────────────────────────────────────────────────────────────────────────────
 
 
+def _cut_off(what: str, out, *tensors) -> bool:
+    """Whether gradients are wanted for an operand of a call that has none; its result is then marked
+    (`_undifferentiable`) instead of dropping out of the graph without a word."""
+    if not torch.is_grad_enabled() or not any(t is not None and t.requires_grad for t in tensors):
+        return False
+    if out is not None:
+        raise RuntimeError(f"{what}: out= with gradients")
+    return True
+
+
 def quantize_int8(x: torch.Tensor) -> tuple:
     """(codes int8 [..., K], scale fp32 [..., 1]): one scale per row of x (bf16 / fp16 / fp32, any K).
 
     scale = amax(|x|) / 127 rounded to fp32; code = the nearest integer of the exact quotient
     x / scale (ties to even), so the codes do not depend on how the division is carried out.  A zero
-    row has codes 0 and scale 0; a row with an infinity or NaN has codes 0 and scale NaN."""
+    row has codes 0 and scale 0; a row with an infinity or NaN has codes 0 and scale NaN.  No gradients:
+    a backward pass through the scale raises."""
     pair = (_HOST or _host()).quantize_int8(x)
     if pair is not None:
         return pair
@@ -354,6 +365,8 @@ def quantize_int8(x: torch.Tensor) -> tuple:
     scale = x.new_empty(tokens, 1, dtype=_F32) if len(shape) == 2 else x.new_empty((*shape[:-1], 1), dtype=_F32)
     _enqueue(_lib.lib().vy_int8_quantize, what, index, rows.data_ptr(), code, stride, tokens, width,
              codes.data_ptr(), scale.data_ptr())
+    if _cut_off(what, None, x):
+        scale, = _undifferentiable((scale,), b"quantize_int8 has no gradients")
     return codes, scale
 
 
@@ -373,7 +386,7 @@ def int8_linear(codes: torch.Tensor, scale: torch.Tensor, weight: torch.Tensor, 
     codes [..., K] int8 with one scale per row (`quantize_int8`'s pair); weight [N, K] int8 with one
     scale per output channel ([N] or [N, 1]); K a multiple of 16 below 131072, any N.  The sum is
     exact (int32); the scales and the bias are applied in fp32, in that order, and the result is
-    rounded once to `dtype` (bf16, fp16 or fp32)."""
+    rounded once to `dtype` (bf16, fp16 or fp32).  No gradients: a backward pass through it raises."""
     what = "int8_linear"
     if out is None and not check:
         y = (_HOST or _host()).int8_linear(codes, scale, weight, weight_scale, bias, _CODE.get(dtype, -1))
@@ -397,6 +410,7 @@ def int8_linear(codes: torch.Tensor, scale: torch.Tensor, weight: torch.Tensor, 
         bias, bias_code = bias.contiguous(), _CODE[bias.dtype]
     index = _device(what, codes, scale, weight, weight_scale, bias, out)
     _no_tangents(what, scale, weight_scale, bias, out)
+    cut = _cut_off(what, out, scale, weight_scale, bias)
     (rows, stride), w = _rows(codes, 16), _aligned(weight)
     tokens = rows.shape[0]
     sx, sw = _scales(scale, tokens, what), _scales(weight_scale, n, what)
@@ -411,7 +425,7 @@ def int8_linear(codes: torch.Tensor, scale: torch.Tensor, weight: torch.Tensor, 
     _enqueue(_lib.lib().vy_int8_linear, what, index, call)
     if check:
         _raise_on(flags, what)
-    return out
+    return _undifferentiable((out,), b"int8_linear has no gradients")[0] if cut else out
 
 
 def _int8_ffn_workspace(tokens: int, hidden: int, inter: int) -> int:
@@ -431,7 +445,7 @@ def int8_gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, gate_scale: torch.Tens
 
     x [..., hidden] bf16 or fp16; w_gate, w_up int8 [inter, hidden]; w_down int8 [hidden, inter];
     hidden and inter multiples of 16; scales [rows] or [rows, 1].  Returns [..., hidden] in x's type.
-    No gradients."""
+    No gradients: a backward pass through it raises."""
     what = "int8_gated_ffn"
     code = _activation(act, what)
     if out is None and not check:
@@ -448,6 +462,7 @@ def int8_gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, gate_scale: torch.Tens
         raise NotImplementedError(f"{what}: hidden {hidden} and inter {inter} must be multiples of 16 below {_MAX_K}")
     index = _device(what, x, w_gate, gate_scale, w_up, up_scale, w_down, down_scale, out)
     _no_tangents(what, x, gate_scale, up_scale, down_scale, out)
+    cut = _cut_off(what, out, x, gate_scale, up_scale, down_scale)
     (rows, stride), wg, wu, wd = _unit_rows(x), _aligned(w_gate), _aligned(w_up), _aligned(w_down)
     sg, su, sd = _scales(gate_scale, inter, what), _scales(up_scale, inter, what), _scales(down_scale, hidden, what)
     if out is None:
@@ -464,4 +479,4 @@ def int8_gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, gate_scale: torch.Tens
     _enqueue(_lib.lib().vy_int8_gated_ffn, what, index, call)
     if check:
         _raise_on(flags, what)
-    return out
+    return _undifferentiable((out,), b"int8_gated_ffn has no gradients")[0] if cut else out
