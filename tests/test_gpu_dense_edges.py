@@ -191,6 +191,27 @@ def test_a_refused_call_of_the_extension_raises():
     assert all(torch.equal(a, b) for a, b in zip(vb.quantize_int8(x), want))
 
 
+# ── views and operands ───────────────────────────────────────────────────────────────────────
+
+
+@pytest.mark.parametrize("tokens", [2, 12, 24, 300])
+def test_rows_that_overlap(tokens):
+    """Rows on top of one another (an expanded row) or overlapping: the same numbers as their copy."""
+    x, wg, wu, wd = block(tokens, 272, 144, BF16)
+    q = [t for w in (wg, wu, wd) for t in vb.quantize_int8(w)]
+    line = randn(272 + 16 * tokens, seed=9).to(BF16)
+    codes, _ = vb.quantize_int8(line.view(1, -1))
+    for rows in (x[:1].expand(tokens, 272), line.as_strided((tokens, 272), (16, 1)),
+                 line.as_strided((tokens, 272), (3, 1)), line.as_strided((tokens, 272), (1, 1))):
+        assert torch.equal(vb.int8_gated_ffn(rows, *q), vb.int8_gated_ffn(rows.contiguous(), *q))
+        assert torch.equal(vb.gated_ffn(rows, wg, wu, wd), vb.gated_ffn(rows.contiguous(), wg, wu, wd))
+        for a, b in zip(vb.quantize_int8(rows), vb.quantize_int8(rows.contiguous())):
+            assert torch.equal(a, b)
+    scale = torch.rand(tokens, 1, device="cuda")
+    rows = codes.view(-1).as_strided((tokens, 272), (16, 1))
+    assert torch.equal(vb.int8_linear(rows, scale, q[0], q[1]), vb.int8_linear(rows.contiguous(), scale, q[0], q[1]))
+
+
 @pytest.mark.parametrize("check", [False, True])
 def test_saved_tensors_that_hooks_give_back(check):
     """Hooks on saved tensors may hand the backward pass equal tensors of another layout: the same

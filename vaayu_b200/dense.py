@@ -464,6 +464,8 @@ def int8_gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, gate_scale: torch.Tens
     _no_tangents(what, x, gate_scale, up_scale, down_scale, out)
     cut = _cut_off(what, out, x, gate_scale, up_scale, down_scale)
     (rows, stride), wg, wu, wd = _unit_rows(x), _aligned(w_gate), _aligned(w_up), _aligned(w_down)
+    if stride < hidden:      # rows on top of one another (an expanded row)
+        rows, stride = rows.contiguous(), hidden
     sg, su, sd = _scales(gate_scale, inter, what), _scales(up_scale, inter, what), _scales(down_scale, hidden, what)
     if out is None:
         out, out_stride = _like(x), hidden
