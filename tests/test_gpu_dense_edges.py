@@ -259,3 +259,28 @@ def test_a_node_called_by_hand(check):
     for wrong in (dy.cpu(), dy.float(), dy[:8], dy[:, :32], dy.view(-1)):
         with pytest.raises((RuntimeError, ValueError, NotImplementedError)):
             node(wrong)
+
+
+def test_out_counts_as_a_write():
+    """A tensor that a backward pass still needs and that then receives a result through out= is
+    noticed, as for torch's own out=; an out that requires gradients is refused."""
+    ops = block(4, 64, 48, BF16)
+    q = [t for w in ops[1:] for t in vb.quantize_int8(w)]
+    codes, scale = vb.quantize_int8(ops[0])
+    calls = [lambda out: vb.gated_ffn(*ops, out=out), lambda out: vb.int8_gated_ffn(ops[0], *q, out=out),
+             lambda out: vb.int8_linear(codes, scale, q[0], q[1], out=out)]
+    for call, width in zip(calls, (64, 64, 48)):
+        out = torch.ones(4, width, dtype=BF16, device="cuda")
+        w = torch.ones(4, width, dtype=BF16, device="cuda", requires_grad=True)
+        y = (w * out).sum()
+        before = out._version
+        assert call(out) is out and out._version == before + 1
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward()
+        leaf = torch.ones(4, width, dtype=BF16, device="cuda", requires_grad=True)
+        with pytest.raises(RuntimeError, match="out="):
+            call(leaf)
+        with torch.no_grad():
+            call(leaf)
+        with torch.inference_mode():
+            call(torch.ones(4, width, dtype=BF16, device="cuda"))

@@ -159,6 +159,12 @@ def _given(out, shape, dtype, what: str) -> tuple:
     return out.view(-1, shape[-1]), shape[-1]
 
 
+def _written(out: torch.Tensor) -> None:
+    """Counts up the version of the caller's out: a backward pass that still needs what it held notices."""
+    if not out.is_inference():
+        torch.autograd.graph.increment_version(out)
+
+
 _SIZES: dict = {}      # an entry point's sizes -> its workspace bytes
 
 
@@ -312,7 +318,7 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
     index = _device(what, x, w_gate, w_up, w_down, out)
     _no_tangents(what, x, w_gate, w_up, w_down, out)
     if torch.is_grad_enabled() and (x.requires_grad or w_gate.requires_grad or w_up.requires_grad
-                                    or w_down.requires_grad):
+                                    or w_down.requires_grad or (out is not None and out.requires_grad)):
         if out is not None:
             raise RuntimeError(f"{what}: out= with gradients")
         return _GatedFfn.apply(x, w_gate, w_up, w_down, code, check)
@@ -323,6 +329,7 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
         flat, stride = _given(out, x.shape, dtype, what)
         if flat.data_ptr() & 15 or stride % 8:
             raise ValueError(f"{what}: out rows must start on 16-byte boundaries")
+        _written(out)
     _ffn_forward(x, w_gate, w_up, w_down, hidden, inter, code, flat, stride, index, False, check)
     return out
 
@@ -333,7 +340,7 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
 def _cut_off(what: str, out, *tensors) -> bool:
     """Whether gradients are wanted for an operand of a call that has none; its result is then marked
     (`_undifferentiable`) instead of dropping out of the graph without a word."""
-    if not torch.is_grad_enabled() or not any(t is not None and t.requires_grad for t in tensors):
+    if not torch.is_grad_enabled() or not any(t is not None and t.requires_grad for t in (*tensors, out)):
         return False
     if out is not None:
         raise RuntimeError(f"{what}: out= with gradients")
@@ -419,6 +426,7 @@ def int8_linear(codes: torch.Tensor, scale: torch.Tensor, weight: torch.Tensor, 
         flat, out_stride = out, n
     else:
         flat, out_stride = _given(out, (*shape[:-1], n), dtype, what)
+        _written(out)
     flags = _flags(codes, check)
     call = _LINEAR.pack(tokens, k, n, rows.data_ptr(), stride, sx.data_ptr(), w.data_ptr(), sw.data_ptr(),
                         _ptr(bias), bias_code, out_code, flat.data_ptr(), out_stride, _ptr(flags))
@@ -472,6 +480,7 @@ def int8_gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, gate_scale: torch.Tens
         flat = out
     else:
         flat, out_stride = _given(out, x.shape, dtype, what)
+        _written(out)
     tokens = rows.shape[0]
     size = _int8_ffn_workspace(tokens, hidden, inter)
     ws, flags = rows.new_empty((size + 1) // 2), _flags(rows, check)
