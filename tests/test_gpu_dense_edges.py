@@ -284,3 +284,29 @@ def test_out_counts_as_a_write():
             call(leaf)
         with torch.inference_mode():
             call(torch.ones(4, width, dtype=BF16, device="cuda"))
+
+
+def test_views_with_the_negative_bit():
+    """A view that torch marks as negated (an imaginary part of a conjugate is one) is taken at its value."""
+    x, wg, wu, wd = block(5, 64, 48, BF16)
+    neg = torch._neg_view
+    want = vb.gated_ffn(-x, wg, wu, wd)
+    for check in (False, True):
+        assert torch.equal(vb.gated_ffn(neg(x), wg, wu, wd, check=check), want)
+        assert torch.equal(vb.gated_ffn(x, wg, neg(wu), wd, check=check), vb.gated_ffn(x, wg, -wu, wd))
+        assert torch.equal(vb.gated_ffn(x, wg, wu, neg(wd), check=check), vb.gated_ffn(x, wg, wu, -wd))
+    for a, b in zip(vb.quantize_int8(neg(x)), vb.quantize_int8(-x)):
+        assert torch.equal(a, b)
+    q = [t for w in (wg, wu, wd) for t in vb.quantize_int8(w)]
+    codes, scale = vb.quantize_int8(x)
+    bias = randn(48)
+    assert torch.equal(vb.int8_linear(neg(codes), scale, q[0], neg(q[1]), neg(bias)),
+                       vb.int8_linear(-codes, scale, q[0], -q[1], -bias))
+    assert torch.equal(vb.int8_gated_ffn(neg(x), *q), vb.int8_gated_ffn(-x, *q))
+    leaf = x.clone().requires_grad_(True)
+    a, = torch.autograd.grad(vb.gated_ffn(leaf, wg, wu, wd), leaf, neg(x))
+    b, = torch.autograd.grad(vb.gated_ffn(leaf, wg, wu, wd, check=True), leaf, neg(x))
+    c, = torch.autograd.grad(vb.gated_ffn(leaf, wg, wu, wd), leaf, -x)
+    assert torch.equal(a, c) and torch.equal(b, c)
+    with pytest.raises(ValueError, match="out"):
+        vb.gated_ffn(x, wg, wu, wd, out=neg(torch.zeros_like(x)))

@@ -97,6 +97,7 @@ def _activation(act: str, what: str) -> int:
 def _rows(x: torch.Tensor, unit: int) -> tuple:
     """(x as [tokens, width] with rows that start on 16-byte boundaries (`unit` elements), its row
     stride): a view where the strides allow it, else a copy."""
+    x = x.resolve_neg()
     if x.dim() != 2:
         x = x.reshape(-1, x.shape[-1])
     tokens, width = x.shape
@@ -112,6 +113,7 @@ def _rows(x: torch.Tensor, unit: int) -> tuple:
 
 def _unit_rows(x: torch.Tensor) -> tuple:
     """(x as [tokens, width] with a unit column stride, its row stride)."""
+    x = x.resolve_neg()
     if x.dim() != 2:
         x = x.reshape(-1, x.shape[-1])
     row, col = x.stride()
@@ -123,6 +125,7 @@ def _unit_rows(x: torch.Tensor) -> tuple:
 
 def _aligned(w: torch.Tensor) -> torch.Tensor:
     """w itself when it is contiguous and starts on a 16-byte boundary, else a copy that does."""
+    w = w.resolve_neg()
     if not w.is_contiguous():
         return w.contiguous()
     return w.clone() if w.data_ptr() & 15 else w
@@ -152,6 +155,8 @@ def _given(out, shape, dtype, what: str) -> tuple:
     """(the caller's out as [tokens, width], its row stride)."""
     if out.shape != shape or out.dtype != dtype:
         raise ValueError(f"{what}: out {tuple(out.shape)} {out.dtype}, expected {tuple(shape)} {dtype}")
+    if out.is_neg():
+        raise ValueError(f"{what}: out is a negated view")
     if not out.is_contiguous():
         if out.dim() != 2 or out.stride(1) != 1 or out.stride(0) < out.shape[1]:
             raise ValueError(f"{what}: out must be contiguous, or a 2-D view with unit column stride")
@@ -380,6 +385,7 @@ def quantize_int8(x: torch.Tensor) -> tuple:
 def _scales(scale: torch.Tensor, n: int, what: str) -> torch.Tensor:
     if scale.numel() != n or not scale.is_floating_point():
         raise ValueError(f"{what}: {tuple(scale.shape)} {scale.dtype} scales for {n} rows")
+    scale = scale.resolve_neg()
     if scale.dtype is not _F32:
         scale = scale.to(_F32)
     return scale if scale.is_contiguous() else scale.contiguous()
@@ -414,7 +420,7 @@ def int8_linear(codes: torch.Tensor, scale: torch.Tensor, weight: torch.Tensor, 
     if bias is not None:
         if bias.dim() != 1 or bias.shape[0] != n:
             raise ValueError(f"{what}: bias {tuple(bias.shape)} for {n} output channels")
-        bias, bias_code = bias.contiguous(), _CODE[bias.dtype]
+        bias, bias_code = bias.resolve_neg().contiguous(), _CODE[bias.dtype]
     index = _device(what, codes, scale, weight, weight_scale, bias, out)
     _no_tangents(what, scale, weight_scale, bias, out)
     cut = _cut_off(what, out, scale, weight_scale, bias)
