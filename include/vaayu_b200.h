@@ -449,7 +449,8 @@ int vy_int8_quantize(const void* x, int32_t x_dtype, int64_t x_row_stride, int64
 
 typedef struct vy_int8_linear_call {
     int64_t n_tokens;
-    int32_t k, n;              /* k: a multiple of 16, below 131072 (an int32 sum cannot overflow) */
+    int32_t k, n;              /* k: a multiple of 16, below 131072 (an int32 sum cannot overflow);
+                                  n: up to 2^31 - 256 */
     const int8_t* codes;       /* [n_tokens, k], 16-byte aligned rows */
     int64_t codes_row_stride;  /* a multiple of 16 */
     const float* scales;       /* [n_tokens] */

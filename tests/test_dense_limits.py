@@ -3,7 +3,9 @@ wait (no GPU: every call fails in its argument checks)."""
 import ctypes
 
 import pytest
+import torch
 
+import vaayu_b200 as vb
 from vaayu_b200 import _lib
 
 A = 1 << 20      # an aligned address that is never read
@@ -45,3 +47,22 @@ def test_sums_that_could_outlast_a_bounded_wait_are_refused():
         setattr(c, name, A)
         assert fn(ctypes.byref(c), None) == -1
         assert b"2^27" in _lib.lib().vy_last_error()
+
+
+@pytest.mark.parametrize("tokens", [1, 500])
+def test_more_output_channels_than_an_int_rounds_up(tokens):
+    """n within a tile of 2^31 overflowed when it was rounded up to whole tiles, and the launch had a
+    grid of its own."""
+    lib, c = _lib.lib(), _lib.Int8LinearCall()
+    c.n_tokens, c.k, c.n = tokens, 16, 0x7FFFFF01
+    c.codes, c.codes_row_stride, c.scales, c.weight, c.weight_scales = A, 16, A, A, A
+    c.out_dtype, c.out, c.out_row_stride = _lib.BF16, A, 1 << 31
+    assert lib.vy_int8_linear(ctypes.byref(c), None) == -1
+    assert b"above" in lib.vy_last_error()
+
+
+@pytest.mark.parametrize("n", [0x7FFFFF01, 1 << 31, 1 << 40])
+def test_int8_linear_refuses_them_by_name(n):
+    codes, w = torch.zeros(2, 16, dtype=torch.int8), torch.zeros(1, dtype=torch.int8).expand(n, 16)
+    with pytest.raises(NotImplementedError, match="up to"):
+        vb.int8_linear(codes, torch.ones(2, 1), w, torch.ones(1).expand(n))

@@ -238,7 +238,7 @@ std::optional<Tensor> int8_linear(const Tensor& codes, const Tensor& scale, cons
     const int device = c10::cuda::current_device();
     vy_int8_linear_call c{};
     const int64_t k = w.size(1), n = w.size(0), rows = codes.numel() / k;
-    if (k % 16 || k >= 131072 || n == 0 || n > 0x7FFFFFFF || !plain(codes, device) || !plain(w, device) || !aligned(codes) ||
+    if (k % 16 || k >= 131072 || n == 0 || n > 0x7FFFFF00 || !plain(codes, device) || !plain(w, device) || !aligned(codes) ||
         !aligned(w) || !plain_scales(scale, rows, device) || !plain_scales(ws, n, device))
         return std::nullopt;
     if (bias.has_value()) {

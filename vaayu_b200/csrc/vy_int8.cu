@@ -12,6 +12,7 @@ namespace vy {
 namespace {
 
 constexpr int kMaxK = 131072;      // 128 * 128 * k stays below 2^31
+constexpr int kMaxN = 0x7FFFFF00;      // rounded up to whole tiles it is still an int
 size_t align256(size_t v) { return (v + 255) & ~size_t(255); }
 
 // ── quantisation ────────────────────────────────────────────────────────────────────────────
@@ -175,6 +176,7 @@ int check_linear(const vy_int8_linear_call* c) {
         return fail(VY_ERR_INVALID, "n_tokens %lld, k %d, n %d", (long long)c->n_tokens, c->k, c->n);
     if (c->n_tokens > (int64_t(1) << 30)) return fail(VY_ERR_UNSUPPORTED, "n_tokens %lld", (long long)c->n_tokens);
     if (c->k % 16 || c->k >= kMaxK) return fail(VY_ERR_UNSUPPORTED, "k %d must be a multiple of 16 below %d", c->k, kMaxK);
+    if (c->n > kMaxN) return fail(VY_ERR_UNSUPPORTED, "n %d above %d", c->n, kMaxN);
     if (!float_dtype(c->out_dtype) || (c->bias && !float_dtype(c->bias_dtype)))
         return fail(VY_ERR_UNSUPPORTED, "out / bias dtype code %d / %d", c->out_dtype, c->bias_dtype);
     if (c->n_tokens == 0) return VY_OK;

@@ -30,6 +30,7 @@ ACTIVATIONS = {"silu": 0, "gelu_tanh": 1}
 _BF16, _F16, _F32, _INT8 = torch.bfloat16, torch.float16, torch.float32, torch.int8
 _CODE = {_BF16: _lib.BF16, _F16: _lib.F16, _F32: _lib.F32}
 _MAX_K = 131072      # an int32 sum of fewer int8 products cannot overflow
+_MAX_N = 0x7FFFFF00
 
 # The call structures of include/vaayu_b200.h, packed in one go: a ctypes structure filled field by
 # field costs more host time than the launch of a small call.
@@ -414,8 +415,8 @@ def int8_linear(codes: torch.Tensor, scale: torch.Tensor, weight: torch.Tensor, 
     if out_code is None or (bias is not None and bias.dtype not in _CODE):
         raise NotImplementedError(f"{what}: dtype {dtype}, bias {None if bias is None else bias.dtype}")
     n, k = weight.shape
-    if k % 16 or not 0 < k < _MAX_K or n == 0:
-        raise NotImplementedError(f"{what}: K {k} must be a multiple of 16 below {_MAX_K} (N {n})")
+    if k % 16 or not 0 < k < _MAX_K or not 0 < n <= _MAX_N:
+        raise NotImplementedError(f"{what}: K {k} must be a multiple of 16 below {_MAX_K}, N {n} up to {_MAX_N}")
     bias_code = 0
     if bias is not None:
         if bias.dim() != 1 or bias.shape[0] != n:
