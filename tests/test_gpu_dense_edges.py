@@ -261,6 +261,39 @@ def test_a_node_called_by_hand(check):
             node(wrong)
 
 
+@pytest.mark.parametrize("check", [False, True])
+@pytest.mark.parametrize("reentrant", [False, True])
+def test_under_activation_checkpoints(check, reentrant):
+    """Recomputed in the backward pass (which ends a recomputation early by raising inside a pack hook)."""
+    from torch.utils.checkpoint import checkpoint
+    ops = block(40, 128, 72, BF16, grad=True)
+    dy = randn(40, 128, seed=4).to(BF16)
+
+    def two(x, wg, wu, wd):
+        return vb.gated_ffn(vb.gated_ffn(x, wg, wu, wd, check=check), wg, wu, wd, check=check)
+
+    want = torch.autograd.grad(two(*ops), ops, dy)
+    checkpoint(two, *ops, use_reentrant=reentrant).backward(dy)
+    assert all(torch.equal(t.grad, w) for t, w in zip(ops, want))
+
+
+def test_an_exception_of_a_hook_comes_through():
+    class Stop(Exception):
+        pass
+
+    def pack(_t):
+        raise Stop
+
+    ops = block(4, 64, 40, BF16, grad=True)
+    for check in (False, True):
+        with pytest.raises(Stop), torch.autograd.graph.saved_tensors_hooks(pack, lambda t: t):
+            vb.gated_ffn(*ops, check=check)
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, pack):
+            y = vb.gated_ffn(*ops, check=check)
+        with pytest.raises(Stop):
+            y.sum().backward()
+
+
 def test_out_counts_as_a_write():
     """A tensor that a backward pass still needs and that then receives a result through out= is
     noticed, as for torch's own out=; an out that requires gradients is refused."""
@@ -310,3 +343,84 @@ def test_views_with_the_negative_bit():
     assert torch.equal(a, c) and torch.equal(b, c)
     with pytest.raises(ValueError, match="out"):
         vb.gated_ffn(x, wg, wu, wd, out=neg(torch.zeros_like(x)))
+
+
+# ── two-part hidden rows ─────────────────────────────────────────────────────────────────────
+
+
+@pytest.mark.parametrize("tokens,hidden,inter", [(1, 1024, 512), (3, 520, 264), (16, 512, 1032), (32, 1024, 512),
+                                                 (33, 1024, 512)])
+@pytest.mark.parametrize("dtype,act", [(BF16, "silu"), (F16, "gelu_tanh"), (BF16, "gelu_tanh")])
+def test_hidden_rows_in_two_parts_up_to_32_tokens(tokens, hidden, inter, dtype, act):
+    """Up to 32 tokens h, dg and du go through their products as a sum of two 16-bit values, so the
+    results carry the rounding of the result alone.
+
+    e is the RMS error against 64 bits, e0 that of the 64-bit results rounded once.  Two parts keep
+    2^-16 (bf16) or better, fp32 sums 2^-19 of their terms: less than a tenth of the rounding's RMS
+    (u / 2), so e <= sqrt(1 + 0.1^2) e0 < 1.05 e0.  One part adds an error of the rounding's own size:
+    sqrt(2) e0, which the 64-bit forms on rounded h, dg and du show to be over 1.2 e0 at these sizes."""
+    ops = block(tokens, hidden, inter, dtype, grad=True)
+    dy = randn(tokens, hidden, seed=7).to(dtype)
+    y = vb.gated_ffn(*ops, act=act)
+    got = [y.detach(), *torch.autograd.grad(y, ops, dy)]
+
+    x, wg, wu, wd = (t.detach().double() for t in ops)
+    a, da = R.act_and_slope(x @ wg.T, act)
+    up, dh = x @ wu.T, dy.double() @ wd
+    exact_rows = (a * up, dh * up * da, dh * a)
+
+    def results(h, dg, du):
+        return [h @ wd.T, dg @ wg + du @ wu, dg.T @ x, du.T @ x, dy.double().T @ h]
+
+    def rms(t):
+        return t.pow(2).mean().sqrt().item()
+
+    exact = results(*exact_rows)
+    one_part = results(*(t.to(dtype).double() for t in exact_rows))
+    for name, g, v, p in zip(("y", "dx", "dw_gate", "dw_up", "dw_down"), got, exact, one_part):
+        e0 = rms(v.to(dtype).double() - v)
+        assert rms(p.to(dtype).double() - v) > 1.2 * e0, name
+        e = rms(g.double() - v)
+        assert e <= (1.05 if tokens <= 32 else 1.6) * e0, f"{name}: {e / e0:.3f} times the rounding's error"
+
+
+# ── sizes and ranges ─────────────────────────────────────────────────────────────────────────
+
+
+def test_gradients_of_more_values_than_32_bits_count():
+    """2.2e9 intermediate values: offsets of g and u, dg, du and h pass 2^31.  Only some rows of dy are
+    not zero, so the weight gradients are theirs alone."""
+    tokens, hidden, inter = 140_000, 16, 16_384
+    ops = block(tokens, hidden, inter, BF16, grad=True)
+    rows = torch.tensor([0, 1, 70_000, 131_071, 131_072, 139_998, 139_999], device="cuda")
+    dy = torch.zeros(tokens, hidden, dtype=BF16, device="cuda")
+    dy[rows] = randn(7, hidden, seed=5).to(BF16)
+    y = vb.gated_ffn(*ops)
+    dx, *dws = torch.autograd.grad(y, ops, dy)
+    few = [ops[0].detach()[rows], *(w.detach() for w in ops[1:])]
+    want, bound, parts = R.ffn(*few, "silu", BF16)
+    R.assert_within(y[rows], want, bound, "y")
+    refs = R.ffn_gradients(parts, dy[rows], BF16)
+    R.assert_within(dx[rows], *refs[0], "dx")
+    rest = torch.ones(tokens, dtype=torch.bool, device="cuda")
+    rest[rows] = False
+    assert (dx[rest] == 0).all()
+    for name, g, (v, e) in zip(("dw_gate", "dw_up", "dw_down"), dws, refs[1:]):
+        R.assert_within(g, v, e, name)
+
+
+@pytest.mark.parametrize("tokens", [3, 40, 300])
+def test_fp16_rows_out_of_range_stay_alone(tokens):
+    """h = act(g) u is an fp16 operand of the second product (two up to 32 tokens): beyond 65504 it is
+    infinite and its token's result not finite, though the sum itself would be; no other token changes."""
+    x, wg, wu, wd = block(tokens, 136, 72, F16)
+    want = vb.gated_ffn(x, wg, wu, wd)
+    x = x.clone()
+    x[1] *= 400 / (x[1].float() @ wg.float().T).abs().amax()
+    x[1] = x[1] * 2
+    g, up = x[1].double() @ wg.double().T, x[1].double() @ wu.double().T
+    h = R.act_and_slope(g, "silu")[0] * up
+    assert h.abs().max() > 7e4
+    y = vb.gated_ffn(x, wg, wu, wd)
+    keep = torch.arange(tokens, device="cuda") != 1
+    assert torch.equal(y[keep], want[keep]) and not torch.isfinite(y[1]).any()
