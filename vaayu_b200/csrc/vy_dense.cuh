@@ -10,7 +10,8 @@ namespace vy {
 
 // Both are g times a sigmoid: silu(g) = g s(g), and since (1 + tanh v) / 2 = s(2v), gelu_tanh(g) =
 // g s(2 sqrt(2/pi) (g + 0.044715 g^3)).  One exponential and one approximate division (2 ulp): no
-// branch, so the loads of a tile's other columns are not held up behind it.
+// branch, so the loads of a tile's other columns are not held up behind it.  (The two ulp are far below
+// the 16-bit roundings; in the int8 block they move the codes of h that lie that near to a tie.)
 constexpr double kGeluCubic = 0.044715, kGeluScale = 1.5957691216057308;      // 2 sqrt(2/pi)
 __device__ __forceinline__ float sigmoid(float z) { return __fdividef(1.f, 1.f + expf(-z)); }
 __device__ __forceinline__ float gate_arg(float g, int act) {
@@ -85,8 +86,8 @@ __device__ __forceinline__ void store16_dyn(void* p, int dtype, int64_t at, cons
 // g and u in fp32 between the passes, in the order the tile epilogues move them: blocks of 32 tokens x
 // 16 channels, g before u, each [4 channels][32 tokens][4 channels], so that a warp (a token per lane)
 // reads and writes its chunk of 16 columns as eight whole 512-byte lines.  (One column after another
-// over all tokens, 32 separate 128-byte lines a chunk: 235 us for dh at 2048 x 4096 x 14336, 214
-// this way.)
+// over all tokens, 32 separate 128-byte lines a chunk, took dh at 2048 x 4096 x 14336 235 us beside
+// 214 this way.)
 constexpr int kSavedBlock = 2 * 16 * 32;
 __host__ __device__ constexpr int64_t saved_bands(int64_t tokens) { return (tokens + 31) / 32; }
 __device__ __forceinline__ int64_t saved_at(int64_t bands, int64_t token, int channel) {
@@ -97,7 +98,8 @@ __device__ __forceinline__ int64_t saved_at(int64_t bands, int64_t token, int ch
 // Calls of up to this many tokens keep the hidden row h (and dg, du) as two 16-bit parts, high and low,
 // and run both through the next product: rounding it to one part adds as much error as rounding the
 // result does, and with few tokens the few roundings do not average out.  The products there cost
-// their weights' bytes, so the second part is free.
+// their weights' bytes, so the second part is free.  (Both parts have the type's range: an fp16 h beyond
+// 65504 is infinite.)  With more tokens a second part would double the next products' operations.
 constexpr int kPartTokens = 32;
 template <int ACT>
 __device__ __forceinline__ float low_part(float v) {

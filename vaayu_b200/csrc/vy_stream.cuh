@@ -17,7 +17,8 @@
 // the sums at the end are idle until then and write the token tile's codes themselves, a 16-value
 // piece of a token each per K block, from rows that are still floats.  The rows' largest magnitudes
 // come from the kernel in front, whose every CTA leaves the maximum of the columns it wrote (no
-// atomics, nothing to clear), or, for one or two tokens, are taken over the whole row in place.
+// global atomics, nothing to clear), or, while all rows together are at most 16384 values (one or two
+// tokens of a wide layer, 16 of a small one), are taken over the whole rows in every CTA.
 //
 // A kernel that is not the first of its call starts loading weights before the kernel in front of it
 // has finished (they do not depend on it); its token tiles wait for it.
@@ -29,10 +30,16 @@
 namespace vy {
 
 constexpr int kStreamRows = 128;        // weight rows of a unit (of each matrix)
-// Up to here a product streams its weights; above, the pairs of vy_tile.cuh are faster.  Measured on
-// both (us, stream against pairs): plain products, int8 4096 -> 4096, 128 tokens 11 : 15, 160 tokens
-// 13 : 15, 192 tokens 15 : 15; the gated product (with the same down product behind it), 128 tokens
-// 2048 x 2048 27 : 25, 7168 x 2048 51 : 46, 4096 x 1024 24 : 27, level at 96 tokens.
+// Up to here a product streams its weights; above, the pairs of vy_tile.cuh take it.  Device time in a
+// captured chain, us, stream : pairs.
+//   plain, int8            96 tokens    128        160
+//     4096 -> 4096         10 : 15      12 : 15    14 : 15   (192 tokens: 15 : 15)
+//     14336 -> 4096                     19 : 27    22 : 27
+//     4096 -> 14336        22 : 18      24 : 19    27 : 19   (112 units leave no K shares: no rule yet)
+//   whole bf16 block       64 tokens    96         128 (in brackets what runs: gate on pairs, down streamed)
+//     2048 x 2048          17 : 28      23 : 28    27 : 29 (25)
+//     7168 x 2048          31 : 43      46 : 43    51 : 44 (46)
+//     4096 x 14336         72 : 96      78 : 96    86 : 97 (81)
 constexpr int kStreamMaxGate = 96, kStreamMaxPlain = 160;
 constexpr int kStreamThreads = 192;     // warps 0-3 read the sums, 4 loads, 5 issues the MMAs
 constexpr int kStreamMaxStages = 12;
@@ -74,7 +81,6 @@ struct StreamBars {
     int abort_flag;
 };
 
-// One output value (weight row `row`, token `t`) from its sums.
 // What an output needs besides its sums, fetched while they are still being formed.
 struct ColumnScale {
     float a, b;      // int8: scale of the weight row, and of its up row or its bias
@@ -94,6 +100,7 @@ __device__ __forceinline__ ColumnScale column_scale(const StreamParams& p, int r
     }
     return c;
 }
+// One output value (weight row `row`, token `t`) from its sums.
 template <int EPI, int ACT>
 __device__ __forceinline__ void stream_put(const StreamParams& p, int row, int t, uint32_t s0, uint32_t s1,
                                            const ColumnScale& cs, const float* token_scale, uint32_t* token_top) {
@@ -427,9 +434,14 @@ struct StreamPlan {
 // The most shares (up to 8) whose CTAs are all resident at once: a second round would leave the
 // memory system idle while its CTAs start and join.  Two CTAs run on an SM (and the next kernel's
 // first ones start under this kernel's last) while ring and received sums take half its shared
-// memory.  Up to 32 tokens two stages a CTA are enough for that (16 x 7168 x 2048, bf16: 27.5 us
-// against 32.3 with one deep ring an SM); with more, the token tiles crowd the ring, and one CTA with
-// five stages is faster than two with two (64 x 4096 x 14336: 82 us against 99).
+// memory.  Up to 32 tokens two stages a CTA are enough for that; with more, the token tiles crowd the
+// ring, and one CTA with five stages is faster than two with two.  Half ring against whole, us (the
+// whole one may also leave fewer K shares, since fewer clusters are resident):
+//   bf16 block  1 x 4096 x 14336 57.8 : 61.5   16 x 7168 x 2048 25.2 : 26.6   64 x 4096 x 14336 85.0 : 71.9
+//   int8 block  16 x 7168 x 2048 20.5 : 22.9   8 x 4096 x 14336 42.8 : 48.2
+//   int8        37 x 7168 -> 2048 7.1 : 8.3    64 x 4096 -> 14336 18.4 : 16.4   128 x 4096 -> 14336 23.7 : 20.2
+// (The last two have 112 CTAs for 148 SMs, where the half ring with its three stages is not the better
+// one; the rule does not tell them apart yet.)
 inline StreamPlan stream_plan(int nw, int tokens, int parts, int n, int nk, const ClusterCaps& caps) {
     const int units = (n + kStreamRows - 1) / kStreamRows;
     StreamPlan p{};

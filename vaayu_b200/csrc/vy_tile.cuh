@@ -10,8 +10,9 @@
 // come in segments from several tensors (dx = dg Wg + du Wu).  One launch takes up to four
 // GEMMs, whose tiles fill the machine together.
 //
-// Few tiles.  Pairs are persistent, one for two SMs, and take tiles in turn.  A launch with at most half
-// as many tiles as pairs instead gives each tile a cluster of 2 or 4 pairs, which split its K: every
+// Few tiles.  Pairs are persistent, one for two SMs, and take tiles in turn.  A launch whose tiles can
+// each have a resident cluster of 2 or 4 pairs (33 and 15 such clusters), and whose K leaves a pair
+// kShareLeast blocks or more, instead gives each tile such a cluster, which splits its K: every
 // pair sends each other pair the sums of the columns that one owns, into shared memory, and adds its
 // own columns over all shares in K order.  (Joining through global memory, the last of the pairs adding
 // all shares, measured 59 us where this takes 21 and no split 27: 1003 x 2048 x 768 forward.)
@@ -512,7 +513,11 @@ inline int tile_operand(CUtensorMap* map, int dtype, const void* base, int64_t r
 
 // Lays a launch's problems out (sizes and K blocks set): tile columns, tiles, K shares.  A gated
 // product's tile has bn / 2 output columns.
-constexpr int kShareLeast = 16;      // K blocks a pair's share is worth joining for
+// K blocks a pair's share is worth joining for.  With 16 : 8 : 4, us: forward 512 x 1024 x 1024 17 : 24 : 24,
+// 200 x 2048 x 768 22 : 21 : 24, 200 x 2048 x 2048 29 : 28 : 28, 1003 x 2048 x 768 24 : 24 : 28; int8
+// 300 x 2048 -> 2048 8.7 : 12.2 : 12.3; with gradients 200 x 2048 x 768 58 : 52 : 56, 1003 x 2048 x 768
+// 64 : 61 : 65.  (8 gains little where it gains and loses 40 % where 16 blocks become two shares.)
+constexpr int kShareLeast = 16;
 inline void tile_layout(TileParams* p, bool gate, const ClusterCaps& caps) {
     const int pairs = caps.one[1];
     int least = 1 << 30, wide = 0;

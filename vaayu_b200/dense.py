@@ -14,7 +14,9 @@ front, a shared expert kept in 16 bits, linears in the "int-quantized" 8-bit for
 
 All run on the calling device's current stream, allocate through torch, and never synchronise --
 except `check=True`, which reads the call's device error flags afterwards and raises RuntimeError
-when a device-side wait ran out.  They may be captured in a CUDA graph.
+when a device-side wait ran out (without it such a call's output is unfinished and nobody says so).
+They may be captured in a CUDA graph.  Forward-mode derivatives (dual tensors) are refused; `out=`
+counts as a write to that tensor and is refused where gradients are wanted.
 """
 from __future__ import annotations
 
@@ -306,8 +308,9 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
 
     x [..., hidden]; w_gate, w_up [inter, hidden]; w_down [hidden, inter]; all bf16 or all fp16,
     hidden and inter multiples of 8; act "silu" or "gelu_tanh".  Returns [..., hidden] in x's type
-    (`out`, when given, receives it).  Sums are fp32; h = act(g) * u is rounded once, as the second
-    product's operand.  Differentiable once in x and the weights: with gradients on, the call keeps g
+    (`out`, when given, receives it).  Sums are fp32.  h = act(g) * u is the second product's operand:
+    rounded once to x's type, or up to 32 tokens to a sum of two such values; in fp16 an h beyond 65504
+    is infinite (dg and du likewise), and its token's result not finite.  Differentiable once in x and the weights: with gradients on, the call keeps g
     and u (8 bytes per token and intermediate channel) for the backward pass; `out` is refused then.
     Rows of x may be strided; rows or weights that do not start on 16-byte boundaries are copied."""
     what = "gated_ffn"
