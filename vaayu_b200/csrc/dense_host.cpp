@@ -131,6 +131,7 @@ Tensor backward_operand(const Tensor& t, at::ScalarType type, int device, const 
     TORCH_CHECK(t.is_cuda() && t.get_device() == device && t.scalar_type() == type, "gated_ffn backward: ", what,
                 " is not on cuda:", device, " in ", type);
     TORCH_CHECK_NOT_IMPLEMENTED(!dual(t), "gated_ffn backward: no forward-mode derivatives (", what, " is a dual tensor)");
+    if (t.is_contiguous() && !t.is_neg() && aligned(t)) return t;
     const Tensor c = t.resolve_neg().contiguous();
     return aligned(c) ? c : c.clone();
 }

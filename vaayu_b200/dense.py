@@ -64,6 +64,7 @@ def _host():
     return _HOST
 
 
+_forward_ad = torch.autograd.forward_ad
 _current_device = torch._C._cuda_getDevice
 _raw_stream = torch._C._cuda_getCurrentRawStream
 
@@ -100,7 +101,8 @@ def _activation(act: str, what: str) -> int:
 def _rows(x: torch.Tensor, unit: int) -> tuple:
     """(x as [tokens, width] with rows that start on 16-byte boundaries (`unit` elements), its row
     stride): a view where the strides allow it, else a copy."""
-    x = x.resolve_neg()
+    if x.is_neg():
+        x = x.resolve_neg()
     if x.dim() != 2:
         x = x.reshape(-1, x.shape[-1])
     tokens, width = x.shape
@@ -116,7 +118,8 @@ def _rows(x: torch.Tensor, unit: int) -> tuple:
 
 def _unit_rows(x: torch.Tensor) -> tuple:
     """(x as [tokens, width] with a unit column stride, its row stride)."""
-    x = x.resolve_neg()
+    if x.is_neg():
+        x = x.resolve_neg()
     if x.dim() != 2:
         x = x.reshape(-1, x.shape[-1])
     row, col = x.stride()
@@ -128,7 +131,8 @@ def _unit_rows(x: torch.Tensor) -> tuple:
 
 def _aligned(w: torch.Tensor) -> torch.Tensor:
     """w itself when it is contiguous and starts on a 16-byte boundary, else a copy that does."""
-    w = w.resolve_neg()
+    if w.is_neg():
+        w = w.resolve_neg()
     if not w.is_contiguous():
         return w.contiguous()
     return w.clone() if w.data_ptr() & 15 else w
@@ -198,8 +202,10 @@ def _raise_on(flags: torch.Tensor, what: str) -> None:
 
 def _no_tangents(what: str, *tensors) -> None:
     """Refuses dual tensors: the kernels would drop their tangents, a derivative of zero."""
+    if _forward_ad._current_level < 0:      # no dual tensors now (asked by hand: unpack_dual costs 1 us a tensor)
+        return
     for t in tensors:
-        if t is not None and t.is_floating_point() and torch.autograd.forward_ad.unpack_dual(t).tangent is not None:
+        if t is not None and t.is_floating_point() and _forward_ad.unpack_dual(t).tangent is not None:
             raise NotImplementedError(f"{what}: no forward-mode derivatives (an operand is a dual tensor)")
 
 
@@ -349,11 +355,13 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
 def _cut_off(what: str, out, *tensors) -> bool:
     """Whether gradients are wanted for an operand of a call that has none; its result is then marked
     (`_undifferentiable`) instead of dropping out of the graph without a word."""
-    if not torch.is_grad_enabled() or not any(t is not None and t.requires_grad for t in (*tensors, out)):
-        return False
-    if out is not None:
-        raise RuntimeError(f"{what}: out= with gradients")
-    return True
+    if torch.is_grad_enabled():
+        for t in (out, *tensors):
+            if t is not None and t.requires_grad:
+                if out is not None:
+                    raise RuntimeError(f"{what}: out= with gradients")
+                return True
+    return False
 
 
 def quantize_int8(x: torch.Tensor) -> tuple:
@@ -389,7 +397,8 @@ def quantize_int8(x: torch.Tensor) -> tuple:
 def _scales(scale: torch.Tensor, n: int, what: str) -> torch.Tensor:
     if scale.numel() != n or not scale.is_floating_point():
         raise ValueError(f"{what}: {tuple(scale.shape)} {scale.dtype} scales for {n} rows")
-    scale = scale.resolve_neg()
+    if scale.is_neg():
+        scale = scale.resolve_neg()
     if scale.dtype is not _F32:
         scale = scale.to(_F32)
     return scale if scale.is_contiguous() else scale.contiguous()
